@@ -166,13 +166,15 @@ def stream_ptr():
     return torch.cuda.current_stream().cuda_stream
 
 
-def call(name: str, *args):
-    """Invoke an int-returning entry point; non-zero status -> RuntimeError (ME raises too)."""
+def call(name: str, *args, accept=()):
+    """Invoke an int-returning entry point; non-zero status -> RuntimeError (ME raises too), unless the caller deals with that
+    status itself (accept): then it is returned."""
     if _PENDING:
         join_pending()
     rc = getattr(load(), name)(*args)
-    if rc != 0:
+    if rc != 0 and rc not in accept:
         raise RuntimeError(f"{name} failed ({rc}): {load().lidiff_last_error().decode()}")
+    return rc
 
 
 def require_device(*tensors):

@@ -1908,7 +1908,13 @@ int lidiff_fps_coop(const double* points, int64_t n_points, int64_t n_samples, i
     LIDIFF_CHECK_HIP(hipMemsetAsync(status, 0, 4, st));
     void* args[] = {(void*)&points, (void*)&n_points, (void*)&n_samples, (void*)&pt, (void*)&selected, (void*)&part_val,
                     (void*)&part_idx, (void*)&counter, (void*)&status};
-    LIDIFF_CHECK_HIP(hipLaunchCooperativeKernel((const void*)fps_coop_kernel, dim3(grid), dim3(kFpsBlock), args, 0, st));
+    const hipError_t rc = hipLaunchCooperativeKernel((const void*)fps_coop_kernel, dim3(grid), dim3(kFpsBlock), args, 0, st);
+    if (rc == hipErrorIllegalState || rc == hipErrorCooperativeLaunchTooLarge) {      // another process holds the device's cooperative queue
+        (void)hipGetLastError();
+        set_error("%s: the cooperative launch is not available now (%s): run lidiff_fps", __func__, hipGetErrorString(rc));
+        return 3;
+    }
+    LIDIFF_CHECK_HIP(rc);
     return 0;
 }
 

@@ -1797,14 +1797,16 @@ def farthest_point_sample(points: torch.Tensor, n_samples: int) -> torch.Tensor:
     ws = torch.empty(_lib.load().lidiff_fps_workspace_bytes(n), dtype=torch.uint8, device=pts.device)
     if FPS_COOPERATIVE and _lib.load().lidiff_fps_coop_supported(n):
         # one persistent cooperative launch (device-wide barrier per selection).  Its status word is read back -- the caller
-        # indexes with the result on the host side of the step anyway.  Only a barrier time-out (reported, not silent)
-        # falls back to the launch-per-selection kernel below (same indices); every other failure raises.
+        # indexes with the result on the host side of the step anyway.  A barrier time-out (reported, not silent) and a launch
+        # that the runtime refuses because another process holds the cooperative queue (status 3) fall back to the
+        # launch-per-selection kernel below (same indices); every other failure raises.
         status = torch.empty(1, dtype=torch.int32, device=pts.device)
-        call("lidiff_fps_coop", ptr(pts), n, int(n_samples), ptr(sel), ptr(ws), ptr(status), stream_ptr())
-        if int(status.item()) == 0:
+        refused = call("lidiff_fps_coop", ptr(pts), n, int(n_samples), ptr(sel), ptr(ws), ptr(status), stream_ptr(), accept=(3,))
+        if not refused and int(status.item()) == 0:
             return sel
         import warnings
-        warnings.warn("lidiff_fps_coop: device-wide barrier timed out; re-running the selection with lidiff_fps")
+        warnings.warn("lidiff_fps_coop: the cooperative launch is held by another process; running lidiff_fps" if refused else
+                      "lidiff_fps_coop: device-wide barrier timed out; re-running the selection with lidiff_fps")
     call("lidiff_fps", ptr(pts), n, int(n_samples), ptr(sel), ptr(ws), stream_ptr())
     return sel
 
