@@ -32,6 +32,7 @@ extern "C" {
 #define LIDIFF_STATUS_KEY_RANGE 1   /* *d_status bit: a coordinate left the 16-bit key range */
 #define LIDIFF_STATUS_HASH_FULL 2
                                     /* *d_status bit: hash table too small (cap < 2*rows)     */
+#define LIDIFF_STATUS_BATCH_ORDER 16 /* *d_status bit: rows are not grouped by ascending batch index (lidiff_batch_segments) */
 #define LIDIFF_STATUS_F16_RANGE 8 /* *d_status bit: a value beyond fp16's range (or Inf / NaN) met the two-piece fp16 split (lidiff_split3_rows / lidiff_spconv_fwd_split3 with pieces = 2) */
 #define LIDIFF_STATUS_BOUND 4       /* *d_status bit: a device-side count exceeded the bound the host sized a buffer for (host-read-free
                                        steps, lidiff_tail_map_fill_bounded): nothing was overrun, the results of the step are void */
@@ -509,6 +510,58 @@ int lidiff_nn_dist(const void* a, int64_t n, const void* b, int64_t m, int32_t e
 int64_t lidiff_nn_dist_grid_workspace_bytes(int64_t n, int64_t m, int32_t elem_bytes);
 int lidiff_nn_dist_grid(const void* a, int64_t n, const void* b, int64_t m, int32_t elem_bytes, double cell, void* d2, int64_t* idx,
                         void* workspace, void* stream);
+
+/* ---- scan-wise operators: rows of the same scan share statistics / attend to each other -------------------------------------------
+ * A batch of scans is ONE row matrix; `segments` (device int32 [n_segments][2]) holds the first row and the row behind the last one of
+ * every scan, ascending and disjoint; NULL with n_segments = 1: all rows.  dtype: 0 fp32, 1 bf16, 2 fp16.  Rows of no segment come out
+ * as zeros (outputs and gradients).  No host synchronisation, no allocation, nothing added by atomics across workgroups: the same bits
+ * on every run. */
+
+/* segments of a coordinate map (rows grouped by ascending batch index, coords int32 [rows][4] = (batch, x, y, z)) for `replicas` copies
+ * of its rows stacked behind each other: segments int32 [replicas * n_batches][2], ZEROED by the caller (a batch without rows stays
+ * empty); d_rows: device int32, the valid rows of a map handed over at its bound, or NULL.  Rows out of order or outside
+ * [0, n_batches) raise LIDIFF_STATUS_BATCH_ORDER in *d_status (int32, cleared by the caller). */
+int lidiff_batch_segments(const int32_t* coords, int64_t rows, const int32_t* d_rows, int32_t n_batches, int32_t replicas,
+                          int32_t* segments, int32_t* d_status, void* stream);
+
+/* y = act((x - mean) rstd weight + bias) on x [rows][c] (c a multiple of 4, at most 1024; 16-byte aligned), mean and variance (biased)
+ * over a segment's rows and a group's c / groups channels; weight / bias fp32 [c] or NULL; act: 0 none, 1 relu, 2 silu.
+ * stats: fp32 [n_segments][groups][2] (mean, rstd), kept for the backward pass.  _bwd: dx, and dweight / dbias fp32 [c] (or NULL). */
+int64_t lidiff_group_norm_workspace_bytes(int32_t c, int64_t n_segments);
+int lidiff_group_norm(const void* x, int64_t rows, int32_t c, int32_t groups, int32_t dtype, const int32_t* segments,
+                      int64_t n_segments, const float* weight, const float* bias, float eps, int32_t act, void* y, float* stats,
+                      void* workspace, void* stream);
+int lidiff_group_norm_bwd(const void* x, const void* dy, int64_t rows, int32_t c, int32_t groups, int32_t dtype,
+                          const int32_t* segments, int64_t n_segments, const float* weight, const float* bias, const float* stats,
+                          int32_t act, void* dx, float* dweight, float* dbias, void* workspace, void* stream);
+
+/* out[i] = sum_j softmax_j(q_i . k_j scale + bias) v_j over the keys j of query i's segment (segment s of the queries reads segment s of
+ * the keys; a query without keys gives zeros).  q [mq][heads][dim], k / v [mk][kv_heads][dim] (query head h reads key head
+ * h * kv_heads / heads), dim a multiple of 8 in [8, 128]; strides: HOST int64 array, in elements: q row, q head, k row, k head, v row,
+ * v head (the channels are contiguous; every stride and pointer a multiple of 16 bytes).  out contiguous.
+ * bias_mode: 0 none; 1: -slopes[head] * |c_i - c_j|; 2: table[bucket][head], bucket = edges <= |c_i - c_j|^2 (table fp32
+ * [buckets][heads], buckets <= 48; cells: the look-up table of the edges that ops.bucket_cells builds).  coords_q / coords_k: int32
+ * [rows][4] = (batch, x, y, z); the batch column is not read.
+ * out_f32 (unrounded copy) and lse ([heads][mq]: log2 of the sum of exponentials; +inf without keys) are kept for the backward pass;
+ * either may be NULL.  exact: with a table and 16-bit operands, out_f32 from probabilities of twice the bits (for dtable).  workspace:
+ * may be NULL where workspace_bytes says 0. */
+int64_t lidiff_segment_attention_workspace_bytes(int64_t mq, int64_t mk, int64_t n_segments, int32_t heads, int32_t kv_heads,
+                                                 int32_t dim, int32_t bias_mode);
+int lidiff_segment_attention(const void* q, const void* k, const void* v, const int64_t* strides, const int32_t* coords_q,
+                             const int32_t* coords_k, const int32_t* seg_q, const int32_t* seg_k, int64_t n_segments, int64_t mq,
+                             int64_t mk, int32_t heads, int32_t kv_heads, int32_t dim, int32_t dtype, float scale, int32_t bias_mode,
+                             const float* slopes, const float* table, const void* cells, int32_t buckets, void* out, float* out_f32,
+                             int32_t exact, float* lse, void* workspace, void* stream);
+/* The gradients of the call above, given out_f32 and lse of it.  strides: the six of the forward call, then grad_out row and head.
+ * dq [mq][heads][dim], dk / dv [mk][kv_heads][dim] (both or neither), dtable fp32 [buckets][heads] or NULL. */
+int64_t lidiff_segment_attention_bwd_workspace_bytes(int64_t mq, int64_t mk, int64_t n_segments, int32_t heads, int32_t kv_heads,
+                                                     int32_t dim, int32_t bias_mode, int32_t buckets, int32_t table_grad);
+int lidiff_segment_attention_bwd(const void* q, const void* k, const void* v, const void* grad_out, const int64_t* strides,
+                                 const int32_t* coords_q, const int32_t* coords_k, const int32_t* seg_q, const int32_t* seg_k,
+                                 int64_t n_segments, int64_t mq, int64_t mk, int32_t heads, int32_t kv_heads, int32_t dim,
+                                 int32_t dtype, float scale, int32_t bias_mode, const float* slopes, const float* table,
+                                 const void* cells, int32_t buckets, const float* out_f32, const float* lse, void* dq, void* dk,
+                                 void* dv, float* dtable, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

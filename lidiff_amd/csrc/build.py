@@ -13,10 +13,11 @@ import sys
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = ["coords.hip", "spconv.hip", "spconv_rows.hip", "spconv_bf16.hip", "spconv_split3.hip", "norm.hip", "step.hip", "head.hip"]
+SOURCES = ["coords.hip", "spconv.hip", "spconv_rows.hip", "spconv_bf16.hip", "spconv_split3.hip", "norm.hip", "step.hip", "head.hip",
+           "groupnorm.hip", "attention_fwd.hip", "attention_bwd.hip"]
 # step.hip restates a sequence of separately rounded torch launches: no fused multiply-adds there
 EXTRA_FLAGS = {"step.hip": ["-ffp-contract=off"]}
-HEADERS = ["common.h", "spconv.h", os.path.join("..", "..", "include", "lidiff_amd.h")]
+HEADERS = ["common.h", "spconv.h", "segments.h", "attention.h", os.path.join("..", "..", "include", "lidiff_amd.h")]
 LIB = os.path.join(HERE, "liblidiff_amd.so")
 ARCH = "gfx950"
 # no packed fp32 instructions (v_pk_add / mul / fma_f32): every fp32 operation is its own instruction

@@ -1988,3 +1988,323 @@ def spconv_centre_tail(in_a, w, tmap: TailMap, m_out, **kw):
             rows = spconv_fwd(in_a, w, tmap.nbr, tmap.n, in_b=in_b, replicas=replicas)
         tail = (rows, tmap.ptr, tmap.idx)
     return spconv_fwd(in_a, w, None, m_out, tail=tail, offset=13, **kw)
+
+
+# ----------------------------------------------------------------------------------------
+# scan-wise operators: group normalisation, attention within a scan (groupnorm.hip, attention_*.hip)
+# ----------------------------------------------------------------------------------------
+STATUS_BATCH_ORDER = 16   # rows of a coordinate map are not grouped by ascending batch index (batch_segments)
+_ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2}
+_BIAS_NONE, _BIAS_SLOPES, _BIAS_TABLE = 0, 1, 2
+MAX_BUCKETS = 48
+MAX_EDGE = 1 << 22        # squared distances are exact in fp32 far beyond this (2^24)
+_CELL_BITS = 5            # kCellBits of attention.h
+
+
+def batch_segments(coords: torch.Tensor, n_batches: int | None = None, d_rows: torch.Tensor | None = None, replicas: int = 1,
+                   status: torch.Tensor | None = None) -> torch.Tensor:
+    """Row ranges of the scans of a coordinate map (rows grouped by ascending batch index): int32 [replicas * n_batches, 2], first
+    row and the row behind the last one; a batch without rows is an empty range.  n_batches=None reads the number of batches from
+    the device (one host read, which also raises ValueError for rows out of order); otherwise nothing is read back and rows out of
+    order raise STATUS_BATCH_ORDER in `status`.  d_rows: the number of valid rows of a map handed over at its bound.  replicas:
+    that many copies of the rows stacked behind each other (a guidance pair)."""
+    if coords.dtype != torch.int32 or coords.dim() != 2 or coords.shape[1] != 4:
+        raise ValueError("coords must be int32 [rows, 4] = (batch, x, y, z)")
+    if replicas < 1 or (n_batches is not None and n_batches < 1):
+        raise ValueError("batch_segments needs at least one batch and one replica")
+    if d_rows is not None and (d_rows.dtype != torch.int32 or d_rows.numel() != 1):
+        raise ValueError("d_rows must be one int32 on the device")
+    _same_device(coords.device, d_rows=d_rows, status=status)
+    require_device(coords)
+    coords = coords.contiguous()
+    rows = coords.shape[0]
+    read = n_batches is None
+    if read:
+        valid = coords if d_rows is None else coords[:int(d_rows.item())]
+        n_batches = int(valid[:, 0].max().item()) + 1 if valid.shape[0] else 1
+        if n_batches < 1:
+            raise ValueError("batch indices must not be negative")
+    with torch.cuda.device(coords.device):
+        seg = torch.zeros((replicas * n_batches, 2), dtype=torch.int32, device=coords.device)
+        if status is None:
+            status = torch.zeros(1, dtype=torch.int32, device=coords.device)
+        call("lidiff_batch_segments", ptr(coords), rows, ptr(d_rows), int(n_batches), int(replicas), ptr(seg), ptr(status), stream_ptr())
+    if read and int(status.item()) & STATUS_BATCH_ORDER:
+        raise ValueError("rows are not grouped by ascending batch index")
+    return seg
+
+
+def _check_segments(name: str, seg, device):
+    if seg is None:
+        return
+    if seg.dtype != torch.int32 or seg.dim() != 2 or seg.shape[1] != 2 or seg.shape[0] < 1:
+        raise ValueError(f"{name} must be int32 [scans, 2] = (first row, row behind the last)")
+    if seg.device != device:
+        raise ValueError(f"{name} is on {seg.device}, the rows are on {device}")
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+class _GroupNorm(torch.autograd.Function):
+    """Group normalisation + activation of rows [M, C] per scan (groupnorm.hip)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, segments, groups, eps, act):
+        x = _aligned(x)
+        m, c = x.shape
+        n_seg = 1 if segments is None else segments.shape[0]
+        w = None if weight is None else _aligned(weight.detach().float())
+        b = None if bias is None else _aligned(bias.detach().float())
+        y = torch.empty_like(x)
+        stats = torch.empty((n_seg, groups, 2), dtype=torch.float32, device=x.device)
+        if m:
+            ws = torch.empty(_lib.load().lidiff_group_norm_workspace_bytes(c, n_seg), dtype=torch.uint8, device=x.device)
+            call("lidiff_group_norm", ptr(x), m, c, groups, _ROW_DTYPES[x.dtype], ptr(segments), n_seg, ptr(w), ptr(b), float(eps),
+                 act, ptr(y), ptr(stats), ptr(ws), stream_ptr())
+        ctx.save_for_backward(x, weight, bias, segments, stats)
+        ctx.args = (groups, act)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, segments, stats = ctx.saved_tensors
+        groups, act = ctx.args
+        m, c = x.shape
+        dev = x.device
+        need_w, need_b = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
+        dx = torch.empty_like(x)
+        new = torch.empty if m else torch.zeros
+        dw = new(c, dtype=torch.float32, device=dev) if need_w else None
+        db = new(c, dtype=torch.float32, device=dev) if need_b else None
+        if m:
+            with torch.cuda.device(dev):
+                n_seg = stats.shape[0]
+                dy = _aligned(dy)
+                w = None if weight is None else _aligned(weight.detach().float())
+                b = None if bias is None else _aligned(bias.detach().float())
+                ws = torch.empty(_lib.load().lidiff_group_norm_workspace_bytes(c, n_seg), dtype=torch.uint8, device=dev)
+                call("lidiff_group_norm_bwd", ptr(x), ptr(dy), m, c, groups, _ROW_DTYPES[x.dtype], ptr(segments), n_seg, ptr(w), ptr(b),
+                     ptr(stats), act, ptr(dx), ptr(dw), ptr(db), ptr(ws), stream_ptr())
+        return (dx if ctx.needs_input_grad[0] else None, dw.to(weight.dtype) if need_w else None, db.to(bias.dtype) if need_b else None,
+                None, None, None, None)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and on a 16-byte boundary (a copy where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               segments: torch.Tensor | None = None, eps: float = 1e-5, activation: str | None = None) -> torch.Tensor:
+    """act((x - mean) / sqrt(var + eps) * weight + bias) on feature rows x [M, C] (fp32, bf16 or fp16): one mean and (biased) variance
+    per scan and group of C / num_groups channels, taken over the scan's rows -- a scan's result does not depend on what it is
+    batched with.  segments [S, 2] (batch_segments): the scans' row ranges, ascending and disjoint; None: all rows are one scan.
+    Rows of no scan give zeros and get zero gradients.  weight / bias: [C].  activation: None, "relu" or "silu", fused.
+    Statistics and their gradients are summed in double in a fixed order (the same bits on every run)."""
+    if x.dim() != 2 or x.dtype not in _ROW_DTYPES:
+        raise ValueError("group_norm takes rows [M, C] of float32, bfloat16 or float16")
+    c = x.shape[1]
+    if c % 4 or not 4 <= c <= 1024:
+        raise ValueError(f"group_norm takes a multiple of 4 channels up to 1024, got {c}")
+    if num_groups < 1 or c % num_groups:
+        raise ValueError(f"{num_groups} groups do not divide {c} channels")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be None, 'relu' or 'silu', got {activation!r}")
+    if not 0.0 <= eps < math.inf:
+        raise ValueError("eps must be finite and not negative")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != (c,) or not t.is_floating_point()):
+            raise ValueError(f"{name} must be floating point [{c}]")
+    _same_device(x.device, weight=weight, bias=bias)
+    _check_segments("segments", segments, x.device)
+    require_device(x)
+    with torch.cuda.device(x.device):
+        return _GroupNorm.apply(x, weight, bias, None if segments is None else segments.contiguous(), int(num_groups), float(eps),
+                                _ACTIVATIONS[activation])
+
+
+def distance_edges(num_buckets: int, reach: float, unit: float = 1.0) -> tuple[int, ...]:
+    """Squared distances at which the next of `num_buckets` distance buckets begins: one bucket per `unit` (the tensor stride of the
+    coordinate map) for the first half of them, then evenly in the logarithm up to `reach` units; everything farther is the last
+    bucket.  For segment_attention(edges=...)."""
+    if not 1 <= num_buckets <= MAX_BUCKETS:
+        raise ValueError(f"1 to {MAX_BUCKETS} buckets, got {num_buckets}")
+    near = num_buckets // 2
+    far = num_buckets - 1 - near
+    if num_buckets > 1 and (unit <= 0 or (far and not reach > max(near, 1))):
+        raise ValueError("reach must lie beyond the buckets of one unit, unit must be positive")
+    marks = [float(i) for i in range(1, near + 1)] + [max(near, 1) * (reach / max(near, 1)) ** (i / far) for i in range(1, far + 1)]
+    edges = tuple(math.ceil((unit * r) ** 2) for r in marks)
+    bucket_cells(edges)          # (refuses what the kernels' look-up table cannot hold)
+    return edges
+
+
+def _cell_of(d2: int) -> int:
+    bits = int(torch.tensor(float(d2), dtype=torch.float32).view(torch.int32))
+    return min(max((bits >> (23 - _CELL_BITS)) - ((127 << _CELL_BITS) - 1), 0), (22 << _CELL_BITS) + 1)
+
+
+def bucket_cells(edges: tuple[int, ...]) -> torch.Tensor:
+    """The kernels' look-up table of ascending squared-distance edges (host tensor int32 [cells, 2] = fp32 bits of the edge inside the
+    cell, bucket in front of it; AtCell of attention.h): the leading bits of a squared distance name a cell, and a cell may hold one
+    edge only."""
+    edges = tuple(edges)
+    if not all(isinstance(e, int) and 1 <= e <= MAX_EDGE for e in edges) or any(b <= a for a, b in zip(edges, edges[1:])):
+        raise ValueError(f"edges must be ascending whole squared distances in [1, {MAX_EDGE}]")
+    cells = [_cell_of(e) for e in edges]
+    if len(set(cells)) != len(cells):
+        raise ValueError("two edges are closer than 1/32 of their squared distance")
+    n = (22 << _CELL_BITS) + 2
+    at = torch.arange(n)
+    bucket = (at[:, None] > torch.tensor(cells, dtype=torch.int64)[None, :]).sum(1) if cells else torch.zeros(n, dtype=torch.int64)
+    edge = torch.full((n,), math.inf, dtype=torch.float32)
+    if cells:
+        edge[torch.tensor(cells)] = torch.tensor(edges, dtype=torch.float32)
+    return torch.stack([edge.view(torch.int32), bucket.to(torch.int32)], 1).contiguous()
+
+
+_BUCKET_CELLS: dict = {}      # (edges, device) -> the table on the device: a constant of the configuration, built once per device
+
+
+def _device_cells(edges: tuple[int, ...], device) -> torch.Tensor:
+    key = (edges, device)
+    hit = _BUCKET_CELLS.get(key)
+    if hit is None:
+        hit = _BUCKET_CELLS[key] = bucket_cells(edges).to(device)       # (a copy from pageable memory: complete when it returns)
+    return hit
+
+
+def _heads_rows(t: torch.Tensor) -> torch.Tensor:
+    """[M, H, D] as the kernels read it: channels contiguous, every row and head on a 16-byte boundary (a copy where it is not)."""
+    piece = 16 // t.element_size()
+    if t.stride(2) == 1 and t.stride(0) % piece == 0 and t.stride(1) % piece == 0 and t.data_ptr() % 16 == 0 and min(t.stride()) >= 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(*tensors):
+    import ctypes
+    flat = [s for t in tensors for s in (t.stride(0), t.stride(1))]
+    return (ctypes.c_int64 * len(flat))(*flat)
+
+
+class _SegmentAttention(torch.autograd.Function):
+    """Attention within a scan with a distance bias (attention_fwd.hip, attention_bwd.hip)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, seg_q, seg_k, coords_q, coords_k, slopes, edges, scale):
+        q, k, v = _heads_rows(q), _heads_rows(k), _heads_rows(v)
+        (mq, heads, dim), (mk, kv_heads, _) = q.shape, k.shape
+        dev = q.device
+        grads = any(ctx.needs_input_grad[:4])
+        mode = _BIAS_TABLE if table is not None else _BIAS_SLOPES if slopes is not None else _BIAS_NONE
+        tab = None if table is None else _aligned(table.detach().float())
+        cells = None if table is None else _device_cells(edges, dev)
+        n_seg = 1 if seg_q is None else seg_q.shape[0]
+        out = torch.empty((mq, heads, dim), dtype=q.dtype, device=dev)
+        # the backward pass needs the output as it was before its rounding (the rows of the score gradient sum to zero through it)
+        out32 = None if not grads else out if q.dtype == torch.float32 else torch.empty((mq, heads, dim), dtype=torch.float32, device=dev)
+        lse = torch.empty((heads, mq), dtype=torch.float32, device=dev) if grads else None
+        if mq:
+            nbytes = _lib.load().lidiff_segment_attention_workspace_bytes(mq, mk, n_seg, heads, kv_heads, dim, mode)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            call("lidiff_segment_attention", ptr(q), ptr(k), ptr(v), _strides(q, k, v), ptr(coords_q), ptr(coords_k), ptr(seg_q), ptr(seg_k),
+                 n_seg, mq, mk, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], float(scale), mode, ptr(slopes), ptr(tab), ptr(cells),
+                 0 if table is None else table.shape[0], ptr(out), ptr(out32) if out32 is not out else None,
+                 int(table is not None and ctx.needs_input_grad[3]), ptr(lse), ptr(ws), stream_ptr())
+        if grads:
+            ctx.save_for_backward(q, k, v, table, seg_q, seg_k, coords_q, coords_k, slopes, out32, lse)
+            ctx.edges, ctx.scale, ctx.mode = edges, scale, mode
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go):
+        q, k, v, table, seg_q, seg_k, coords_q, coords_k, slopes, out32, lse = ctx.saved_tensors
+        (mq, heads, dim), (mk, kv_heads, _) = q.shape, k.shape
+        dev = q.device
+        need_kv, need_t = ctx.needs_input_grad[1] or ctx.needs_input_grad[2], table is not None and ctx.needs_input_grad[3]
+        with torch.cuda.device(dev):
+            new = torch.empty if mq else torch.zeros
+            dq = torch.empty((mq, heads, dim), dtype=q.dtype, device=dev)
+            dk, dv = (new((mk, kv_heads, dim), dtype=q.dtype, device=dev) if need_kv else None for _ in range(2))
+            dt = new(tuple(table.shape), dtype=torch.float32, device=dev) if need_t else None
+            if mq:
+                go = _heads_rows(go)
+                tab = None if table is None else _aligned(table.detach().float())
+                buckets = 0 if table is None else table.shape[0]
+                n_seg = 1 if seg_q is None else seg_q.shape[0]
+                ws = torch.empty(_lib.load().lidiff_segment_attention_bwd_workspace_bytes(mq, mk, n_seg, heads, kv_heads, dim, ctx.mode, buckets,
+                                                                                         int(need_t)), dtype=torch.uint8, device=dev)
+                call("lidiff_segment_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(go), _strides(q, k, v, go), ptr(coords_q), ptr(coords_k),
+                     ptr(seg_q), ptr(seg_k), n_seg, mq, mk, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], float(ctx.scale), ctx.mode,
+                     ptr(slopes), ptr(tab), ptr(None if table is None else _device_cells(ctx.edges, dev)), buckets, ptr(out32), ptr(lse),
+                     ptr(dq), ptr(dk), ptr(dv), ptr(dt), ptr(ws), stream_ptr())
+        need = ctx.needs_input_grad
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dt.to(table.dtype) if need_t else None) + (None,) * 7
+
+
+def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seg_q: torch.Tensor | None = None,
+                      seg_k: torch.Tensor | None = None, *, coords_q: torch.Tensor | None = None, coords_k: torch.Tensor | None = None,
+                      slopes: torch.Tensor | None = None, bias: torch.Tensor | None = None, edges: tuple[int, ...] | None = None,
+                      scale: float | None = None) -> torch.Tensor:
+    """Attention of query rows q [Mq, H, D] over the key / value rows k, v [Mk, Hkv, D] of the same scan: seg_q / seg_k [S, 2]
+    (batch_segments) hold the scans' row ranges on both sides, ascending and disjoint; None, None: one scan.  Returns [Mq, H, D]; a
+    query whose scan has no keys, and a row of no scan, gives zeros.  Query head h reads key head h * Hkv // H.  fp32, bf16 or fp16
+    (softmax and sums in fp32); D a multiple of 8 up to 128; scale defaults to 1 / sqrt(D).  Scores may carry a bias that depends on
+    the distance of the two voxels (coords_q / coords_k: int32 [M, 4] = (batch, x, y, z)):
+      slopes [H]            -slopes[h] * |c_i - c_j|, fixed (no gradient)
+      bias [buckets, H]     a learned table: bias[b, h], b = number of `edges` (ascending whole squared distances, one less than
+                            buckets: distance_edges) that |c_i - c_j|^2 reaches
+    Gradients for q, k, v and bias; deterministic.  The backward pass keeps q, k, v, an fp32 copy of the output and one number per
+    query and head -- never the scores."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise ValueError(f"need q [Mq, H, D] and k, v [Mk, Hkv, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in _ROW_DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must share one dtype: float32, bfloat16 or float16")
+    heads, kv_heads, dim = q.shape[1], k.shape[1], q.shape[2]
+    if kv_heads < 1 or heads < 1 or heads > 1024 or heads % kv_heads:
+        raise ValueError(f"{kv_heads} key heads do not divide {heads} query heads")
+    if dim % 8 or not 8 <= dim <= 128:
+        raise ValueError(f"the head dimension must be a multiple of 8 up to 128, got {dim}")
+    dev = q.device
+    _same_device(dev, k=k, v=v, coords_q=coords_q, coords_k=coords_k, slopes=slopes, bias=bias)
+    if (seg_q is None) != (seg_k is None) or (seg_q is not None and seg_q.shape != seg_k.shape):
+        raise ValueError("seg_q and seg_k must name the same scans")
+    _check_segments("seg_q", seg_q, dev)
+    _check_segments("seg_k", seg_k, dev)
+    if slopes is not None and bias is not None:
+        raise ValueError("slopes and a bias table exclude each other")
+    if (bias is None) != (edges is None):
+        raise ValueError("a bias table and its edges come together")
+    if slopes is not None:
+        if slopes.shape != (heads,) or not slopes.is_floating_point():
+            raise ValueError(f"slopes must be floating point [{heads}]")
+        if slopes.requires_grad:
+            raise ValueError("slopes are fixed: no gradient is computed for them (a learned bias is a table)")
+    if bias is not None:
+        edges = tuple(edges)
+        if bias.dim() != 2 or bias.shape[1] != heads or not 1 <= bias.shape[0] <= MAX_BUCKETS or not bias.is_floating_point():
+            raise ValueError(f"the bias table must be floating point [buckets <= {MAX_BUCKETS}, {heads}]")
+        if len(edges) != bias.shape[0] - 1:
+            raise ValueError(f"{bias.shape[0]} buckets have {bias.shape[0] - 1} edges, got {len(edges)}")
+    if slopes is not None or bias is not None:
+        for name, c, m in (("coords_q", coords_q, q.shape[0]), ("coords_k", coords_k, k.shape[0])):
+            if c is None or c.dtype != torch.int32 or c.shape != (m, 4):
+                raise ValueError(f"a distance bias needs {name}: int32 [{m}, 4]")
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    require_device(q)
+    fit = lambda t: None if t is None else _aligned(t)
+    with torch.cuda.device(dev):
+        biased = slopes is not None or bias is not None
+        return _SegmentAttention.apply(q, k, v, bias, fit(seg_q), fit(seg_k), fit(coords_q) if biased else None, fit(coords_k) if biased else None,
+                                       None if slopes is None else _aligned(slopes.float()), edges, scale)
