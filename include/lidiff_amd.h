@@ -537,7 +537,7 @@ int lidiff_group_norm_bwd(const void* x, const void* dy, int64_t rows, int32_t c
 
 /* out[i] = sum_j softmax_j(q_i . k_j scale + bias) v_j over the keys j of query i's segment (segment s of the queries reads segment s of
  * the keys; a query without keys gives zeros).  q [mq][heads][dim], k / v [mk][kv_heads][dim] (query head h reads key head
- * h * kv_heads / heads), dim a multiple of 8 in [8, 128]; strides: HOST int64 array, in elements: q row, q head, k row, k head, v row,
+ * h * kv_heads / heads), dim a multiple of 8 in [8, 128], 1e-6 <= scale <= 1e6; strides: HOST int64 array, in elements: q row, q head, k row, k head, v row,
  * v head (the channels are contiguous; every stride and pointer a multiple of 16 bytes).  out contiguous.
  * bias_mode: 0 none; 1: -slopes[head] * |c_i - c_j|; 2: table[bucket][head], bucket = edges <= |c_i - c_j|^2 (table fp32
  * [buckets][heads], buckets <= 48; cells: the look-up table of the edges that ops.bucket_cells builds).  coords_q / coords_k: int32
@@ -546,7 +546,7 @@ int lidiff_group_norm_bwd(const void* x, const void* dy, int64_t rows, int32_t c
  * either may be NULL.  exact: with a table and 16-bit operands, out_f32 from probabilities of twice the bits (for dtable).  workspace:
  * may be NULL where workspace_bytes says 0. */
 int64_t lidiff_segment_attention_workspace_bytes(int64_t mq, int64_t mk, int64_t n_segments, int32_t heads, int32_t kv_heads,
-                                                 int32_t dim, int32_t bias_mode);
+                                                 int32_t dim, int32_t dtype, int32_t bias_mode);
 int lidiff_segment_attention(const void* q, const void* k, const void* v, const int64_t* strides, const int32_t* coords_q,
                              const int32_t* coords_k, const int32_t* seg_q, const int32_t* seg_k, int64_t n_segments, int64_t mq,
                              int64_t mk, int32_t heads, int32_t kv_heads, int32_t dim, int32_t dtype, float scale, int32_t bias_mode,
@@ -555,7 +555,8 @@ int lidiff_segment_attention(const void* q, const void* k, const void* v, const 
 /* The gradients of the call above, given out_f32 and lse of it.  strides: the six of the forward call, then grad_out row and head.
  * dq [mq][heads][dim], dk / dv [mk][kv_heads][dim] (both or neither), dtable fp32 [buckets][heads] or NULL. */
 int64_t lidiff_segment_attention_bwd_workspace_bytes(int64_t mq, int64_t mk, int64_t n_segments, int32_t heads, int32_t kv_heads,
-                                                     int32_t dim, int32_t bias_mode, int32_t buckets, int32_t table_grad);
+                                                     int32_t dim, int32_t dtype, int32_t bias_mode, int32_t buckets,
+                                                     int32_t table_grad);
 int lidiff_segment_attention_bwd(const void* q, const void* k, const void* v, const void* grad_out, const int64_t* strides,
                                  const int32_t* coords_q, const int32_t* coords_k, const int32_t* seg_q, const int32_t* seg_k,
                                  int64_t n_segments, int64_t mq, int64_t mk, int32_t heads, int32_t kv_heads, int32_t dim,

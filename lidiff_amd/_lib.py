@@ -97,10 +97,10 @@ SIGNATURES = {
     "lidiff_group_norm_workspace_bytes": (_i64, [_i32, _i64]),
     "lidiff_group_norm": (_i32, [_p, _i64, _i32, _i32, _i32, _p, _i64, _p, _p, C.c_float, _i32, _p, _p, _p, _p]),
     "lidiff_group_norm_bwd": (_i32, [_p, _p, _i64, _i32, _i32, _i32, _p, _i64, _p, _p, _p, _i32, _p, _p, _p, _p, _p]),
-    "lidiff_segment_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32, _i32]),
+    "lidiff_segment_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32]),
     "lidiff_segment_attention": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, C.c_float, _i32,
                                         _p, _p, _p, _i32, _p, _p, _i32, _p, _p, _p]),
-    "lidiff_segment_attention_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "lidiff_segment_attention_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "lidiff_segment_attention_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
                                             C.c_float, _i32, _p, _p, _p, _i32, _p, _p, _p, _p, _p, _p, _p, _p]),
 }

@@ -1,93 +1,107 @@
-// Pieces shared by the attention kernels (attention_fwd.hip, attention_bwd.hip): element types, matrix products, distance biases,
-// row tiles in LDS.
+// Pieces shared by the attention kernels (attention_fwd.hip, attention_bwd.hip): operands, matrix products, row tiles in LDS, distance
+// biases.
 //
-// One wave owns 16 "columns" (queries, or keys in the dK / dV kernel) of HG heads at a time and walks over tiles of 64 "rows" of the
-// other side.  A product S = X Y^T with 16 x 16 blocks of v_mfma_f32_16x16x32 leaves in lane l the column l & 15 and the rows
-// 4 (l >> 4) .. + 3 of a block: a column's statistics live in its own lanes, and the block IS (after rounding to the operands' type) half
-// of the B operand of the next product over the rows -- no value crosses a lane.  A contraction may take its terms in any order as long
-// as both operands agree, so rows 32 j + 16 (e / 4) + 4 g + e % 4 are the terms 8 g + e of lane group g of product j.
+// One wave owns 16 or 32 "columns" (queries, or keys in the dk / dv kernel) of HG heads and walks over tiles of "rows" of the other side.
+// A product S = X Y^T in 16 x 16 blocks of v_mfma_f32_16x16x32 leaves in lane l the column l & 15 and the rows 4 (l >> 4) .. + 3 of a
+// block: a column's statistics live in its own lanes, and the block IS (after rounding to the operands' type) half of the B operand of the
+// next product over the rows -- no value crosses a lane.  A contraction may take its terms in any order as long as both operands agree, so
+// rows 32 j + 16 (e / 4) + 4 g + e % 4 are the terms 8 g + e of lane group g = l >> 4 of product j; the A operand with exactly these rows
+// is read from the same row-major tile by the transposing LDS read, so a tile is held once.
 #pragma once
 #include "segments.h"
 
 namespace lidiff {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-struct alignas(16) f32x8 { f32x4 lo, hi; };
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* at_lds_t;
 
 constexpr int kAtBlock = 256;      // 4 waves
-constexpr int kAtRows = 64;        // rows of a tile
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// -- operands -----------------------------------------------------------------------------------------------------------------------
+// fp32 tensors enter the matrix pipe as three bf16 pieces x = x0 + x1 + x2 (exact: 8 + 8 + 8 bits); of the nine products the six that
+// reach 2^-24 |x y| are formed: fp32 accuracy in 6 / 16 of the time of the fp32 matrix instruction.
+// kLift: fp16 ends at 2^-24, where a probability of a long scan may well lie.  Probabilities are multiplied by a power of two before they
+// are rounded to an fp16 operand and the sums divided by it -- exact, and an addend of an exponent that is formed anyway.
+struct AtPieces { bf16x8 p[3]; };
 template <typename T> struct AtType;
-template <> struct AtType<__bf16> { typedef bf16x8 Frag; typedef bf16x4 Quad; static constexpr int kPad = 8; static constexpr int kLift = 0, kPieces = 2; };
-template <> struct AtType<_Float16> { typedef f16x8 Frag; typedef f16x4 Quad; static constexpr int kPad = 8; static constexpr int kLift = 15, kPieces = 2; };
-template <> struct AtType<float> { typedef f32x8 Frag; typedef f32x4 Quad; static constexpr int kPad = 4; static constexpr int kLift = 0, kPieces = 1; };
-// kLift: fp16 ends at 2^-24, where a probability of a long scan may well lie: probabilities are multiplied by 2^15 (at most 32768) before
-// they are rounded to an fp16 operand, and the sums by 2^-15 -- exact, and an addend of the exponent that is there anyway.
+template <> struct AtType<__bf16> { typedef bf16x8 Frag; typedef bf16x4 Quad; typedef __bf16 Elem; static constexpr int kPlanes = 1, kLift = 0; };
+template <> struct AtType<_Float16> { typedef f16x8 Frag; typedef f16x4 Quad; typedef _Float16 Elem; static constexpr int kPlanes = 1, kLift = 15; };
+template <> struct AtType<float> { typedef AtPieces Frag; typedef f32x4 Quad; typedef __bf16 Elem; static constexpr int kPlanes = 3, kLift = 0; };
 
-// acc += A B over 32 terms: lane group g = lane >> 4 holds the terms 8 g .. 8 g + 7 of row (A) / column (B) lane & 15
+// acc += A B over 32 terms: lane group g holds the terms 8 g .. 8 g + 7 of row (A) / column (B) lane & 15
 __device__ __forceinline__ void at_mma(f32x4& acc, const bf16x8& a, const bf16x8& b) { acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0); }
 __device__ __forceinline__ void at_mma(f32x4& acc, const f16x8& a, const f16x8& b) { acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0); }
-__device__ __forceinline__ void at_mma(f32x4& acc, const f32x8& a, const f32x8& b) {      // eight products of four terms, one of each lane group
+__device__ __forceinline__ void at_mma(f32x4& acc, const AtPieces& a, const AtPieces& b) {
+    at_mma(acc, a.p[0], b.p[2]); at_mma(acc, a.p[1], b.p[1]); at_mma(acc, a.p[2], b.p[0]);
+    at_mma(acc, a.p[0], b.p[1]); at_mma(acc, a.p[1], b.p[0]); at_mma(acc, a.p[0], b.p[0]);
+}
+
+// x into its pieces; a value that is not finite goes into the first alone (so that it stays what it is), and one that rounds beyond
+// bf16's largest is cut to it first
+__device__ __forceinline__ void at_split(float x, __bf16& p0, __bf16& p1, __bf16& p2) {
+    const float big = 3.38953139e38f;
+    const bool finite = fabsf(x) < INFINITY;
+    p0 = (__bf16)(finite ? fminf(fmaxf(x, -big), big) : x);
+    const float r = finite ? x - (float)p0 : 0.f;
+    p1 = (__bf16)r;
+    p2 = (__bf16)(r - (float)p1);
+}
+
+// eight consecutive elements of a row as an operand
+__device__ __forceinline__ bf16x8 at_load8(const __bf16* p) { return *reinterpret_cast<const bf16x8*>(p); }
+__device__ __forceinline__ f16x8 at_load8(const _Float16* p) { return *reinterpret_cast<const f16x8*>(p); }
+__device__ __forceinline__ AtPieces at_load8(const float* p) {
+    AtPieces f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.lo[e], b.lo[e], acc, 0, 0, 0);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi[e], b.hi[e], acc, 0, 0, 0);
-}
-
-template <typename T>
-__device__ __forceinline__ typename AtType<T>::Frag at_zero() {
-    return typename AtType<T>::Frag{};
-}
-
-// eight consecutive elements (16 or 32 bytes)
-template <typename T>
-__device__ __forceinline__ typename AtType<T>::Frag at_frag(const T* p) {
-    return *reinterpret_cast<const typename AtType<T>::Frag*>(p);
-}
-template <>
-__device__ __forceinline__ f32x8 at_frag<float>(const float* p) {
-    return f32x8{*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
-}
-
-// a fragment of a transposed tile: four consecutive rows, and the four rows 16 further
-template <typename T>
-__device__ __forceinline__ typename AtType<T>::Frag at_frag_rows(const T* p) {
-    typedef typename AtType<T>::Quad Quad;
-    const Quad lo = *reinterpret_cast<const Quad*>(p), hi = *reinterpret_cast<const Quad*>(p + 16);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-template <>
-__device__ __forceinline__ f32x8 at_frag_rows<float>(const float* p) {
-    return f32x8{*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 16)};
+    for (int e = 0; e < 8; ++e) {
+        __bf16 a, b, c;
+        at_split(p[e], a, b, c);
+        f.p[0][e] = a; f.p[1][e] = b; f.p[2][e] = c;
+    }
+    return f;
 }
 
 // two accumulator blocks (rows 32 j .. + 15 and + 16 .. + 31) as the B operand of the next product.  For 16-bit operands this rounds the
 // probabilities (or their gradients) once, to the type the other operand has: the matrix instruction takes one type.
-__device__ __forceinline__ void at_pack(bf16x8& f, const f32x4& a, const f32x4& b) {
-    typedef float f32x8v __attribute__((ext_vector_type(8)));
-    const f32x8v v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    f = __builtin_convertvector(v, bf16x8);
+__device__ __forceinline__ f32x8 at_join(const f32x4& a, const f32x4& b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ void at_pack(bf16x8& f, const f32x8& v) { f = __builtin_convertvector(v, bf16x8); }
+__device__ __forceinline__ void at_pack(f16x8& f, const f32x8& v) { f = __builtin_convertvector(v, f16x8); }
+__device__ __forceinline__ void at_pack(AtPieces& f, const f32x8& v) {
+    at_pack(f.p[0], v);
+    const f32x8 r = v - __builtin_convertvector(f.p[0], f32x8);
+    at_pack(f.p[1], r);
+    at_pack(f.p[2], r - __builtin_convertvector(f.p[1], f32x8));
 }
-__device__ __forceinline__ void at_pack(f16x8& f, const f32x4& a, const f32x4& b) {
-    typedef float f32x8v __attribute__((ext_vector_type(8)));
-    const f32x8v v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    f = __builtin_convertvector(v, f16x8);
-}
-__device__ __forceinline__ void at_pack(f32x8& f, const f32x4& a, const f32x4& b) { f = f32x8{a, b}; }
-
-// what the rounding of at_pack left (a, b: the values on entry, what is still left on return), as a second operand: two pieces carry 16
-// (bf16) or 22 (fp16) bits; a third one changed the table gradient of 3 10^8 pairs by nothing (1.19e-6 against 1.18e-6)
+// what the rounding of at_pack left, as a second operand: two pieces carry 16 (bf16) or 22 (fp16) bits; a third one changed the table
+// gradient of 3 10^8 pairs by nothing (1.19e-6 against 1.18e-6)
 template <typename F>
-__device__ __forceinline__ void at_pack_rest(F& rest, const F& piece, f32x4& a, f32x4& b) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { a[e] -= (float)piece[e]; b[e] -= (float)piece[4 + e]; }
-    at_pack(rest, a, b);
+__device__ __forceinline__ void at_pack_rest(F& rest, const F& piece, const f32x8& v) {
+    at_pack(rest, v - __builtin_convertvector(piece, f32x8));
 }
+
+// A probability is exp2(s scale2 - base) with one rounding (fma).  Where the base is so large that the rounding of base alone is a factor
+// (|base| > 2^20: differences of such scores are whole powers of two anyway) the product is rounded first, so that the scores the base was
+// formed from give 1.  Returns the factor that is left for the fma.
+constexpr float kHuge = 1048576.f;
+template <int N>
+__device__ __forceinline__ float at_scale(f32x4 (&s)[N], float scale2, bool huge) {
+    if (!huge) return scale2;
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[b][e] = __fmul_rn(s[b][e], scale2);
+    return 1.f;
+}
+__device__ __forceinline__ bool at_huge(float base) { return __any(fabsf(base) > kHuge && fabsf(base) < INFINITY); }
 
 // four consecutive outputs
 template <typename T>
@@ -96,107 +110,187 @@ __device__ __forceinline__ void at_store4(T* p, const f32x4& v) {
     *reinterpret_cast<Quad*>(p) = __builtin_convertvector(v, Quad);
 }
 
+// -- row tiles ------------------------------------------------------------------------------------------------------------------------
+// a tensor as the kernels stream it: rows of DP 16-bit elements; strides in bytes; fp32 tensors come as three planes
+struct AtRows {
+    const char* p;
+    int64_t row, head, plane;
+};
+
+// ROWS rows x SLOTS heads x planes in LDS without padding, 16-byte pieces.  Piece c of a row stands at c ^ swz(row): sixteen rows read at
+// one piece (b128, the A operand as it is) and four rows read at a pair of pieces (the transposing read) each touch every bank alike.
+template <typename T, int DP, int SLOTS, int ROWS>
+struct AtTile {
+    typedef typename AtType<T>::Frag Frag;
+    static constexpr int P = AtType<T>::kPlanes;
+    static constexpr int CH = DP / 8;                                   // pieces of a row
+    static constexpr int RP = CH >= 16 ? 1 : 16 / CH;                   // rows of 256 bytes, the width of the banks
+    static constexpr int N = P * SLOTS * ROWS * CH;
+    static constexpr int kBytes = N * 16;
+    static constexpr int kPlane = SLOTS * ROWS * CH * 16;
+
+    __device__ static __forceinline__ int swz(int row) { return (row / RP) & (CH - 1); }
+
+    // Requests rows [lo, lo + left) of heads h0 .. h0 + SLOTS - 1 straight into LDS (no registers, no waiting: at_arrive()).  The
+    // descriptor ends with the last of these rows and pieces beyond `dim` are addressed out of its range: both arrive as zeros.
+    __device__ static __forceinline__ void request(const AtRows& src, int h0, int dim, int lo, int left, unsigned lds) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
+#pragma unroll
+        for (int n = 0; n < (N + kAtBlock - 1) / kAtBlock; ++n) {
+            const int first = n * kAtBlock + wave * kWave;
+            if (N % kAtBlock && first >= N) break;
+            const int ps = first / (CH * ROWS), slot = ps % SLOTS, plane = ps / SLOTS;
+            const int row = (first + lane) / CH % ROWS, c = (lane % CH) ^ swz(row);
+            const uint64_t base = (uint64_t)(uintptr_t)src.p + (int64_t)lo * src.row + (int64_t)(h0 + slot) * src.head + plane * src.plane;
+            const int voff = c * 8 < dim ? row * (int)src.row + c * 16 : (int)0x80000000;
+            i32x4 rsrc = {(int)(uint32_t)base, (int)(uint32_t)((base >> 32) & 0xffffu), (left - 1) * (int)src.row + dim * 2, 0x00020000};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :: "s"(__builtin_amdgcn_readfirstlane(lds + first * 16)), "v"(voff), "s"(rsrc) : "memory");
+        }
+    }
+
+    // byte offset of lane's part of rows 16 b + (lane & 15), elements 32 c + 8 g ..: the A operand of a product over the elements
+    __device__ static __forceinline__ int at_rows(int slot, int b, int c) {
+        const int lane = lane_id(), row = 16 * b + (lane & 15);
+        return ((slot * ROWS + row) * CH + ((4 * c + (lane >> 4)) ^ swz(row))) * 16;
+    }
+    __device__ static __forceinline__ Frag frag(const char* tile, int off) {
+        if constexpr (P == 1) return *reinterpret_cast<const Frag*>(tile + off);
+        else {
+            Frag f;
+#pragma unroll
+            for (int i = 0; i < P; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(tile + i * kPlane + off);
+            return f;
+        }
+    }
+    // the A operand of a product over rows 32 j ..: elements 16 b + (lane & 15).  Sixteen lanes read four rows of sixteen elements,
+    // lane i row i / 4 and elements 4 (i % 4) .., and receive element i of each row.
+    __device__ static __forceinline__ i16x8 turned(const char* tile, int slot, int j, int b) {
+        const int lane = lane_id(), i = lane & 15, g = lane >> 4;
+        i16x4 r[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int row = 32 * j + 16 * half + 4 * g + i / 4, c = 2 * b + (i % 4) / 2;
+            const char* p = tile + ((slot * ROWS + row) * CH + (c ^ swz(row))) * 16 + (i & 1) * 8;
+            r[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(at_lds_t)p);
+        }
+        return __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    __device__ static __forceinline__ Frag frag_turned(const char* tile, int slot, int j, int b) {
+        if constexpr (P == 1) return __builtin_bit_cast(Frag, turned(tile, slot, j, b));
+        else {
+            Frag f;
+#pragma unroll
+            for (int i = 0; i < P; ++i) f.p[i] = __builtin_bit_cast(bf16x8, turned(tile + i * kPlane, slot, j, b));
+            return f;
+        }
+    }
+};
+
+// every request of this wave has arrived and its LDS accesses are done; then the workgroup meets
+#define AT_ARRIVE() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
+
 // -- distance biases ----------------------------------------------------------------------------------------------------------------
 // kSlope: -slope_h |c_i - c_j|.   kTable: table[bucket][h], bucket = number of edges (squared distances, ascending) <= |c_i - c_j|^2.
 // The squared distance is a sum of squares of integers: exact in fp32 below 2^24, and every edge is at most 2^22.
+// A bias enters a product as the accumulator it starts from, divided by the score's scale.
 enum { kNone = 0, kSlope = 1, kTable = 2 };
 
 // A bucket without a search: the leading bits of the fp32 squared distance (its octave and kCellBits bits behind) name a cell; a cell
-// holds at most one edge (the host checks), so the bucket is the cell's first bucket, plus one behind that edge.
-constexpr int kCellBits = 5;
-constexpr int kCellFirst = 127 << kCellBits;                              // cell of 1.0; squared distance 0 shares the cell in front
+// holds at most one edge (the host checks), so the bucket is the cell's first bucket, plus one behind that edge.  A cell is one word: the
+// bucket in front in the low 8 bits, the edge's remaining bits above (beyond all of them: no edge).
+constexpr int kCellBits = 5, kCellRest = 23 - kCellBits;
+constexpr int kCellFirst = (127 << kCellBits) - 1;                        // 1.0 is cell 1; squared distance 0 is cell 0
 constexpr int kCells = (22 << kCellBits) + 2;                             // 0, then [1, 2^22), then everything from 2^22 on
-struct alignas(8) AtCell { float edge; int bucket; };
-
-__device__ __forceinline__ int at_cell(float d2) {
-    const int c = (__builtin_bit_cast(int, d2) >> (23 - kCellBits)) - (kCellFirst - 1);
-    return min(max(c, 0), kCells - 1);
-}
 
 struct AtBias {
-    const float* table;        // [buckets][H]
-    const AtCell* cells;       // [kCells]
-    const float* slopes;       // [H]
+    const float* table;        // [buckets][heads]
+    const unsigned* cells;     // [kCells]
+    const float* slopes;       // [heads]
     int buckets;
 };
 
-// tiles in LDS: [slot][64][DP + pad] rows as they are, [slot][DP][64 + 4] transposed
-template <typename T, int DP>
-struct AtTile {
-    static constexpr int kRow = DP + AtType<T>::kPad;
-    static constexpr int kCol = kAtRows + 4;
-    static constexpr int kRows = kAtRows * kRow;
-    static constexpr int kCols = DP * kCol;
-};
-
-// rows [lo, lo + 64) of `src` (element strides row / head, first head h0) into registers: 16 bytes a piece, kPieces a thread
-template <typename T, int DP, int SLOTS>
-struct AtLoad {
-    static constexpr int kVec = 16 / (int)sizeof(T);
-    static constexpr int kPerRow = DP / kVec;                          // pieces of a (row, head)
-    static constexpr int kPieces = kAtRows * SLOTS * kPerRow / kAtBlock;
-    static_assert(kAtRows * SLOTS * kPerRow % kAtBlock == 0, "whole pieces per thread");
-    f32x4 r[kPieces];
-
-    __device__ __forceinline__ static void place(int p, int& row, int& slot, int& d) {
-        const int i = p * kAtBlock + threadIdx.x;
-        d = (i % kPerRow) * kVec;
-        slot = (i / kPerRow) % SLOTS;
-        row = i / (kPerRow * SLOTS);
-    }
-    __device__ __forceinline__ void fetch(const T* __restrict__ src, int64_t row_stride, int64_t head_stride, int h0, int dim, int lo, int hi) {
-#pragma unroll
-        for (int p = 0; p < kPieces; ++p) {
-            int row, slot, d;
-            place(p, row, slot, d);
-            r[p] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (lo + row < hi && d < dim) r[p] = *reinterpret_cast<const f32x4*>(src + (int64_t)(lo + row) * row_stride + (int64_t)(h0 + slot) * head_stride + d);
-        }
-    }
-    __device__ __forceinline__ void put_rows(T* __restrict__ dst) const {
-#pragma unroll
-        for (int p = 0; p < kPieces; ++p) {
-            int row, slot, d;
-            place(p, row, slot, d);
-            *reinterpret_cast<f32x4*>(dst + slot * AtTile<T, DP>::kRows + row * AtTile<T, DP>::kRow + d) = r[p];
-        }
-    }
-    __device__ __forceinline__ void put_cols(T* __restrict__ dst) const {
-#pragma unroll
-        for (int p = 0; p < kPieces; ++p) {
-            int row, slot, d;
-            place(p, row, slot, d);
-            union { f32x4 v; T e[kVec]; } u;
-            u.v = r[p];
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) dst[slot * AtTile<T, DP>::kCols + (d + e) * AtTile<T, DP>::kCol + row] = u.e[e];
-        }
-    }
-};
-
-}  // namespace lidiff
-
-namespace lidiff {
-
-// Heads of one wave: the distances of a (query, key) pair are the same for every head, so with a distance bias a wave takes as many heads
-// as the LDS tiles hold (4 x 32 or 2 x 64 elements); they have to be whole groups of one key head, or all have key heads of their own.
-inline int at_heads_per_wave(int dim, int heads, int share, int mode) {
-    const int n = dim <= 32 ? 4 : dim <= 64 ? 2 : 1;
-    return mode != kNone && heads % n == 0 && (share == 1 || share % n == 0) ? n : 1;
+__device__ __forceinline__ int at_bucket(const unsigned* cells, float d2) {
+    const int bits = __builtin_bit_cast(int, d2);
+    const unsigned c = cells[min(max(bits >> kCellRest, kCellFirst), kCellFirst + kCells - 1) - kCellFirst];
+    return (int)(c & 255u) + ((unsigned)(bits & ((1 << kCellRest) - 1)) >= (c >> 8) ? 1 : 0);
 }
 
-inline const char* at_check(int64_t nseg, int64_t mq, int64_t mk, int heads, int kv_heads, int dim, int dtype, int mode, int buckets, const int64_t* strides,
-                            int n_strides) {
+// what the heads of a wave share about four pairs: distances, or buckets
+template <int BIAS>
+struct AtPairs {
+    float d[4];
+    int b[4];
+    __device__ __forceinline__ void form(const float* cs, int rows, int at, float x, float y, float z, const unsigned* cells) {
+        const f32x4 rx = *reinterpret_cast<const f32x4*>(cs + at), ry = *reinterpret_cast<const f32x4*>(cs + rows + at), rz = *reinterpret_cast<const f32x4*>(cs + 2 * rows + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float dx = rx[e] - x, dy = ry[e] - y, dz = rz[e] - z, d2 = dx * dx + dy * dy + dz * dz;
+            if (BIAS == kSlope) d[e] = __builtin_amdgcn_sqrtf(d2);
+            if (BIAS == kTable) b[e] = at_bucket(cells, d2);
+        }
+    }
+    // the accumulator a head's block starts from; slope: -slope / scale, table: this head's column divided by the scale
+    __device__ __forceinline__ f32x4 start(float slope, const float* table) const {
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (BIAS == kSlope) s[e] = slope * d[e];
+            if (BIAS == kTable) s[e] = table[b[e]];
+        }
+        return s;
+    }
+};
+
+inline const char* at_check(int64_t nseg, int64_t mq, int64_t mk, int heads, int kv_heads, int dim, int dtype, float scale, int mode, int buckets,
+                            const int64_t* strides, int n_strides) {
     if (nseg < 1 || nseg > 1 << 20) return "need 1 <= segments <= 2^20";
     if (mq < 1 || mk < 0 || mq > 0x7fffffff - (1 << 22) || mk > 0x7fffffff - (1 << 22)) return "need 1 <= query rows, 0 <= key rows, both below 2^31 - 2^22";
     if (heads < 1 || heads > 1024 || kv_heads < 1 || heads % kv_heads) return "the key heads must divide the query heads (at most 1024)";
     if (dim < 8 || dim > 128 || dim % 8) return "head dimension: a multiple of 8 in [8, 128]";
     if (dtype < 0 || dtype > 2) return "dtype: 0 fp32, 1 bf16, 2 fp16";
+    if (!(scale >= 1e-6f && scale <= 1e6f)) return "need 1e-6 <= scale <= 1e6";
     if (mode < kNone || mode > kTable) return "bias: 0 none, 1 slopes, 2 table";
     if (mode == kTable && (buckets < 1 || buckets > 48)) return "need 1 <= buckets <= 48";
     for (int i = 0; i < n_strides; ++i)
         if (strides[i] < 0 || strides[i] % (dtype == 0 ? 4 : 8)) return "strides must be whole 16-byte pieces";
+    for (int i = 0; i < n_strides; i += 2)
+        if (strides[i] >= 1 << 22) return "a row stride must be below 2^22 elements";
     return nullptr;
+}
+
+// -- fp32 tensors as three bf16 planes [3][rows][heads][dim] -------------------------------------------------------------------------
+inline int64_t at_plane_bytes(int64_t rows, int heads, int dim) { return rows * heads * dim * 2; }
+
+static __global__ __launch_bounds__(256) void at_planes_kernel(const float* __restrict__ src, int64_t row_stride, int64_t head_stride, int64_t rows, int heads, int dim,
+                                                              __bf16* __restrict__ out) {
+    const int quads = dim / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = rows * heads * quads;
+    if (i >= total) return;
+    const int d = (int)(i % quads) * 4, h = (int)(i / quads % heads);
+    const f32x4 v = *reinterpret_cast<const f32x4*>(src + i / quads / heads * row_stride + (int64_t)h * head_stride + d);
+    bf16x4 p[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        __bf16 a, b, c;
+        at_split(v[e], a, b, c);
+        p[0][e] = a; p[1][e] = b; p[2][e] = c;
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x4*>(out + ((int64_t)k * total + i) * 4) = p[k];
+}
+
+// the rows of a tensor as the kernels stream them: as they are, or (fp32) cut into planes at `planes`
+template <typename T>
+static AtRows at_stream(const void* p, int64_t row_stride, int64_t head_stride, int64_t rows, int heads, int dim, void* planes, hipStream_t st) {
+    if constexpr (sizeof(T) == 4) {
+        if (rows > 0)
+            at_planes_kernel<<<(unsigned)ceil_div(rows * heads * (dim / 4), 256), 256, 0, st>>>((const float*)p, row_stride, head_stride, rows, heads, dim, (__bf16*)planes);
+        return AtRows{(const char*)planes, (int64_t)heads * dim * 2, (int64_t)dim * 2, at_plane_bytes(rows, heads, dim)};
+    }
+    return AtRows{(const char*)p, row_stride * 2, head_stride * 2, 0};
 }
 
 }  // namespace lidiff

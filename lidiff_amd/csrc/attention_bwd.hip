@@ -15,14 +15,15 @@ namespace lidiff {
 
 struct AtBwd {
     const void *q, *k, *v, *go;
-    int64_t q_row, q_head, k_row, k_head, v_row, v_head, go_row, go_head;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, go_row, go_head;      // strides in elements
+    AtRows qs, ks, vs, gs;                                    // the same tensors as they are streamed
     const int4 *cq, *ck;
     const int32_t *seg_q, *seg_k;
     int nseg, mq, mk, heads, share, dim;
-    float scale;                                              // as it is (not times log2 e)
+    float scale;
     AtBias bias;
     const float *out32, *lse;                                 // [mq][heads][dim], [heads][mq]
-    float* delta;                                             // [heads][mq]
+    float* stat;                                              // [2][heads][mq]: lse (less kLift) and -delta, for the dk / dv kernel
     void *dq, *dk, *dv;                                       // contiguous
     int splits;                                               // dk / dv: the queries of a scan are shared out over `splits` workgroups
     float* part_kv;                                           // splits > 1: [splits][2][mk][heads / share][dim]
@@ -56,50 +57,65 @@ __global__ __launch_bounds__(256) void at_bound_kernel(const T* __restrict__ src
     if (lane_id() == 0) atomicMax(bound + blockIdx.y / share, __builtin_bit_cast(unsigned, sum));
 }
 
-// one workgroup: 64 queries of one scan x HG heads: dq, delta, and its part of the table's gradient
-template <typename T, int DP, int HG, int SLOTS, int BIAS, bool GRAD>
-__global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
-    typedef AtTile<T, DP> Tile;
-    typedef typename AtType<T>::Frag Frag;
-    constexpr int DC = DP / 32, DB = DP / 16;
-    constexpr bool kLifted = AtType<T>::kLift != 0;
-    extern __shared__ __align__(16) unsigned char at_sm[];
-    T* ks = reinterpret_cast<T*>(at_sm);
-    T* vs = ks + SLOTS * Tile::kRows;
-    T* kt = vs + SLOTS * Tile::kRows;
-    float* cs = reinterpret_cast<float*>(kt + SLOTS * Tile::kCols);
-    float* table = cs + 3 * kAtRows;
-    AtCell* cells = reinterpret_cast<AtCell*>(table + (BIAS == kTable ? ((a.bias.buckets * HG + 3) & ~3) : 0));
-    float* hist = reinterpret_cast<float*>(cells + (BIAS == kTable ? kCells : 0));      // [wave][bucket][HG][64 lanes]: a lane adds to its own word only
+// what a workgroup takes: heads at a time (the distances of a pair are the same for every head), rows of a tile, buffers of it
+template <typename T, int DP> struct AtBwdPlan {
+    static constexpr int kHeads = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 ? 2 : 1;
+    static constexpr int kGradHeads = sizeof(T) == 4 ? 1 : DP == 32 ? 2 : 1;      // with the table's gradient: a histogram of 256 bytes a wave, bucket and head
+    static constexpr int kGradRows = 32;
+    static constexpr int kRows = 64;
+    static constexpr int kBuf = sizeof(T) == 4 ? 1 : 2;
+};
 
-    const int lane = lane_id(), wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+inline int at_bwd_heads(int most, int heads, int share, int mode) {      // whole groups of one key head, or key heads of their own
+    return mode != kNone && heads % most == 0 && (share == 1 || share % most == 0) ? most : 1;
+}
+
+// one workgroup: 64 queries of one scan x HG heads: dq, delta, and its part of the table's gradient
+template <typename T, int DP, int HG, int SLOTS, int BIAS, bool GRAD, int ROWS, int NBUF>
+__global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
+    constexpr int DC = DP / 32, DB = DP / 16;
+    typedef AtTile<T, DP, SLOTS, ROWS> Tile;
+    typedef typename AtType<T>::Frag Frag;
+    constexpr bool kLifted = AtType<T>::kLift != 0;
+    extern __shared__ __align__(16) char at_sm[];
+    char* const ks = at_sm;
+    char* const vs = ks + NBUF * Tile::kBytes;
+    float* const cs = reinterpret_cast<float*>(vs + NBUF * Tile::kBytes);
+    unsigned* const cells = reinterpret_cast<unsigned*>(cs + 2 * 3 * ROWS);
+    float* const table = reinterpret_cast<float*>(cells + (BIAS == kTable ? kCells : 0));
+    float* const hist = table + (BIAS == kTable ? a.bias.buckets * HG : 0);              // [wave][HG][bucket][64 lanes]: a lane adds to words of its own
+    const unsigned ks_at = (unsigned)(uintptr_t)(at_lds_t)ks, vs_at = (unsigned)(uintptr_t)(at_lds_t)vs;
+
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int groups = a.heads / HG, h0 = (blockIdx.x % groups) * HG, kv0 = h0 / a.share, tile_id = blockIdx.x / groups;
-    const SegTile t = find_seg_tile(a.seg_q, a.nseg, a.mq, kAtRows, tile_id);
+    const SegTile t = find_seg_tile(a.seg_q, a.nseg, a.mq, 64, tile_id);
     if (t.lo >= t.hi) {
         if (GRAD)
             for (int i = threadIdx.x; i < HG * a.bias.buckets; i += kAtBlock)
-                a.part_t[((int64_t)tile_id * a.heads + h0 + i / a.bias.buckets) * a.bias.buckets + i % a.bias.buckets] = 0.f;
+                a.part_t[((int64_t)tile_id * a.heads + h0) * a.bias.buckets + i] = 0.f;
         return;
     }
-    const int qi = t.lo + wave * 16 + col;
-    const bool have = qi < t.hi;
     const int2 kr = t.seg >= 0 ? seg_range(a.seg_k, t.seg, a.mk) : make_int2(0, 0);
-    const int tiles = (kr.y - kr.x + kAtRows - 1) / kAtRows;
+    const int k_lo = __builtin_amdgcn_readfirstlane(kr.x), k_hi = __builtin_amdgcn_readfirstlane(kr.y), last = (k_hi - k_lo + ROWS - 1) / ROWS;
+    const int q0 = t.lo + wave * 16, qi = q0 + col;
+    const bool have = qi < t.hi;
     const float scale2 = a.scale * kLog2e;
 
     Frag qf[HG][DC], gf[HG][DC];
-    float lse[HG], delta[HG], slope[HG], unlift[HG];
+    float lse[HG], slope[HG], unlift[HG];
+    bool huge[HG];
+    f32x4 down[HG];                                            // -delta, what the products do . v start from
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
         float sum = 0.f, g2 = 0.f;
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
             const int d = 32 * c + 8 * g;
-            const bool in = have && d < a.dim;
-            qf[h][c] = in ? at_frag((const T*)a.q + (int64_t)qi * a.q_row + (int64_t)(h0 + h) * a.q_head + d) : at_zero<T>();
-            const T* go = (const T*)a.go + (int64_t)qi * a.go_row + (int64_t)(h0 + h) * a.go_head + d;
-            gf[h][c] = in ? at_frag(go) : at_zero<T>();
-            if (in) {
+            qf[h][c] = gf[h][c] = Frag{};
+            if (have && d < a.dim) {
+                const T* go = (const T*)a.go + (int64_t)qi * a.go_row + (int64_t)(h0 + h) * a.go_head + d;
+                qf[h][c] = at_load8((const T*)a.q + (int64_t)qi * a.q_row + (int64_t)(h0 + h) * a.q_head + d);
+                gf[h][c] = at_load8(go);
                 const float* o = a.out32 + ((int64_t)qi * a.heads + h0 + h) * a.dim + d;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -109,9 +125,13 @@ __global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
             }
         }
         sum += __shfl_xor(sum, 16);
-        delta[h] = sum + __shfl_xor(sum, 32);
+        sum += __shfl_xor(sum, 32);
+        down[h] = f32x4{-sum, -sum, -sum, -sum};
         lse[h] = have ? a.lse[(int64_t)(h0 + h) * a.mq + qi] : INFINITY;
-        if (have && g == 0) a.delta[(int64_t)(h0 + h) * a.mq + qi] = delta[h];
+        if (have && g == 0) {
+            a.stat[(int64_t)(h0 + h) * a.mq + qi] = lse[h] - AtType<T>::kLift;
+            a.stat[(int64_t)(a.heads + h0 + h) * a.mq + qi] = -sum;
+        }
         unlift[h] = 1.f;
         if (kLifted) {
             g2 += __shfl_xor(g2, 16);
@@ -121,7 +141,8 @@ __global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
             lse[h] -= lift;                                    // p, and with it ds, carries the power of two
             unlift[h] = __builtin_amdgcn_exp2f(-lift);
         }
-        slope[h] = BIAS == kSlope ? -a.bias.slopes[h0 + h] * kLog2e : 0.f;
+        slope[h] = BIAS == kSlope ? -a.bias.slopes[h0 + h] / a.scale : 0.f;
+        huge[h] = at_huge(lse[h]);
     }
     float qx = 0.f, qy = 0.f, qz = 0.f;
     if (BIAS != kNone && have) {
@@ -129,90 +150,98 @@ __global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
         qx = (float)c.y; qy = (float)c.z; qz = (float)c.w;
     }
     if (BIAS == kTable) {
-        for (int i = threadIdx.x; i < a.bias.buckets * HG; i += kAtBlock) table[i] = a.bias.table[(int64_t)(i / HG) * a.heads + h0 + i % HG] * kLog2e;
+        for (int i = threadIdx.x; i < a.bias.buckets * HG; i += kAtBlock)
+            table[i] = a.bias.table[(int64_t)(i % a.bias.buckets) * a.heads + h0 + i / a.bias.buckets] / a.scale;
         for (int i = threadIdx.x; i < kCells; i += kAtBlock) cells[i] = a.bias.cells[i];
         if (GRAD)
             for (int i = threadIdx.x; i < 4 * a.bias.buckets * HG * 64; i += kAtBlock) hist[i] = 0.f;
     }
-    float* mine = hist + (int64_t)wave * a.bias.buckets * HG * 64 + lane;
+    float* const mine = hist + wave * a.bias.buckets * HG * 64 + lane;
 
-    f32x4 dq[HG][DB] = {};
-    AtLoad<T, DP, SLOTS> kl, vl;
-    int4 kc = make_int4(0, 0, 0, 0);
-    auto fetch = [&](int tile) {
-        const int lo = kr.x + tile * kAtRows;
-        kl.fetch((const T*)a.k, a.k_row, a.k_head, kv0, a.dim, lo, kr.y);
-        vl.fetch((const T*)a.v, a.v_row, a.v_head, kv0, a.dim, lo, kr.y);
-        if (BIAS != kNone && threadIdx.x < kAtRows && lo + (int)threadIdx.x < kr.y) kc = a.ck[lo + threadIdx.x];
+    f32x4 dq[HG][DB];
+#pragma unroll
+    for (int h = 0; h < HG; ++h)
+#pragma unroll
+        for (int b = 0; b < DB; ++b) dq[h][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    int4 kc = make_int4(0, 0, 0, 0);                           // the coordinates one tile further than the requests
+    auto coords = [&](int tile) {
+        const int row = k_lo + tile * ROWS + (int)threadIdx.x;
+        if (BIAS != kNone && tile < last && threadIdx.x < ROWS && row < k_hi) kc = a.ck[row];
     };
-    if (tiles > 0) fetch(0);
-    for (int tile = 0; tile < tiles; ++tile) {
-        __syncthreads();
-        kl.put_rows(ks);
-        kl.put_cols(kt);
-        vl.put_rows(vs);
-        if (BIAS != kNone && threadIdx.x < kAtRows) {
-            cs[threadIdx.x] = (float)kc.y;
-            cs[kAtRows + threadIdx.x] = (float)kc.z;
-            cs[2 * kAtRows + threadIdx.x] = (float)kc.w;
+    auto put_coords = [&](int tile) {
+        if (BIAS == kNone || threadIdx.x >= ROWS) return;
+        float* c = cs + (tile & 1) * 3 * ROWS + threadIdx.x;
+        c[0] = (float)kc.y; c[ROWS] = (float)kc.z; c[2 * ROWS] = (float)kc.w;
+    };
+    auto request = [&](int tile) {
+        const int lo = k_lo + tile * ROWS, left = min(ROWS, k_hi - lo), at = (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
+        Tile::request(a.ks, kv0, a.dim, lo, left, ks_at + at);
+        Tile::request(a.vs, kv0, a.dim, lo, left, vs_at + at);
+    };
+    if (last > 0) {
+        coords(0);
+        put_coords(0);
+        coords(1);
+        request(0);
+    }
+    for (int tile = 0; tile < last; ++tile) {
+        AT_ARRIVE();
+        if (NBUF == 2 && tile + 1 < last) request(tile + 1);
+        if (tile + 1 < last) {
+            put_coords(tile + 1);
+            coords(tile + 2);
         }
-        __syncthreads();
-        if (tile + 1 < tiles) fetch(tile + 1);
-        if (t.lo + wave * 16 >= t.hi) continue;
-        const int left = kr.y - (kr.x + tile * kAtRows);
+        if (q0 < t.hi) {
+            const char* const kt = ks + (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
+            const char* const vt = vs + (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
+            const float* const ct = cs + (tile & 1) * 3 * ROWS;
+            const int left = k_hi - (k_lo + tile * ROWS);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {                          // 32 keys at a time
-            float dist[8];
-            int row_of[8];
-            if (BIAS != kNone) {
+            for (int j = 0; j < ROWS / 32; ++j) {              // 32 keys at a time
+                AtPairs<BIAS> pairs[2];
+                if (BIAS != kNone) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int at = 32 * j + 16 * b + 4 * g;
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(cs + at), y = *reinterpret_cast<const f32x4*>(cs + kAtRows + at),
-                                z = *reinterpret_cast<const f32x4*>(cs + 2 * kAtRows + at);
+                    for (int b = 0; b < 2; ++b) pairs[b].form(ct, ROWS, 32 * j + 16 * b + 4 * g, qx, qy, qz, cells);
+                }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float dx = x[e] - qx, dy = y[e] - qy, dz = z[e] - qz, d2 = dx * dx + dy * dy + dz * dz;
-                        if (BIAS == kSlope) dist[4 * b + e] = __builtin_amdgcn_sqrtf(d2);
-                        if (BIAS == kTable) {
-                            const AtCell c = cells[at_cell(d2)];
-                            row_of[4 * b + e] = c.bucket + (d2 >= c.edge ? 1 : 0);
+                for (int h = 0; h < HG; ++h) {
+                    const int slot = SLOTS == 1 ? 0 : h;
+                    f32x4 s[2], dp[2];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        s[b] = pairs[b].start(slope[h], table + h * a.bias.buckets);
+                        dp[b] = down[h];
+#pragma unroll
+                        for (int c = 0; c < DC; ++c) {
+                            const int at = Tile::at_rows(slot, 2 * j + b, c);
+                            at_mma(s[b], Tile::frag(kt, at), qf[h][c]);
+                            at_mma(dp[b], Tile::frag(vt, at), gf[h][c]);
                         }
                     }
+                    const float factor = at_scale(s, scale2, huge[h]);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float p = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][e], factor, -lse[h]));
+                            if (left < ROWS && 32 * j + 16 * b + 4 * g + e >= left) p = 0.f;
+                            s[b][e] = p * dp[b][e];
+                            if (GRAD)
+                                __hip_atomic_fetch_add(mine + (pairs[b].b[e] + h * a.bias.buckets) * 64, kLifted ? s[b][e] * unlift[h] : s[b][e], __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_WORKGROUP);
+                        }
+                    }
+                    Frag p;
+                    at_pack(p, at_join(s[0], s[1]));
+#pragma unroll
+                    for (int b = 0; b < DB; ++b) at_mma(dq[h][b], Tile::frag_turned(kt, slot, j, b), p);
                 }
             }
-#pragma unroll
-            for (int h = 0; h < HG; ++h) {
-                const int slot = SLOTS == 1 ? 0 : h;
-                f32x4 s[2], dp[2];
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    dp[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int c = 0; c < DC; ++c) {
-                        const int at = slot * Tile::kRows + (32 * j + 16 * b + col) * Tile::kRow + 32 * c + 8 * g;
-                        at_mma(s[b], at_frag(ks + at), qf[h][c]);
-                        at_mma(dp[b], at_frag(vs + at), gf[h][c]);
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float v = s[b][e] * scale2;
-                        if (BIAS == kSlope) v += slope[h] * dist[4 * b + e];
-                        if (BIAS == kTable) v += table[row_of[4 * b + e] * HG + h];
-                        float p = __builtin_amdgcn_exp2f(v - lse[h]);
-                        if (left < kAtRows && 32 * j + 16 * b + 4 * g + e >= left) p = 0.f;
-                        s[b][e] = p * (dp[b][e] - delta[h]);
-                        if (GRAD) __hip_atomic_fetch_add(mine + (row_of[4 * b + e] * HG + h) * 64, s[b][e] * unlift[h], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                    }
-                Frag p;
-                at_pack(p, s[0], s[1]);
-#pragma unroll
-                for (int b = 0; b < DB; ++b) at_mma(dq[h][b], at_frag_rows(kt + slot * Tile::kCols + (16 * b + col) * Tile::kCol + 32 * j + 4 * g), p);
-            }
+        }
+        if (NBUF == 1 && tile + 1 < last) {
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the tile has been read
+            request(tile + 1);
         }
     }
     if (have) {
@@ -225,54 +254,65 @@ __global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
     if (GRAD) {
         __syncthreads();
         for (int i = threadIdx.x; i < HG * a.bias.buckets; i += kAtBlock) {
-            const int b = i / HG, h = i % HG;
             double u = 0;                                      // (the 4 x 64 lanes' sums in a fixed order)
             for (int w = 0; w < 4; ++w)
-                for (int l = 0; l < 64; ++l) u += hist[((w * a.bias.buckets + b) * HG + h) * 64 + ((l + i) & 63)];
-            a.part_t[((int64_t)tile_id * a.heads + h0 + h) * a.bias.buckets + b] = (float)u;
+                for (int l = 0; l < 64; ++l) u += hist[(w * HG * a.bias.buckets + i) * 64 + ((l + i) & 63)];
+            a.part_t[((int64_t)tile_id * a.heads + h0) * a.bias.buckets + i] = (float)u;
         }
     }
 }
 
 // one workgroup: 64 keys of one scan x SLOTS key heads x one share of the queries: dk, dv
-template <typename T, int DP, int HG, int SLOTS, int BIAS>
+template <typename T, int DP, int HG, int SLOTS, int BIAS, int NBUF>
 __global__ __launch_bounds__(kAtBlock) void at_bwd_kv_kernel(const AtBwd a) {
-    typedef AtTile<T, DP> Tile;
+    constexpr int ROWS = 64, DC = DP / 32, DB = DP / 16;
+    typedef AtTile<T, DP, HG, ROWS> Tile;
     typedef typename AtType<T>::Frag Frag;
-    constexpr int DC = DP / 32, DB = DP / 16;
     constexpr bool kLifted = AtType<T>::kLift != 0;
-    extern __shared__ __align__(16) unsigned char at_sm[];
-    T* qs = reinterpret_cast<T*>(at_sm);
-    T* gs = qs + HG * Tile::kRows;
-    T* qt = gs + HG * Tile::kRows;
-    T* gt = qt + HG * Tile::kCols;
-    float* cs = reinterpret_cast<float*>(gt + HG * Tile::kCols);                  // x, y, z, then [HG][64] lse, [HG][64] delta
-    float* ls = cs + 3 * kAtRows;
-    float* ds = ls + HG * kAtRows;
-    float* table = ds + HG * kAtRows;
-    AtCell* cells = reinterpret_cast<AtCell*>(table + (BIAS == kTable ? ((a.bias.buckets * HG + 3) & ~3) : 0));
+    extern __shared__ __align__(16) char at_sm[];
+    char* const qs = at_sm;
+    char* const gs = qs + NBUF * Tile::kBytes;
+    float* const st = reinterpret_cast<float*>(gs + NBUF * Tile::kBytes);          // [NBUF][2][HG][64] lse, -delta
+    float* const cs = st + NBUF * 2 * HG * ROWS;
+    unsigned* const cells = reinterpret_cast<unsigned*>(cs + 2 * 3 * ROWS);
+    float* const table = reinterpret_cast<float*>(cells + (BIAS == kTable ? kCells : 0));
+    const unsigned qs_at = (unsigned)(uintptr_t)(at_lds_t)qs, gs_at = (unsigned)(uintptr_t)(at_lds_t)gs, st_at = (unsigned)(uintptr_t)(at_lds_t)st;
 
-    const int lane = lane_id(), wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int kv_heads = a.heads / a.share, groups = kv_heads / SLOTS, kv0 = (blockIdx.x % groups) * SLOTS, split = blockIdx.y;
-    const SegTile t = find_seg_tile(a.seg_k, a.nseg, a.mk, kAtRows, blockIdx.x / groups);
+    const SegTile t = find_seg_tile(a.seg_k, a.nseg, a.mk, 64, blockIdx.x / groups);
     if (t.lo >= t.hi) return;
-    const int ki = t.lo + wave * 16 + col;
-    const bool have = ki < t.hi;
     const int2 qr = t.seg >= 0 ? seg_range(a.seg_q, t.seg, a.mq) : make_int2(0, 0);
-    const int tiles = (qr.y - qr.x + kAtRows - 1) / kAtRows;
+    const int q_lo = __builtin_amdgcn_readfirstlane(qr.x), q_hi = __builtin_amdgcn_readfirstlane(qr.y), tiles = (q_hi - q_lo + ROWS - 1) / ROWS;
     const int first = (int)((int64_t)tiles * split / a.splits), last = (int)((int64_t)tiles * (split + 1) / a.splits);
+    const int k0 = t.lo + wave * 16, ki = k0 + col;
+    const bool have = ki < t.hi;
     const float scale2 = a.scale * kLog2e;
 
     Frag kf[SLOTS][DC], vf[SLOTS][DC];
+    float ds_lift[SLOTS], dk_unlift[SLOTS];
+    f32x4 dk[SLOTS][DB], dv[SLOTS][DB];
 #pragma unroll
-    for (int h = 0; h < SLOTS; ++h)
+    for (int h = 0; h < SLOTS; ++h) {
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
             const int d = 32 * c + 8 * g;
-            const bool in = have && d < a.dim;
-            kf[h][c] = in ? at_frag((const T*)a.k + (int64_t)ki * a.k_row + (int64_t)(kv0 + h) * a.k_head + d) : at_zero<T>();
-            vf[h][c] = in ? at_frag((const T*)a.v + (int64_t)ki * a.v_row + (int64_t)(kv0 + h) * a.v_head + d) : at_zero<T>();
+            kf[h][c] = vf[h][c] = Frag{};
+            if (have && d < a.dim) {
+                kf[h][c] = at_load8((const T*)a.k + (int64_t)ki * a.k_row + (int64_t)(kv0 + h) * a.k_head + d);
+                vf[h][c] = at_load8((const T*)a.v + (int64_t)ki * a.v_row + (int64_t)(kv0 + h) * a.v_head + d);
+            }
         }
+        ds_lift[h] = dk_unlift[h] = 1.f;
+        if (kLifted) {
+            const float lift = at_lift(__builtin_bit_cast(float, a.bound[kv0 + h]), __builtin_bit_cast(float, a.bound[kv_heads + kv0 + h]));
+            ds_lift[h] = __builtin_amdgcn_exp2f(lift - AtType<T>::kLift);             // (p carries kLift already)
+            dk_unlift[h] = __builtin_amdgcn_exp2f(-lift);
+        }
+#pragma unroll
+        for (int b = 0; b < DB; ++b) dk[h][b] = dv[h][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    constexpr float kUnlift = kLifted ? 1.f / (1 << AtType<T>::kLift) : 1.f;
     float kx = 0.f, ky = 0.f, kz = 0.f;
     if (BIAS != kNone && have) {
         const int4 c = a.ck[ki];
@@ -281,119 +321,106 @@ __global__ __launch_bounds__(kAtBlock) void at_bwd_kv_kernel(const AtBwd a) {
     if (BIAS == kTable)
         for (int i = threadIdx.x; i < kCells; i += kAtBlock) cells[i] = a.bias.cells[i];
 
-    float ds_lift[SLOTS], dk_unlift[SLOTS];
-#pragma unroll
-    for (int h = 0; h < SLOTS; ++h) {
-        ds_lift[h] = dk_unlift[h] = 1.f;
-        if (kLifted) {
-            const float lift = at_lift(__builtin_bit_cast(float, a.bound[kv0 + h]), __builtin_bit_cast(float, a.bound[kv_heads + kv0 + h]));
-            ds_lift[h] = __builtin_amdgcn_exp2f(lift - AtType<T>::kLift);             // (p carries kLift already)
-            dk_unlift[h] = __builtin_amdgcn_exp2f(-lift);
-        }
-    }
-    constexpr float kUnlift = kLifted ? 1.f / (1 << AtType<T>::kLift) : 1.f;
-
-    f32x4 dk[SLOTS][DB] = {}, dv[SLOTS][DB] = {};
     // the query heads that read these key heads, HG at a time
     for (int h0 = kv0 * a.share; h0 < (kv0 + SLOTS) * a.share; h0 += HG) {
-        AtLoad<T, DP, HG> ql, gl;
-        int4 qc = make_int4(0, 0, 0, 0);
-        float lse_r[(HG * kAtRows + kAtBlock - 1) / kAtBlock], delta_r[(HG * kAtRows + kAtBlock - 1) / kAtBlock], slope[HG];
-        auto fetch = [&](int tile) {
-            const int lo = qr.x + tile * kAtRows;
-            ql.fetch((const T*)a.q, a.q_row, a.q_head, h0, a.dim, lo, qr.y);
-            gl.fetch((const T*)a.go, a.go_row, a.go_head, h0, a.dim, lo, qr.y);
-            if (BIAS != kNone && threadIdx.x < kAtRows && lo + (int)threadIdx.x < qr.y) qc = a.cq[lo + threadIdx.x];
+        float slope[HG];
 #pragma unroll
-            for (int p = 0; p < (HG * kAtRows + kAtBlock - 1) / kAtBlock; ++p) {
-                const int i = p * kAtBlock + threadIdx.x, row = lo + i % kAtRows;
-                const bool in = i < HG * kAtRows && row < qr.y;
-                lse_r[p] = in ? a.lse[(int64_t)(h0 + i / kAtRows) * a.mq + row] : INFINITY;       // behind the end: p = 0
-                delta_r[p] = in ? a.delta[(int64_t)(h0 + i / kAtRows) * a.mq + row] : 0.f;
+        for (int h = 0; h < HG; ++h) slope[h] = BIAS == kSlope ? -a.bias.slopes[h0 + h] / a.scale : 0.f;
+        int4 qc = make_int4(0, 0, 0, 0);
+        auto coords = [&](int tile) {
+            const int row = q_lo + tile * ROWS + (int)threadIdx.x;
+            if (BIAS != kNone && tile < last && threadIdx.x < ROWS && row < q_hi) qc = a.cq[row];
+        };
+        auto put_coords = [&](int tile) {
+            if (BIAS == kNone || threadIdx.x >= ROWS) return;
+            float* c = cs + (tile & 1) * 3 * ROWS + threadIdx.x;
+            c[0] = (float)qc.y; c[ROWS] = (float)qc.z; c[2 * ROWS] = (float)qc.w;
+        };
+        auto request = [&](int tile) {
+            const int lo = q_lo + tile * ROWS, left = min(ROWS, q_hi - lo), buf = NBUF == 2 ? tile & 1 : 0;
+            Tile::request(a.qs, h0, a.dim, lo, left, qs_at + buf * Tile::kBytes);
+            Tile::request(a.gs, h0, a.dim, lo, left, gs_at + buf * Tile::kBytes);
+            for (int i = wave; i < 2 * HG; i += 4) {           // lse and -delta: 64 words a head
+                const uint64_t base = (uint64_t)(uintptr_t)(a.stat + ((int64_t)(i / HG) * a.heads + h0 + i % HG) * a.mq + lo);
+                i32x4 rsrc = {(int)(uint32_t)base, (int)(uint32_t)((base >> 32) & 0xffffu), left * 4, 0x00020000};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) rsrc[k] = __builtin_amdgcn_readfirstlane(rsrc[k]);
+                asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                             :: "s"(__builtin_amdgcn_readfirstlane(st_at + (buf * 2 * HG + i) * ROWS * 4)), "v"(lane * 4), "s"(rsrc) : "memory");
             }
         };
-#pragma unroll
-        for (int h = 0; h < HG; ++h) slope[h] = BIAS == kSlope ? -a.bias.slopes[h0 + h] * kLog2e : 0.f;
         __syncthreads();                                       // the chunk of heads before has been read
         if (BIAS == kTable)
-            for (int i = threadIdx.x; i < a.bias.buckets * HG; i += kAtBlock) table[i] = a.bias.table[(int64_t)(i / HG) * a.heads + h0 + i % HG] * kLog2e;
-        if (first < last) fetch(first);
+            for (int i = threadIdx.x; i < a.bias.buckets * HG; i += kAtBlock)
+                table[i] = a.bias.table[(int64_t)(i % a.bias.buckets) * a.heads + h0 + i / a.bias.buckets] / a.scale;
+        if (first < last) {
+            coords(first);
+            put_coords(first);
+            coords(first + 1);
+            request(first);
+        }
         for (int tile = first; tile < last; ++tile) {
-            __syncthreads();
-            ql.put_rows(qs);
-            ql.put_cols(qt);
-            gl.put_rows(gs);
-            gl.put_cols(gt);
-            if (BIAS != kNone && threadIdx.x < kAtRows) {
-                cs[threadIdx.x] = (float)qc.y;
-                cs[kAtRows + threadIdx.x] = (float)qc.z;
-                cs[2 * kAtRows + threadIdx.x] = (float)qc.w;
+            AT_ARRIVE();
+            if (NBUF == 2 && tile + 1 < last) request(tile + 1);
+            if (tile + 1 < last) {
+                put_coords(tile + 1);
+                coords(tile + 2);
             }
+            if (k0 < t.hi) {
+                const int buf = NBUF == 2 ? tile & 1 : 0;
+                const char* const qt = qs + buf * Tile::kBytes;
+                const char* const gt = gs + buf * Tile::kBytes;
+                const float* const lt = st + buf * 2 * HG * ROWS;
+                const float* const ct = cs + (tile & 1) * 3 * ROWS;
+                const int left = q_hi - (q_lo + tile * ROWS);
 #pragma unroll
-            for (int p = 0; p < (HG * kAtRows + kAtBlock - 1) / kAtBlock; ++p) {
-                const int i = p * kAtBlock + threadIdx.x;
-                if (i < HG * kAtRows) { ls[i] = lse_r[p] - AtType<T>::kLift; ds[i] = delta_r[p]; }
-            }
-            __syncthreads();
-            if (tile + 1 < last) fetch(tile + 1);
-            if (t.lo + wave * 16 >= t.hi) continue;
+                for (int j = 0; j < 2; ++j) {
+                    AtPairs<BIAS> pairs[2];
+                    if (BIAS != kNone) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float dist[8];
-                int row_of[8];
-                if (BIAS != kNone) {
+                        for (int b = 0; b < 2; ++b) pairs[b].form(ct, ROWS, 32 * j + 16 * b + 4 * g, kx, ky, kz, cells);
+                    }
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const int at = 32 * j + 16 * b + 4 * g;
-                        const f32x4 x = *reinterpret_cast<const f32x4*>(cs + at), y = *reinterpret_cast<const f32x4*>(cs + kAtRows + at),
-                                    z = *reinterpret_cast<const f32x4*>(cs + 2 * kAtRows + at);
+                    for (int h = 0; h < HG; ++h) {
+                        const int slot = SLOTS == 1 ? 0 : h;
+                        f32x4 s[2], dp[2];
+                        const bool huge = at_huge(lt[h * ROWS + lane]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float dx = x[e] - kx, dy = y[e] - ky, dz = z[e] - kz, d2 = dx * dx + dy * dy + dz * dz;
-                            if (BIAS == kSlope) dist[4 * b + e] = __builtin_amdgcn_sqrtf(d2);
-                            if (BIAS == kTable) {
-                                const AtCell c = cells[at_cell(d2)];
-                                row_of[4 * b + e] = c.bucket + (d2 >= c.edge ? 1 : 0);
+                        for (int b = 0; b < 2; ++b) {
+                            const f32x4 lse = *reinterpret_cast<const f32x4*>(lt + h * ROWS + 32 * j + 16 * b + 4 * g);
+                            s[b] = pairs[b].start(slope[h], table + h * a.bias.buckets);
+                            dp[b] = *reinterpret_cast<const f32x4*>(lt + (HG + h) * ROWS + 32 * j + 16 * b + 4 * g);
+#pragma unroll
+                            for (int c = 0; c < DC; ++c) {
+                                const int at = Tile::at_rows(h, 2 * j + b, c);
+                                at_mma(s[b], Tile::frag(qt, at), kf[slot][c]);
+                                at_mma(dp[b], Tile::frag(gt, at), vf[slot][c]);
+                            }
+                            f32x4 (&one)[1] = reinterpret_cast<f32x4 (&)[1]>(s[b]);
+                            const float factor = at_scale(one, scale2, huge);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float p = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][e], factor, -lse[e]));
+                                if (left < ROWS && 32 * j + 16 * b + 4 * g + e >= left) p = 0.f;
+                                s[b][e] = p;
+                                dp[b][e] = p * dp[b][e];
+                                if (kLifted) dp[b][e] *= ds_lift[slot];
                             }
                         }
-                    }
-                }
+                        Frag p, ds;
+                        at_pack(p, at_join(s[0], s[1]));
+                        at_pack(ds, at_join(dp[0], dp[1]));
 #pragma unroll
-                for (int h = 0; h < HG; ++h) {
-                    const int slot = SLOTS == 1 ? 0 : h;
-                    f32x4 s[2], dp[2];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-                        dp[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int c = 0; c < DC; ++c) {
-                            const int at = h * Tile::kRows + (32 * j + 16 * b + col) * Tile::kRow + 32 * c + 8 * g;
-                            at_mma(s[b], at_frag(qs + at), kf[slot][c]);
-                            at_mma(dp[b], at_frag(gs + at), vf[slot][c]);
-                        }
-                        const f32x4 lse = *reinterpret_cast<const f32x4*>(ls + h * kAtRows + 32 * j + 16 * b + 4 * g),
-                                    delta = *reinterpret_cast<const f32x4*>(ds + h * kAtRows + 32 * j + 16 * b + 4 * g);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float v = s[b][e] * scale2;
-                            if (BIAS == kSlope) v += slope[h] * dist[4 * b + e];
-                            if (BIAS == kTable) v += table[row_of[4 * b + e] * HG + h];
-                            s[b][e] = __builtin_amdgcn_exp2f(v - lse[e]);
-                            dp[b][e] = s[b][e] * (dp[b][e] - delta[e]);
-                            if (kLifted) dp[b][e] *= ds_lift[slot];
+                        for (int b = 0; b < DB; ++b) {
+                            at_mma(dv[slot][b], Tile::frag_turned(gt, h, j, b), p);
+                            at_mma(dk[slot][b], Tile::frag_turned(qt, h, j, b), ds);
                         }
                     }
-                    Frag p, dsf;
-                    at_pack(p, s[0], s[1]);
-                    at_pack(dsf, dp[0], dp[1]);
-#pragma unroll
-                    for (int b = 0; b < DB; ++b) {
-                        const int at = h * Tile::kCols + (16 * b + col) * Tile::kCol + 32 * j + 4 * g;
-                        at_mma(dv[slot][b], at_frag_rows(gt + at), p);
-                        at_mma(dk[slot][b], at_frag_rows(qt + at), dsf);
-                    }
                 }
+            }
+            if (NBUF == 1 && tile + 1 < last) {
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                request(tile + 1);
             }
         }
     }
@@ -439,89 +466,125 @@ __global__ __launch_bounds__(kWave) void at_table_kernel(const float* __restrict
 
 template <typename T, int DP, int HG, int SLOTS, int BIAS, bool GRAD>
 static hipError_t at_bwd_q_launch(const AtBwd& a, hipStream_t st) {
-    typedef AtTile<T, DP> Tile;
-    size_t lds = (size_t)SLOTS * (2 * Tile::kRows + Tile::kCols) * sizeof(T) + 3 * kAtRows * sizeof(float);
-    if (BIAS == kTable) lds += (size_t)((a.bias.buckets * HG + 3) & ~3) * sizeof(float) + kCells * sizeof(AtCell);
+    typedef AtBwdPlan<T, DP> Plan;
+    constexpr int ROWS = GRAD ? Plan::kGradRows : Plan::kRows, NBUF = GRAD ? 1 : Plan::kBuf;
+    size_t lds = (size_t)2 * NBUF * AtTile<T, DP, SLOTS, ROWS>::kBytes + 2 * 3 * ROWS * sizeof(float);
+    if (BIAS == kTable) lds += (kCells + a.bias.buckets * HG) * sizeof(float);
     if (GRAD) lds += (size_t)4 * a.bias.buckets * HG * 64 * sizeof(float);
-    const hipError_t e = hipFuncSetAttribute((const void*)at_bwd_q_kernel<T, DP, HG, SLOTS, BIAS, GRAD>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    auto kern = at_bwd_q_kernel<T, DP, HG, SLOTS, BIAS, GRAD, ROWS, NBUF>;
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return e;
-    at_bwd_q_kernel<T, DP, HG, SLOTS, BIAS, GRAD><<<(unsigned)((int64_t)a.tiles * (a.heads / HG)), kAtBlock, lds, st>>>(a);
+    kern<<<(unsigned)((int64_t)a.tiles * (a.heads / HG)), kAtBlock, lds, st>>>(a);
     return hipGetLastError();
 }
 
 template <typename T, int DP, int HG, int SLOTS, int BIAS>
 static hipError_t at_bwd_kv_launch(const AtBwd& a, hipStream_t st) {
-    typedef AtTile<T, DP> Tile;
-    size_t lds = (size_t)HG * 2 * (Tile::kRows + Tile::kCols) * sizeof(T) + (3 + 2 * HG) * kAtRows * sizeof(float);
-    if (BIAS == kTable) lds += (size_t)((a.bias.buckets * HG + 3) & ~3) * sizeof(float) + kCells * sizeof(AtCell);
-    const hipError_t e = hipFuncSetAttribute((const void*)at_bwd_kv_kernel<T, DP, HG, SLOTS, BIAS>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    constexpr int NBUF = AtBwdPlan<T, DP>::kBuf;
+    size_t lds = (size_t)2 * NBUF * AtTile<T, DP, HG, 64>::kBytes + (NBUF * 2 * HG + 2 * 3) * 64 * sizeof(float);
+    if (BIAS == kTable) lds += (kCells + a.bias.buckets * HG) * sizeof(float);
+    auto kern = at_bwd_kv_kernel<T, DP, HG, SLOTS, BIAS, NBUF>;
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return e;
-    const int64_t wg = seg_tiles_bound(a.mk, kAtRows, a.seg_k, a.nseg) * (a.heads / a.share / SLOTS);
-    at_bwd_kv_kernel<T, DP, HG, SLOTS, BIAS><<<dim3((unsigned)wg, (unsigned)a.splits), kAtBlock, lds, st>>>(a);
+    const int64_t wg = seg_tiles_bound(a.mk, 64, a.seg_k, a.nseg) * (a.heads / a.share / SLOTS);
+    kern<<<dim3((unsigned)wg, (unsigned)a.splits), kAtBlock, lds, st>>>(a);
     if (a.splits > 1)
         at_join_kv_kernel<T><<<(unsigned)ceil_div((int64_t)a.mk * (a.heads / a.share) * a.dim / 4, 256), 256, 0, st>>>(a);
     return hipGetLastError();
 }
 
 template <typename T, int DP, int HG, int SLOTS>
-static hipError_t at_bwd_bias(const AtBwd& a, int mode, hipStream_t st) {
-    hipError_t e = hipErrorInvalidValue;
-    if (mode == kTable && a.part_t) e = at_bwd_q_launch<T, DP, 1, 1, kTable, true>(a, st);      // (the histogram leaves room for one head)
-    else if (mode == kTable) e = at_bwd_q_launch<T, DP, HG, SLOTS, kTable, false>(a, st);
-    else if (mode == kSlope) e = at_bwd_q_launch<T, DP, HG, SLOTS, kSlope, false>(a, st);
-    else if constexpr (HG == 1) e = at_bwd_q_launch<T, DP, HG, SLOTS, kNone, false>(a, st);
-    if (e != hipSuccess || a.dk == nullptr) return e;
+static hipError_t at_bwd_q_bias(const AtBwd& a, int mode, hipStream_t st) {
+    if (mode == kTable) return at_bwd_q_launch<T, DP, HG, SLOTS, kTable, false>(a, st);
+    if (mode == kSlope) return at_bwd_q_launch<T, DP, HG, SLOTS, kSlope, false>(a, st);
+    if constexpr (HG == 1) return at_bwd_q_launch<T, DP, HG, SLOTS, kNone, false>(a, st);
+    return hipErrorInvalidValue;
+}
+
+template <typename T, int DP, int HG, int SLOTS>
+static hipError_t at_bwd_kv_bias(const AtBwd& a, int mode, hipStream_t st) {
     if (mode == kTable) return at_bwd_kv_launch<T, DP, HG, SLOTS, kTable>(a, st);
     if (mode == kSlope) return at_bwd_kv_launch<T, DP, HG, SLOTS, kSlope>(a, st);
     if constexpr (HG == 1) return at_bwd_kv_launch<T, DP, HG, SLOTS, kNone>(a, st);
     return hipErrorInvalidValue;
 }
 
+template <typename T, int DP>
+static hipError_t at_bwd_width(const AtBwd& a, int mode, hipStream_t st) {
+    constexpr int most = AtBwdPlan<T, DP>::kHeads, grad = AtBwdPlan<T, DP>::kGradHeads;
+    const bool wide = most > 1 && at_bwd_heads(most, a.heads, a.share, mode) == most, one = a.share > 1;
+    hipError_t e;
+    if (a.part_t) {
+        e = hipErrorInvalidValue;
+        if constexpr (grad > 1) {
+            if (at_bwd_heads(grad, a.heads, a.share, mode) == grad)
+                e = one ? at_bwd_q_launch<T, DP, grad, 1, kTable, true>(a, st) : at_bwd_q_launch<T, DP, grad, grad, kTable, true>(a, st);
+            else e = at_bwd_q_launch<T, DP, 1, 1, kTable, true>(a, st);
+        } else e = at_bwd_q_launch<T, DP, 1, 1, kTable, true>(a, st);
+    } else if (wide) e = one ? at_bwd_q_bias<T, DP, most, 1>(a, mode, st) : at_bwd_q_bias<T, DP, most, most>(a, mode, st);
+    else e = at_bwd_q_bias<T, DP, 1, 1>(a, mode, st);
+    if (e != hipSuccess || a.dk == nullptr) return e;
+    if (wide) return one ? at_bwd_kv_bias<T, DP, most, 1>(a, mode, st) : at_bwd_kv_bias<T, DP, most, most>(a, mode, st);
+    return at_bwd_kv_bias<T, DP, 1, 1>(a, mode, st);
+}
+
+// Shares of the queries for dk / dv: so many that there are two workgroups of a compute unit each and the last round of them is not a
+// large part of the time, each with at least two tiles of an average scan's queries.
+template <typename T, int DP>
+static int at_bwd_splits(int64_t mq, int64_t mk, int64_t nseg, int heads, int kv_heads, int mode) {
+    const int share = heads / kv_heads, slots = share > 1 ? 1 : at_bwd_heads(AtBwdPlan<T, DP>::kHeads, heads, share, mode);
+    const int64_t wg = (ceil_div(mk > 0 ? mk : 1, 64) + nseg - 1) * (kv_heads / slots);
+    if (wg >= 2048) return 1;
+    const int64_t want = ceil_div(2048, wg), most = ceil_div(mq, nseg) / 128;
+    const int64_t n = want < most ? want : most;
+    return n < 1 ? 1 : (int)(n < 64 ? n : 64);
+}
+
+struct AtBwdLayout { int splits; int64_t bound, q, k, v, go, table, kv, bytes; };      // workspace; the row statistics come first
+
 template <typename T>
-static hipError_t at_bwd_dispatch(const AtBwd& a, int mode, hipStream_t st) {
+static AtBwdLayout at_bwd_layout(int64_t mq, int64_t mk, const void* seg, int64_t nseg, int heads, int kv_heads, int dim, int mode, int buckets, bool table_grad) {
+    auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+    AtBwdLayout l;
+    l.splits = dim <= 32 ? at_bwd_splits<T, 32>(mq, mk, nseg, heads, kv_heads, mode) : dim <= 64 ? at_bwd_splits<T, 64>(mq, mk, nseg, heads, kv_heads, mode)
+                                                                                               : at_bwd_splits<T, 128>(mq, mk, nseg, heads, kv_heads, mode);
+    const int64_t pq = sizeof(T) == 4 ? up(3 * at_plane_bytes(mq, heads, dim)) : 0, pk = sizeof(T) == 4 ? up(3 * at_plane_bytes(mk, kv_heads, dim)) : 0;
+    l.bound = up(2 * mq * heads * (int64_t)sizeof(float));
+    l.q = l.bound + up(2 * kv_heads * (int64_t)sizeof(float));
+    l.go = l.q + pq;
+    l.k = l.go + pq;
+    l.v = l.k + pk;
+    l.table = l.v + pk;
+    l.kv = l.table + (table_grad ? up(seg_tiles_bound(mq, 64, seg, nseg) * heads * buckets * (int64_t)sizeof(float)) : 0);
+    l.bytes = l.kv + (l.splits > 1 ? up(2 * l.splits * mk * kv_heads * dim * (int64_t)sizeof(float)) : 0);
+    return l;
+}
+
+template <typename T>
+static hipError_t at_bwd_run(AtBwd a, const AtBwdLayout& l, int mode, char* ws, hipStream_t st) {
+    const int kv_heads = a.heads / a.share;
     if (AtType<T>::kLift) {
-        const int kv_heads = a.heads / a.share;
         at_bound_clear_kernel<<<(unsigned)ceil_div(2 * kv_heads, 256), 256, 0, st>>>(a.bound, 2 * kv_heads);
         at_bound_kernel<T><<<dim3((unsigned)ceil_div(a.mq, 256), (unsigned)a.heads), 256, 0, st>>>((const T*)a.go, a.go_row, a.go_head, a.mq, a.dim, a.share, a.bound);
         if (a.mk > 0)
             at_bound_kernel<T><<<dim3((unsigned)ceil_div(a.mk, 256), (unsigned)kv_heads), 256, 0, st>>>((const T*)a.v, a.v_row, a.v_head, a.mk, a.dim, 1,
                                                                                                     a.bound + kv_heads);
     }
-    const int hg = at_heads_per_wave(a.dim, a.heads, a.share, mode);
-    const bool one = a.share > 1;
-    if (a.dim <= 32) {
-        if (hg == 4) return one ? at_bwd_bias<T, 32, 4, 1>(a, mode, st) : at_bwd_bias<T, 32, 4, 4>(a, mode, st);
-        return at_bwd_bias<T, 32, 1, 1>(a, mode, st);
+    a.ks = at_stream<T>(a.k, a.k_row, a.k_head, a.mk, kv_heads, a.dim, ws + l.k, st);
+    a.vs = at_stream<T>(a.v, a.v_row, a.v_head, a.mk, kv_heads, a.dim, ws + l.v, st);
+    if (a.dk) {
+        a.qs = at_stream<T>(a.q, a.q_row, a.q_head, a.mq, a.heads, a.dim, ws + l.q, st);
+        a.gs = at_stream<T>(a.go, a.go_row, a.go_head, a.mq, a.heads, a.dim, ws + l.go, st);
     }
-    if (a.dim <= 64) {
-        if (hg == 2) return one ? at_bwd_bias<T, 64, 2, 1>(a, mode, st) : at_bwd_bias<T, 64, 2, 2>(a, mode, st);
-        return at_bwd_bias<T, 64, 1, 1>(a, mode, st);
-    }
-    return at_bwd_bias<T, 128, 1, 1>(a, mode, st);
+    if (a.dim <= 32) return at_bwd_width<T, 32>(a, mode, st);
+    if (a.dim <= 64) return at_bwd_width<T, 64>(a, mode, st);
+    return at_bwd_width<T, 128>(a, mode, st);
 }
 
-// shares of the queries for dk / dv, by the rule of the forward pass
-static int at_bwd_splits(int64_t mq, int64_t mk, int nseg, int kv_heads, int slots) {
-    const int64_t wg = (ceil_div(mk > 0 ? mk : 1, kAtRows) + (nseg > 1 ? nseg - 1 : 0)) * (kv_heads / slots);
-    if (wg >= 512) return 1;
-    const int64_t want = ceil_div(1024, wg), most = ceil_div(mq, nseg) / (4 * kAtRows);
-    const int64_t n = want < most ? want : most;
-    return n < 1 ? 1 : (int)(n < 64 ? n : 64);
-}
-
-static int at_bwd_slots(int heads, int kv_heads, int dim, int mode) {
-    const int share = heads / kv_heads;
-    return share > 1 ? 1 : at_heads_per_wave(dim, heads, share, mode);
-}
-
-// workspace: delta and the bounds, the table's parts, the shares of dk / dv -- each on a 256-byte boundary
-static int64_t at_bwd_layout(int64_t mq, int64_t mk, const void* seg, int64_t nseg, int heads, int kv_heads, int dim, int mode, int buckets, bool table_grad,
-                             int64_t* off_t, int64_t* off_kv) {
-    auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-    *off_t = up((mq * heads + 2 * kv_heads) * (int64_t)sizeof(float));
-    *off_kv = *off_t + (table_grad ? up(seg_tiles_bound(mq, kAtRows, seg, nseg) * heads * buckets * (int64_t)sizeof(float)) : 0);
-    const int s = at_bwd_splits(mq, mk, (int)nseg, kv_heads, at_bwd_slots(heads, kv_heads, dim, mode));
-    return *off_kv + (s > 1 ? up(2 * s * mk * kv_heads * dim * (int64_t)sizeof(float)) : 0);
+static AtBwdLayout at_bwd_layout_of(int dtype, int64_t mq, int64_t mk, const void* seg, int64_t nseg, int heads, int kv_heads, int dim, int mode, int buckets,
+                                    bool table_grad) {
+    return dtype == 0 ? at_bwd_layout<float>(mq, mk, seg, nseg, heads, kv_heads, dim, mode, buckets, table_grad)
+                      : at_bwd_layout<__bf16>(mq, mk, seg, nseg, heads, kv_heads, dim, mode, buckets, table_grad);
 }
 
 }  // namespace lidiff
@@ -529,10 +592,9 @@ static int64_t at_bwd_layout(int64_t mq, int64_t mk, const void* seg, int64_t ns
 using namespace lidiff;
 
 extern "C" int64_t lidiff_segment_attention_bwd_workspace_bytes(int64_t mq, int64_t mk, int64_t n_segments, int32_t heads, int32_t kv_heads, int32_t dim,
-                                                                int32_t bias_mode, int32_t buckets, int32_t table_grad) {
+                                                                int32_t dtype, int32_t bias_mode, int32_t buckets, int32_t table_grad) {
     if (mq < 1 || mk < 0 || n_segments < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 8 || dim > 128) return 0;
-    int64_t t, kv;
-    return at_bwd_layout(mq, mk, &t, n_segments, heads, kv_heads, dim, bias_mode, buckets, table_grad != 0, &t, &kv);      // (segments given: the larger bound)
+    return at_bwd_layout_of(dtype, mq, mk, &mq, n_segments, heads, kv_heads, dim, bias_mode, buckets, table_grad != 0).bytes;      // (with segments: the larger bound)
 }
 
 extern "C" int lidiff_segment_attention_bwd(const void* q, const void* k, const void* v, const void* grad_out, const int64_t* strides,
@@ -542,7 +604,7 @@ extern "C" int lidiff_segment_attention_bwd(const void* q, const void* k, const 
                                             const float* out_f32, const float* lse, void* dq, void* dk, void* dv, float* dtable, void* workspace,
                                             void* stream) {
     LIDIFF_CHECK_ARG(q && grad_out && strides && out_f32 && lse && dq && workspace && (mk == 0 || (k && v)) && (dk != nullptr) == (dv != nullptr), "null pointer");
-    const char* bad = at_check(n_segments, mq, mk, heads, kv_heads, dim, dtype, bias_mode, buckets, strides, 8);
+    const char* bad = at_check(n_segments, mq, mk, heads, kv_heads, dim, dtype, scale, bias_mode, buckets, strides, 8);
     LIDIFF_CHECK_ARG(bad == nullptr, bad);
     LIDIFF_CHECK_ARG((seg_q != nullptr) == (seg_k != nullptr) && (seg_q || n_segments == 1), "segments of queries and keys come together");
     LIDIFF_CHECK_ARG(bias_mode == kNone || (coords_q && (coords_k || mk == 0)), "a distance bias needs the coordinates");
@@ -551,7 +613,7 @@ extern "C" int lidiff_segment_attention_bwd(const void* q, const void* k, const 
     LIDIFF_CHECK_ARG(dtable == nullptr || bias_mode == kTable, "a table gradient without a table");
     LIDIFF_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)grad_out | (uintptr_t)out_f32 | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv |
                        (uintptr_t)coords_q | (uintptr_t)coords_k | (uintptr_t)workspace) & 15) == 0 &&
-                     (((uintptr_t)seg_q | (uintptr_t)seg_k | (uintptr_t)cells) & 7) == 0, "misaligned pointer");
+                     (((uintptr_t)seg_q | (uintptr_t)seg_k) & 7) == 0, "misaligned pointer");
     AtBwd a;
     a.q = q; a.k = k; a.v = v; a.go = grad_out;
     a.q_row = strides[0]; a.q_head = strides[1]; a.k_row = strides[2]; a.k_head = strides[3]; a.v_row = strides[4]; a.v_head = strides[5];
@@ -560,20 +622,20 @@ extern "C" int lidiff_segment_attention_bwd(const void* q, const void* k, const 
     a.seg_q = seg_q; a.seg_k = seg_k; a.nseg = (int)n_segments; a.mq = (int)mq; a.mk = (int)mk;
     a.heads = heads; a.share = heads / kv_heads; a.dim = dim;
     a.scale = scale;
-    a.bias = AtBias{table, (const AtCell*)cells, slopes, buckets};
+    a.bias = AtBias{table, (const unsigned*)cells, slopes, bias_mode == kTable ? buckets : 0};
     a.out32 = out_f32; a.lse = lse;
     a.dq = dq; a.dk = mk > 0 ? dk : nullptr; a.dv = dv;
-    int64_t off_t, off_kv;
-    at_bwd_layout(mq, mk, seg_q, n_segments, heads, kv_heads, dim, bias_mode, buckets, dtable != nullptr, &off_t, &off_kv);
-    a.delta = (float*)workspace;
-    a.bound = (unsigned*)(a.delta + mq * heads);
-    a.part_t = dtable ? (float*)((char*)workspace + off_t) : nullptr;
-    a.part_kv = (float*)((char*)workspace + off_kv);
-    a.tiles = (int)seg_tiles_bound(mq, kAtRows, seg_q, n_segments);
-    a.splits = at_bwd_splits(mq, mk, a.nseg, kv_heads, at_bwd_slots(heads, kv_heads, dim, bias_mode));
+    const AtBwdLayout l = at_bwd_layout_of(dtype, mq, mk, seg_q, n_segments, heads, kv_heads, dim, bias_mode, buckets, dtable != nullptr);
+    char* ws = (char*)workspace;
+    a.stat = (float*)ws;
+    a.bound = (unsigned*)(ws + l.bound);
+    a.part_t = dtable ? (float*)(ws + l.table) : nullptr;
+    a.part_kv = (float*)(ws + l.kv);
+    a.tiles = (int)seg_tiles_bound(mq, 64, seg_q, n_segments);
+    a.splits = l.splits;
     hipStream_t st = (hipStream_t)stream;
-    LIDIFF_CHECK_HIP(dtype == 0 ? at_bwd_dispatch<float>(a, bias_mode, st) : dtype == 1 ? at_bwd_dispatch<__bf16>(a, bias_mode, st)
-                                                                                      : at_bwd_dispatch<_Float16>(a, bias_mode, st));
+    LIDIFF_CHECK_HIP(dtype == 0 ? at_bwd_run<float>(a, l, bias_mode, ws, st) : dtype == 1 ? at_bwd_run<__bf16>(a, l, bias_mode, ws, st)
+                                                                                        : at_bwd_run<_Float16>(a, l, bias_mode, ws, st));
     if (dtable) {
         at_table_kernel<<<(unsigned)(buckets * heads), kWave, 0, st>>>(a.part_t, a.tiles, heads, buckets, dtable);
         LIDIFF_CHECK_LAUNCH();

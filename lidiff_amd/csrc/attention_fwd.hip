@@ -1,18 +1,27 @@
 // Attention between the rows of the same scan, forward: out_i = sum_j softmax_j(q_i . k_j scale + bias_h(|c_i - c_j|)) v_j over the keys j of
-// i's scan (segments.h), in one pass over the keys with a running maximum and sum per query and head.  A query whose scan has no keys,
-// and a row of no scan, gives zeros.
-// Scores are kept in units of log 2 (scale, slopes and table times log2 e), so a probability is one v_exp_f32.
+// i's scan (segments.h), in one pass over the keys with a running base and sum per query and head.  A query whose scan has no keys, and a
+// row of no scan, gives zeros.
+//
+// The base need not be the maximum: it follows a score that exceeds it by more than 8 (in units of log 2), so after the first tiles the
+// sums are almost never rescaled, and the maximum over the lanes of a query is only formed when some lane needs it.  With 16-bit operands
+// the sum of the probabilities comes from the matrix pipe too (a row of ones), of the values that multiply v.
 #include "attention.h"
+
+#ifndef AT_FWD_QB
+#define AT_FWD_QB 1
+#define AT_FWD_BUF 2
+#endif
 
 namespace lidiff {
 
 struct AtFwd {
-    const void *q, *k, *v;
-    int64_t q_row, q_head, k_row, k_head, v_row, v_head;      // strides in elements
+    const void* q;
+    int64_t q_row, q_head;                                    // strides in elements
+    AtRows k, v;
     const int4 *cq, *ck;                                      // (batch, x, y, z) of every row, for the biases
     const int32_t *seg_q, *seg_k;
     int nseg, mq, mk, heads, share, dim;                      // share: query heads per key head
-    float scale;                                              // already times log2 e
+    float scale;
     AtBias bias;
     int splits;                                               // the keys of a scan are shared out over `splits` workgroups
     void* out;                                                // [mq][heads][dim]
@@ -22,180 +31,246 @@ struct AtFwd {
     float *part_o, *part_ml;                                  // splits > 1: [splits][mq][heads][dim], [splits][2][heads][mq]
 };
 
-// one workgroup: 64 queries of one scan (16 a wave) x HG heads x one share of the keys.
+// What a workgroup takes: QB x 16 queries a wave, HG heads, tiles of 64 keys in NBUF buffers.
+// HG: the distances of a (query, key) pair are the same for every head, so a wave takes as many heads as its registers hold.
+template <typename T, int DP> struct AtFwdPlan {
+    static constexpr int kHeads = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 ? 2 : 1;
+    static constexpr int kQB = AT_FWD_QB;
+    static constexpr int kBuf = sizeof(T) == 4 ? 1 : AT_FWD_BUF;
+};
+constexpr int kFwdRows = 64;
+
+inline int at_fwd_heads(int most, int heads, int share, int mode) {      // whole groups of one key head, or key heads of their own
+    return mode != kNone && heads % most == 0 && (share == 1 || share % most == 0) ? most : 1;
+}
+
 // EXACT (16-bit operands, when the table's gradient is wanted): probabilities enter the product with the values in pieces, rounding and
 // rest.  d table sums ds over millions of pairs whose rows cancel to zero through delta = do . out, so an output from probabilities of 8 or
 // 11 bits costs it more than fp32 sums do.
-template <typename T, int DP, int HG, int SLOTS, int BIAS, bool EXACT>
+template <typename T, int DP, int HG, int SLOTS, int BIAS, int QB, int NBUF, bool EXACT>
 __global__ __launch_bounds__(kAtBlock) void at_fwd_kernel(const AtFwd a) {
-    typedef AtTile<T, DP> Tile;
+    constexpr int ROWS = kFwdRows, DC = DP / 32, DB = DP / 16, KB = ROWS / 16;
+    typedef AtTile<T, DP, SLOTS, ROWS> Tile;
     typedef typename AtType<T>::Frag Frag;
-    constexpr int DC = DP / 32, DB = DP / 16;
-    constexpr float kLift = AtType<T>::kLift, kUnlift = AtType<T>::kLift ? 1.f / (1 << AtType<T>::kLift) : 1.f;
-    extern __shared__ __align__(16) unsigned char at_sm[];
-    T* ks = reinterpret_cast<T*>(at_sm);                                          // keys, row by row
-    T* vs = ks + SLOTS * Tile::kRows;                                             // values, transposed
-    float* cs = reinterpret_cast<float*>(vs + SLOTS * Tile::kCols);               // x, y, z of the tile's keys
-    float* table = cs + 3 * kAtRows;                                              // [buckets][HG]
-    AtCell* cells = reinterpret_cast<AtCell*>(table + (BIAS == kTable ? ((a.bias.buckets * HG + 3) & ~3) : 0));
+    // (7, not 15: a probability may exceed the base's by 2^8)
+    constexpr float kLift = AtType<T>::kLift ? 7.f : 0.f, kUnlift = AtType<T>::kLift ? 1.f / 128.f : 1.f, kSlack = 8.f;
+    constexpr bool kOnes = sizeof(T) == 2;
+    extern __shared__ __align__(16) char at_sm[];
+    char* const ks = at_sm;                                                       // [NBUF] keys, [NBUF] values
+    char* const vs = ks + NBUF * Tile::kBytes;
+    float* const cs = reinterpret_cast<float*>(vs + NBUF * Tile::kBytes);         // [2][x, y, z] of the tile's keys
+    unsigned* const cells = reinterpret_cast<unsigned*>(cs + 2 * 3 * ROWS);
+    float* const table = reinterpret_cast<float*>(cells + (BIAS == kTable ? kCells : 0));      // [HG][buckets]
+    const unsigned ks_at = (unsigned)(uintptr_t)(at_lds_t)ks, vs_at = (unsigned)(uintptr_t)(at_lds_t)vs;
 
-    const int lane = lane_id(), wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int groups = a.heads / HG, h0 = (blockIdx.x % groups) * HG, kv0 = h0 / a.share, split = blockIdx.y;
-    const SegTile t = find_seg_tile(a.seg_q, a.nseg, a.mq, kAtRows, blockIdx.x / groups);
+    const SegTile t = find_seg_tile(a.seg_q, a.nseg, a.mq, 64 * QB, blockIdx.x / groups);
     if (t.lo >= t.hi) return;
-    const int qi = t.lo + wave * 16 + col;
-    const bool have = qi < t.hi;
     const int2 kr = t.seg >= 0 ? seg_range(a.seg_k, t.seg, a.mk) : make_int2(0, 0);
-    const int tiles = (kr.y - kr.x + kAtRows - 1) / kAtRows;
+    const int k_lo = __builtin_amdgcn_readfirstlane(kr.x), k_hi = __builtin_amdgcn_readfirstlane(kr.y), tiles = (k_hi - k_lo + ROWS - 1) / ROWS;
     const int first = (int)((int64_t)tiles * split / a.splits), last = (int)((int64_t)tiles * (split + 1) / a.splits);
+    const int q0 = t.lo + wave * 16 * QB;
+    const float scale2 = a.scale * kLog2e;
 
-    Frag qf[HG][DC];
+    Frag qf[QB][HG][DC];
+    float qx[QB], qy[QB], qz[QB], slope[HG];
 #pragma unroll
-    for (int h = 0; h < HG; ++h)
+    for (int n = 0; n < QB; ++n) {
+        const int qi = q0 + 16 * n + col;
+        const bool have = qi < t.hi;
 #pragma unroll
-        for (int c = 0; c < DC; ++c) {
-            const int d = 32 * c + 8 * g;
-            qf[h][c] = have && d < a.dim ? at_frag((const T*)a.q + (int64_t)qi * a.q_row + (int64_t)(h0 + h) * a.q_head + d) : at_zero<T>();
+        for (int h = 0; h < HG; ++h)
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                const int d = 32 * c + 8 * g;
+                qf[n][h][c] = Frag{};
+                if (have && d < a.dim) qf[n][h][c] = at_load8((const T*)a.q + (int64_t)qi * a.q_row + (int64_t)(h0 + h) * a.q_head + d);
+            }
+        qx[n] = qy[n] = qz[n] = 0.f;
+        if (BIAS != kNone && have) {
+            const int4 c = a.cq[qi];
+            qx[n] = (float)c.y; qy[n] = (float)c.z; qz[n] = (float)c.w;
         }
-    float qx = 0.f, qy = 0.f, qz = 0.f, slope[HG];
-    if (BIAS != kNone && have) {
-        const int4 c = a.cq[qi];
-        qx = (float)c.y; qy = (float)c.z; qz = (float)c.w;
     }
 #pragma unroll
-    for (int h = 0; h < HG; ++h) slope[h] = BIAS == kSlope ? -a.bias.slopes[h0 + h] * kLog2e : 0.f;
+    for (int h = 0; h < HG; ++h) slope[h] = BIAS == kSlope ? -a.bias.slopes[h0 + h] / a.scale : 0.f;
     if (BIAS == kTable) {
-        for (int i = threadIdx.x; i < a.bias.buckets * HG; i += kAtBlock) table[i] = a.bias.table[(int64_t)(i / HG) * a.heads + h0 + i % HG] * kLog2e;
+        for (int i = threadIdx.x; i < a.bias.buckets * HG; i += kAtBlock)
+            table[i] = a.bias.table[(int64_t)(i % a.bias.buckets) * a.heads + h0 + i / a.bias.buckets] / a.scale;
         for (int i = threadIdx.x; i < kCells; i += kAtBlock) cells[i] = a.bias.cells[i];
     }
 
-    f32x4 o[HG][DB] = {};
-    float m[HG], l[HG];
+    f32x4 o[QB][HG][DB], l[QB][HG];
+    float base[QB][HG];                                        // in units of log 2; -inf: nothing seen yet
 #pragma unroll
-    for (int h = 0; h < HG; ++h) { m[h] = -INFINITY; l[h] = 0.f; }
-
-    AtLoad<T, DP, SLOTS> kl, vl;
-    int4 kc = make_int4(0, 0, 0, 0);
-    auto fetch = [&](int tile) {
-        const int lo = kr.x + tile * kAtRows;
-        kl.fetch((const T*)a.k, a.k_row, a.k_head, kv0, a.dim, lo, kr.y);
-        vl.fetch((const T*)a.v, a.v_row, a.v_head, kv0, a.dim, lo, kr.y);
-        if (BIAS != kNone && threadIdx.x < kAtRows && lo + (int)threadIdx.x < kr.y) kc = a.ck[lo + threadIdx.x];
-    };
-    if (first < last) fetch(first);
-    for (int tile = first; tile < last; ++tile) {
-        __syncthreads();                                       // the tile before has been read
-        kl.put_rows(ks);
-        vl.put_cols(vs);
-        if (BIAS != kNone && threadIdx.x < kAtRows) {
-            cs[threadIdx.x] = (float)kc.y;
-            cs[kAtRows + threadIdx.x] = (float)kc.z;
-            cs[2 * kAtRows + threadIdx.x] = (float)kc.w;
-        }
-        __syncthreads();
-        if (tile + 1 < last) fetch(tile + 1);                  // in flight under the products
-        if (t.lo + wave * 16 >= t.hi) continue;                // a wave without queries only loads
-        const int left = kr.y - (kr.x + tile * kAtRows);       // keys of this tile, 64 except at the end
-
-        // what the heads share: distance, or the offset of the bucket's row in the table
-        float dist[16];
-        int row_of[16];
-        if (BIAS != kNone) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(cs + 16 * b + 4 * g), y = *reinterpret_cast<const f32x4*>(cs + kAtRows + 16 * b + 4 * g),
-                            z = *reinterpret_cast<const f32x4*>(cs + 2 * kAtRows + 16 * b + 4 * g);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float dx = x[e] - qx, dy = y[e] - qy, dz = z[e] - qz, d2 = dx * dx + dy * dy + dz * dz;
-                    if (BIAS == kSlope) dist[4 * b + e] = __builtin_amdgcn_sqrtf(d2);
-                    if (BIAS == kTable) {
-                        const AtCell c = cells[at_cell(d2)];
-                        row_of[4 * b + e] = c.bucket + (d2 >= c.edge ? 1 : 0);
-                    }
-                }
-            }
-        }
+    for (int n = 0; n < QB; ++n)
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
-            const int slot = SLOTS == 1 ? 0 : h;
-            f32x4 s[4];
+            base[n][h] = -INFINITY;
+            l[n][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int b = 0; b < DB; ++b) o[n][h][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    Frag ones{};
+    if constexpr (kOnes) {
 #pragma unroll
-                for (int c = 0; c < DC; ++c) at_mma(s[b], at_frag(ks + slot * Tile::kRows + (16 * b + col) * Tile::kRow + 32 * c + 8 * g), qf[h][c]);
+        for (int e = 0; e < 8; ++e) ones[e] = (typename AtType<T>::Elem)1.f;
+    }
+
+    int4 kc = make_int4(0, 0, 0, 0);                           // the coordinates one tile further than the requests
+    auto coords = [&](int tile) {
+        const int row = k_lo + tile * ROWS + (int)threadIdx.x;
+        if (BIAS != kNone && tile < last && threadIdx.x < ROWS && row < k_hi) kc = a.ck[row];
+    };
+    auto put_coords = [&](int tile) {
+        if (BIAS == kNone || threadIdx.x >= ROWS) return;
+        float* c = cs + (tile & 1) * 3 * ROWS + threadIdx.x;
+        c[0] = (float)kc.y; c[ROWS] = (float)kc.z; c[2 * ROWS] = (float)kc.w;
+    };
+    auto request = [&](int tile) {
+        const int lo = k_lo + tile * ROWS, left = min(ROWS, k_hi - lo), at = (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
+        Tile::request(a.k, kv0, a.dim, lo, left, ks_at + at);
+        Tile::request(a.v, kv0, a.dim, lo, left, vs_at + at);
+    };
+    if (first < last) {
+        coords(first);
+        put_coords(first);
+        coords(first + 1);
+        request(first);
+    }
+    for (int tile = first; tile < last; ++tile) {
+        AT_ARRIVE();
+        if (NBUF == 2 && tile + 1 < last) request(tile + 1);
+        if (tile + 1 < last) {
+            put_coords(tile + 1);
+            coords(tile + 2);
+        }
+        if (q0 < t.hi) {                                       // (a wave without queries only takes part in the requests)
+            const char* const kt = ks + (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
+            const char* const vt = vs + (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
+            const float* const ct = cs + (tile & 1) * 3 * ROWS;
+            const int left = k_hi - (k_lo + tile * ROWS);      // keys of this tile, 64 except at the end
+            AtPairs<BIAS> pairs[QB][KB];
+            if (BIAS != kNone) {
+#pragma unroll
+                for (int n = 0; n < QB; ++n)
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) pairs[n][b].form(ct, ROWS, 16 * b + 4 * g, qx[n], qy[n], qz[n], cells);
             }
-            float top = -INFINITY;
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+            for (int h = 0; h < HG; ++h) {
+                const int slot = SLOTS == 1 ? 0 : h;
+                f32x4 s[QB][KB];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = s[b][e] * a.scale;
-                    if (BIAS == kSlope) v += slope[h] * dist[4 * b + e];
-                    if (BIAS == kTable) v += table[row_of[4 * b + e] * HG + h];
-                    if (left < kAtRows && 16 * b + 4 * g + e >= left) v = -INFINITY;
-                    s[b][e] = v;
-                    top = fmaxf(top, v);
+                for (int b = 0; b < KB; ++b) {
+#pragma unroll
+                    for (int n = 0; n < QB; ++n) s[n][b] = pairs[n][b].start(slope[h], table + h * a.bias.buckets);
+#pragma unroll
+                    for (int c = 0; c < DC; ++c) {
+                        const Frag kf = Tile::frag(kt, Tile::at_rows(slot, b, c));
+#pragma unroll
+                        for (int n = 0; n < QB; ++n) at_mma(s[n][b], kf, qf[n][h][c]);
+                    }
                 }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float now = fmaxf(m[h], top), safe = now == -INFINITY ? 0.f : now, base = safe - kLift;
-            const float fade = __builtin_amdgcn_exp2f(m[h] - safe);
-            m[h] = now;
-            l[h] *= fade;
+                if (left < ROWS) {
 #pragma unroll
-            for (int b = 0; b < DB; ++b) o[h][b] *= fade;
+                    for (int n = 0; n < QB; ++n)
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+                        for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[b][e] = __builtin_amdgcn_exp2f(s[b][e] - base);
-                    l[h] += s[b][e];
+                            for (int e = 0; e < 4; ++e)
+                                if (16 * b + 4 * g + e >= left) s[n][b][e] = -INFINITY;
+                }
+                constexpr int PIECES = EXACT ? 2 : 1;
+                Frag p[QB][KB / 2][PIECES];
+#pragma unroll
+                for (int n = 0; n < QB; ++n) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[n][b][e]);
+                    top *= scale2;
+                    if (__any(top > base[n][h] + kSlack)) {
+                        top = fmaxf(top, __shfl_xor(top, 16));
+                        top = fmaxf(top, __shfl_xor(top, 32));
+                        const float now = fmaxf(base[n][h], top), fade = __builtin_amdgcn_exp2f(base[n][h] - (now == -INFINITY ? 0.f : now));
+                        base[n][h] = now;
+                        l[n][h] *= fade;
+#pragma unroll
+                        for (int b = 0; b < DB; ++b) o[n][h][b] *= fade;
+                    }
+                    const float down = base[n][h] == -INFINITY ? 0.f : kLift - base[n][h];
+                    const float factor = at_scale(s[n], scale2, at_huge(base[n][h]));
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[n][b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[n][b][e], factor, down));
+                            if (!kOnes) l[n][h][e] += s[n][b][e];
+                        }
+#pragma unroll
+                    for (int j = 0; j < KB / 2; ++j) {
+                        const f32x8 v = at_join(s[n][2 * j], s[n][2 * j + 1]);
+                        at_pack(p[n][j][0], v);
+                        if constexpr (EXACT) at_pack_rest(p[n][j][1], p[n][j][0], v);
+                        if constexpr (kOnes) {
+#pragma unroll
+                            for (int i = 0; i < PIECES; ++i) at_mma(l[n][h], ones, p[n][j][i]);
+                        }
+                    }
                 }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                constexpr int PIECES = EXACT ? AtType<T>::kPieces : 1;
-                Frag p[PIECES];
-                at_pack(p[0], s[2 * j], s[2 * j + 1]);
-                if constexpr (PIECES > 1) {
+                for (int j = 0; j < KB / 2; ++j)
 #pragma unroll
-                    for (int i = 1; i < PIECES; ++i) at_pack_rest(p[i], p[i - 1], s[2 * j], s[2 * j + 1]);
-                }
+                    for (int b = 0; b < DB; ++b) {
+                        const Frag vf = Tile::frag_turned(vt, slot, j, b);
 #pragma unroll
-                for (int b = 0; b < DB; ++b) {
-                    const Frag vf = at_frag_rows(vs + slot * Tile::kCols + (16 * b + col) * Tile::kCol + 32 * j + 4 * g);
+                        for (int n = 0; n < QB; ++n)
 #pragma unroll
-                    for (int i = 0; i < PIECES; ++i) at_mma(o[h][b], vf, p[i]);
-                }
+                            for (int i = 0; i < PIECES; ++i) at_mma(o[n][h][b], vf, p[n][j][i]);
+                    }
             }
+        }
+        if (NBUF == 1 && tile + 1 < last) {
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the tile has been read
+            request(tile + 1);
         }
     }
-    if (!have) return;
 #pragma unroll
-    for (int h = 0; h < HG; ++h) {
-        float sum = l[h] + __shfl_xor(l[h], 16);               // (the four lanes of a query leave together: `have` is the same for them)
-        sum += __shfl_xor(sum, 32);
-        const int head = h0 + h;
-        if (a.splits > 1) {
-            if (g == 0) {
-                a.part_ml[((int64_t)(2 * split) * a.heads + head) * a.mq + qi] = m[h];
-                a.part_ml[((int64_t)(2 * split + 1) * a.heads + head) * a.mq + qi] = sum * kUnlift;
+    for (int n = 0; n < QB; ++n) {
+        const int qi = q0 + 16 * n + col;
+        if (qi >= t.hi) continue;
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+            float sum = l[n][h][0];                            // (ones: every row of the product holds the sum)
+            if (!kOnes) {
+                sum = (l[n][h][0] + l[n][h][1]) + (l[n][h][2] + l[n][h][3]);
+                sum += __shfl_xor(sum, 16);                    // (the four lanes of a query are here together)
+                sum += __shfl_xor(sum, 32);
             }
+            const int head = h0 + h;
+            if (a.splits > 1) {
+                if (g == 0) {
+                    a.part_ml[((int64_t)(2 * split) * a.heads + head) * a.mq + qi] = base[n][h];
+                    a.part_ml[((int64_t)(2 * split + 1) * a.heads + head) * a.mq + qi] = sum * kUnlift;
+                }
 #pragma unroll
-            for (int b = 0; b < DB; ++b)
-                if (16 * b + 4 * g < a.dim) at_store4(a.part_o + (((int64_t)split * a.mq + qi) * a.heads + head) * a.dim + 16 * b + 4 * g, o[h][b] * kUnlift);
-            continue;
-        }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        if (a.lse && g == 0) a.lse[(int64_t)head * a.mq + qi] = sum == 0.f ? INFINITY : m[h] - kLift + log2f(sum);
+                for (int b = 0; b < DB; ++b)
+                    if (16 * b + 4 * g < a.dim) at_store4(a.part_o + (((int64_t)split * a.mq + qi) * a.heads + head) * a.dim + 16 * b + 4 * g, o[n][h][b] * kUnlift);
+                continue;
+            }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            if (a.lse && g == 0) a.lse[(int64_t)head * a.mq + qi] = sum == 0.f ? INFINITY : base[n][h] - kLift + log2f(sum);
 #pragma unroll
-        for (int b = 0; b < DB; ++b) {
-            if (16 * b + 4 * g >= a.dim) continue;
-            const f32x4 r = o[h][b] * inv;
-            const int64_t at = ((int64_t)qi * a.heads + head) * a.dim + 16 * b + 4 * g;
-            at_store4((T*)a.out + at, r);
-            if (a.out32) at_store4(a.out32 + at, r);
+            for (int b = 0; b < DB; ++b) {
+                if (16 * b + 4 * g >= a.dim) continue;
+                const f32x4 r = o[n][h][b] * inv;
+                const int64_t at = ((int64_t)qi * a.heads + head) * a.dim + 16 * b + 4 * g;
+                at_store4((T*)a.out + at, r);
+                if (a.out32) at_store4(a.out32 + at, r);
+            }
         }
     }
 }
@@ -228,13 +303,15 @@ __global__ void at_join_kernel(const AtFwd a) {
 
 template <typename T, int DP, int HG, int SLOTS, int BIAS, bool EXACT = false>
 static hipError_t at_fwd_launch(const AtFwd& a, hipStream_t st) {
-    typedef AtTile<T, DP> Tile;
-    const int64_t wg = seg_tiles_bound(a.mq, kAtRows, a.seg_q, a.nseg) * (a.heads / HG);
-    size_t lds = (size_t)SLOTS * (Tile::kRows + Tile::kCols) * sizeof(T) + 3 * kAtRows * sizeof(float);
-    if (BIAS == kTable) lds += (size_t)((a.bias.buckets * HG + 3) & ~3) * sizeof(float) + kCells * sizeof(AtCell);
-    const hipError_t e = hipFuncSetAttribute((const void*)at_fwd_kernel<T, DP, HG, SLOTS, BIAS, EXACT>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    typedef AtFwdPlan<T, DP> Plan;
+    constexpr int QB = Plan::kQB, NBUF = Plan::kBuf;
+    const int64_t wg = seg_tiles_bound(a.mq, 64 * QB, a.seg_q, a.nseg) * (a.heads / HG);
+    size_t lds = (size_t)2 * NBUF * AtTile<T, DP, SLOTS, kFwdRows>::kBytes + 2 * 3 * kFwdRows * sizeof(float);
+    if (BIAS == kTable) lds += (kCells + a.bias.buckets * HG) * sizeof(float);
+    auto kern = at_fwd_kernel<T, DP, HG, SLOTS, BIAS, QB, NBUF, EXACT>;
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return e;
-    at_fwd_kernel<T, DP, HG, SLOTS, BIAS, EXACT><<<dim3((unsigned)wg, (unsigned)a.splits), kAtBlock, lds, st>>>(a);
+    kern<<<dim3((unsigned)wg, (unsigned)a.splits), kAtBlock, lds, st>>>(a);
     if (a.splits > 1) at_join_kernel<T><<<(unsigned)ceil_div((int64_t)a.mq * a.heads * (a.dim / 4), 256), 256, 0, st>>>(a);
     return hipGetLastError();
 }
@@ -249,72 +326,103 @@ static hipError_t at_fwd_bias(const AtFwd& a, int mode, hipStream_t st) {
     return hipErrorInvalidValue;
 }
 
-template <typename T>
-static hipError_t at_fwd_dispatch(const AtFwd& a, int mode, hipStream_t st) {
-    const int hg = at_heads_per_wave(a.dim, a.heads, a.share, mode);
-    const bool one = a.share > 1;
-    if (a.dim <= 32) {
-        if (hg == 4) return one ? at_fwd_bias<T, 32, 4, 1>(a, mode, st) : at_fwd_bias<T, 32, 4, 4>(a, mode, st);
-        return at_fwd_bias<T, 32, 1, 1>(a, mode, st);
-    }
-    if (a.dim <= 64) {
-        if (hg == 2) return one ? at_fwd_bias<T, 64, 2, 1>(a, mode, st) : at_fwd_bias<T, 64, 2, 2>(a, mode, st);
-        return at_fwd_bias<T, 64, 1, 1>(a, mode, st);
-    }
-    return at_fwd_bias<T, 128, 1, 1>(a, mode, st);
+template <typename T, int DP>
+static hipError_t at_fwd_width(const AtFwd& a, int mode, hipStream_t st) {
+    constexpr int most = AtFwdPlan<T, DP>::kHeads;
+    if constexpr (most > 1)
+        if (at_fwd_heads(most, a.heads, a.share, mode) == most) return a.share > 1 ? at_fwd_bias<T, DP, most, 1>(a, mode, st) : at_fwd_bias<T, DP, most, most>(a, mode, st);
+    return at_fwd_bias<T, DP, 1, 1>(a, mode, st);
 }
 
 // how many workgroups share a scan's keys: one while there are workgroups enough for the card, else so many that there are, each with
-// at least four tiles of an average scan's keys
-static int at_fwd_splits(int64_t mq, int64_t mk, int nseg, int heads, int hg) {
-    const int64_t wg = (ceil_div(mq, kAtRows) + (nseg > 1 ? nseg - 1 : 0)) * (heads / hg);
+// at least two tiles of an average scan's keys
+template <typename T, int DP>
+static int at_fwd_splits(int64_t mq, int64_t mk, int64_t nseg, int heads, int share, int mode) {
+    typedef AtFwdPlan<T, DP> Plan;
+    const int64_t wg = (ceil_div(mq, 64 * Plan::kQB) + nseg - 1) * (heads / at_fwd_heads(Plan::kHeads, heads, share, mode));
     if (wg >= 512) return 1;
-    const int64_t want = ceil_div(1024, wg), most = ceil_div(mk, nseg) / (4 * kAtRows);
+    const int64_t want = ceil_div(1024, wg), most = ceil_div(mk, nseg) / (2 * kFwdRows);
     const int64_t n = want < most ? want : most;
     return n < 1 ? 1 : (int)(n < 64 ? n : 64);
+}
+
+struct AtFwdLayout { int splits; int64_t k, v, part, bytes; };      // workspace: the planes of k and v (fp32), the shares' sums
+
+template <typename T>
+static AtFwdLayout at_fwd_layout(int64_t mq, int64_t mk, int64_t nseg, int heads, int kv_heads, int dim, int mode) {
+    auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+    AtFwdLayout l;
+    const int share = heads / kv_heads;
+    l.splits = dim <= 32 ? at_fwd_splits<T, 32>(mq, mk, nseg, heads, share, mode) : dim <= 64 ? at_fwd_splits<T, 64>(mq, mk, nseg, heads, share, mode)
+                                                                                            : at_fwd_splits<T, 128>(mq, mk, nseg, heads, share, mode);
+    const int64_t planes = sizeof(T) == 4 ? up(3 * at_plane_bytes(mk, kv_heads, dim)) : 0;
+    l.k = 0;
+    l.v = planes;
+    l.part = 2 * planes;
+    l.bytes = l.part + (l.splits > 1 ? l.splits * mq * heads * (dim + 2) * (int64_t)sizeof(float) : 0);
+    return l;
+}
+
+struct AtFwdIn {
+    const void *k, *v;
+    int64_t k_row, k_head, v_row, v_head;
+    int kv_heads;
+    char* ws;
+};
+
+template <typename T>
+static hipError_t at_fwd_run(AtFwd a, const AtFwdIn& in, const AtFwdLayout& l, int mode, hipStream_t st) {
+    a.k = at_stream<T>(in.k, in.k_row, in.k_head, a.mk, in.kv_heads, a.dim, in.ws + l.k, st);
+    a.v = at_stream<T>(in.v, in.v_row, in.v_head, a.mk, in.kv_heads, a.dim, in.ws + l.v, st);
+    if (a.dim <= 32) return at_fwd_width<T, 32>(a, mode, st);
+    if (a.dim <= 64) return at_fwd_width<T, 64>(a, mode, st);
+    return at_fwd_width<T, 128>(a, mode, st);
 }
 
 }  // namespace lidiff
 
 using namespace lidiff;
 
+static AtFwdLayout at_fwd_layout_of(int dtype, int64_t mq, int64_t mk, int64_t nseg, int heads, int kv_heads, int dim, int mode) {
+    return dtype == 0 ? at_fwd_layout<float>(mq, mk, nseg, heads, kv_heads, dim, mode) : at_fwd_layout<__bf16>(mq, mk, nseg, heads, kv_heads, dim, mode);
+}
+
 extern "C" int64_t lidiff_segment_attention_workspace_bytes(int64_t mq, int64_t mk, int64_t n_segments, int32_t heads, int32_t kv_heads, int32_t dim,
-                                                            int32_t bias_mode) {
-    if (mq < 1 || n_segments < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 8 || dim > 128) return 0;
-    const int s = at_fwd_splits(mq, mk, (int)n_segments, heads, at_heads_per_wave(dim, heads, heads / kv_heads, bias_mode));
-    return s == 1 ? 0 : (int64_t)s * mq * heads * (dim + 2) * (int64_t)sizeof(float);
+                                                            int32_t dtype, int32_t bias_mode) {
+    if (mq < 1 || mk < 0 || n_segments < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 8 || dim > 128) return 0;
+    return at_fwd_layout_of(dtype, mq, mk, n_segments, heads, kv_heads, dim, bias_mode).bytes;
 }
 
 extern "C" int lidiff_segment_attention(const void* q, const void* k, const void* v, const int64_t* strides, const int32_t* coords_q, const int32_t* coords_k,
                                         const int32_t* seg_q, const int32_t* seg_k, int64_t n_segments, int64_t mq, int64_t mk, int32_t heads,
                                         int32_t kv_heads, int32_t dim, int32_t dtype, float scale, int32_t bias_mode, const float* slopes,
                                         const float* table, const void* cells, int32_t buckets, void* out, float* out_f32, int32_t exact, float* lse,
-                                        void* workspace,
-                                        void* stream) {
+                                        void* workspace, void* stream) {
     LIDIFF_CHECK_ARG(q && out && strides && (mk == 0 || (k && v)), "null pointer");
-    const char* bad = at_check(n_segments, mq, mk, heads, kv_heads, dim, dtype, bias_mode, buckets, strides, 6);
+    const char* bad = at_check(n_segments, mq, mk, heads, kv_heads, dim, dtype, scale, bias_mode, buckets, strides, 6);
     LIDIFF_CHECK_ARG(bad == nullptr, bad);
     LIDIFF_CHECK_ARG((seg_q != nullptr) == (seg_k != nullptr) && (seg_q || n_segments == 1), "segments of queries and keys come together");
     LIDIFF_CHECK_ARG(bias_mode == kNone || (coords_q && (coords_k || mk == 0)), "a distance bias needs the coordinates");
     LIDIFF_CHECK_ARG(bias_mode != kSlope || slopes, "null pointer");
     LIDIFF_CHECK_ARG(bias_mode != kTable || (table && cells), "null pointer");
     LIDIFF_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)out_f32 | (uintptr_t)coords_q | (uintptr_t)coords_k |
-                       (uintptr_t)workspace) & 15) == 0 && (((uintptr_t)seg_q | (uintptr_t)seg_k | (uintptr_t)cells) & 7) == 0, "misaligned pointer");
+                       (uintptr_t)workspace) & 15) == 0 && (((uintptr_t)seg_q | (uintptr_t)seg_k) & 7) == 0, "misaligned pointer");
+    const AtFwdLayout l = at_fwd_layout_of(dtype, mq, mk, n_segments, heads, kv_heads, dim, bias_mode);
+    LIDIFF_CHECK_ARG(l.bytes == 0 || workspace, "workspace missing (lidiff_segment_attention_workspace_bytes)");
     AtFwd a;
-    a.q = q; a.k = k; a.v = v;
-    a.q_row = strides[0]; a.q_head = strides[1]; a.k_row = strides[2]; a.k_head = strides[3]; a.v_row = strides[4]; a.v_head = strides[5];
+    a.q = q; a.q_row = strides[0]; a.q_head = strides[1];
     a.cq = (const int4*)coords_q; a.ck = (const int4*)coords_k;
     a.seg_q = seg_q; a.seg_k = seg_k; a.nseg = (int)n_segments; a.mq = (int)mq; a.mk = (int)mk;
     a.heads = heads; a.share = heads / kv_heads; a.dim = dim;
-    a.scale = scale * kLog2e;
-    a.bias = AtBias{table, (const AtCell*)cells, slopes, buckets};
-    a.splits = at_fwd_splits(mq, mk, a.nseg, heads, at_heads_per_wave(dim, heads, a.share, bias_mode));
+    a.scale = scale;
+    a.bias = AtBias{table, (const unsigned*)cells, slopes, bias_mode == kTable ? buckets : 0};
+    a.splits = l.splits;
     a.out = out; a.out32 = out_f32; a.exact = exact; a.lse = lse;
-    a.part_o = (float*)workspace;
-    a.part_ml = a.part_o ? a.part_o + (int64_t)a.splits * mq * heads * dim : nullptr;
-    LIDIFF_CHECK_ARG(a.splits == 1 || workspace, "workspace missing (lidiff_segment_attention_workspace_bytes)");
+    a.part_o = (float*)((char*)workspace + l.part);
+    a.part_ml = a.part_o + (int64_t)l.splits * mq * heads * dim;
+    const AtFwdIn in = {k, v, strides[2], strides[3], strides[4], strides[5], kv_heads, (char*)workspace};
     hipStream_t st = (hipStream_t)stream;
-    LIDIFF_CHECK_HIP(dtype == 0 ? at_fwd_dispatch<float>(a, bias_mode, st) : dtype == 1 ? at_fwd_dispatch<__bf16>(a, bias_mode, st)
-                                                                                      : at_fwd_dispatch<_Float16>(a, bias_mode, st));
+    LIDIFF_CHECK_HIP(dtype == 0 ? at_fwd_run<float>(a, in, l, bias_mode, st) : dtype == 1 ? at_fwd_run<__bf16>(a, in, l, bias_mode, st)
+                                                                                          : at_fwd_run<_Float16>(a, in, l, bias_mode, st));
     return 0;
 }

@@ -2146,28 +2146,22 @@ def distance_edges(num_buckets: int, reach: float, unit: float = 1.0) -> tuple[i
     return edges
 
 
-def _cell_of(d2: int) -> int:
-    bits = int(torch.tensor(float(d2), dtype=torch.float32).view(torch.int32))
-    return min(max((bits >> (23 - _CELL_BITS)) - ((127 << _CELL_BITS) - 1), 0), (22 << _CELL_BITS) + 1)
-
-
 def bucket_cells(edges: tuple[int, ...]) -> torch.Tensor:
-    """The kernels' look-up table of ascending squared-distance edges (host tensor int32 [cells, 2] = fp32 bits of the edge inside the
-    cell, bucket in front of it; AtCell of attention.h): the leading bits of a squared distance name a cell, and a cell may hold one
-    edge only."""
+    """The kernels' look-up table of ascending squared-distance edges (host tensor int32 [cells]; attention.h): the leading bits of a
+    squared distance name a cell, which holds the bucket in front of it (low 8 bits) and the remaining bits of the edge inside it (above;
+    beyond all of them: no edge).  A cell may hold one edge only."""
     edges = tuple(edges)
     if not all(isinstance(e, int) and 1 <= e <= MAX_EDGE for e in edges) or any(b <= a for a, b in zip(edges, edges[1:])):
         raise ValueError(f"edges must be ascending whole squared distances in [1, {MAX_EDGE}]")
-    cells = [_cell_of(e) for e in edges]
-    if len(set(cells)) != len(cells):
-        raise ValueError("two edges are closer than 1/32 of their squared distance")
+    rest, first = 23 - _CELL_BITS, (127 << _CELL_BITS) - 1
     n = (22 << _CELL_BITS) + 2
-    at = torch.arange(n)
-    bucket = (at[:, None] > torch.tensor(cells, dtype=torch.int64)[None, :]).sum(1) if cells else torch.zeros(n, dtype=torch.int64)
-    edge = torch.full((n,), math.inf, dtype=torch.float32)
-    if cells:
-        edge[torch.tensor(cells)] = torch.tensor(edges, dtype=torch.float32)
-    return torch.stack([edge.view(torch.int32), bucket.to(torch.int32)], 1).contiguous()
+    bits = torch.tensor(edges, dtype=torch.float32).view(torch.int32).long()
+    cells = ((bits >> rest) - first).clamp(0, n - 1)
+    if len(set(cells.tolist())) != len(edges):
+        raise ValueError("two edges are closer than 1/32 of their squared distance")
+    word = (torch.arange(n)[:, None] > cells[None, :]).sum(1) + ((1 << rest) << 8)
+    word[cells] = (torch.arange(len(edges))) + ((bits & ((1 << rest) - 1)) << 8)
+    return word.to(torch.int32)
 
 
 _BUCKET_CELLS: dict = {}      # (edges, device) -> the table on the device: a constant of the configuration, built once per device
@@ -2184,7 +2178,7 @@ def _device_cells(edges: tuple[int, ...], device) -> torch.Tensor:
 def _heads_rows(t: torch.Tensor) -> torch.Tensor:
     """[M, H, D] as the kernels read it: channels contiguous, every row and head on a 16-byte boundary (a copy where it is not)."""
     piece = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % piece == 0 and t.stride(1) % piece == 0 and t.data_ptr() % 16 == 0 and min(t.stride()) >= 0:
+    if t.stride(2) == 1 and t.stride(0) % piece == 0 and t.stride(1) % piece == 0 and t.data_ptr() % 16 == 0 and 0 <= t.stride(0) < 1 << 22:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -2213,7 +2207,7 @@ class _SegmentAttention(torch.autograd.Function):
         out32 = None if not grads else out if q.dtype == torch.float32 else torch.empty((mq, heads, dim), dtype=torch.float32, device=dev)
         lse = torch.empty((heads, mq), dtype=torch.float32, device=dev) if grads else None
         if mq:
-            nbytes = _lib.load().lidiff_segment_attention_workspace_bytes(mq, mk, n_seg, heads, kv_heads, dim, mode)
+            nbytes = _lib.load().lidiff_segment_attention_workspace_bytes(mq, mk, n_seg, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], mode)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
             call("lidiff_segment_attention", ptr(q), ptr(k), ptr(v), _strides(q, k, v), ptr(coords_q), ptr(coords_k), ptr(seg_q), ptr(seg_k),
                  n_seg, mq, mk, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], float(scale), mode, ptr(slopes), ptr(tab), ptr(cells),
@@ -2241,8 +2235,8 @@ class _SegmentAttention(torch.autograd.Function):
                 tab = None if table is None else _aligned(table.detach().float())
                 buckets = 0 if table is None else table.shape[0]
                 n_seg = 1 if seg_q is None else seg_q.shape[0]
-                ws = torch.empty(_lib.load().lidiff_segment_attention_bwd_workspace_bytes(mq, mk, n_seg, heads, kv_heads, dim, ctx.mode, buckets,
-                                                                                         int(need_t)), dtype=torch.uint8, device=dev)
+                ws = torch.empty(_lib.load().lidiff_segment_attention_bwd_workspace_bytes(mq, mk, n_seg, heads, kv_heads, dim, _ROW_DTYPES[q.dtype],
+                                                                                         ctx.mode, buckets, int(need_t)), dtype=torch.uint8, device=dev)
                 call("lidiff_segment_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(go), _strides(q, k, v, go), ptr(coords_q), ptr(coords_k),
                      ptr(seg_q), ptr(seg_k), n_seg, mq, mk, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], float(ctx.scale), ctx.mode,
                      ptr(slopes), ptr(tab), ptr(None if table is None else _device_cells(ctx.edges, dev)), buckets, ptr(out32), ptr(lse),
@@ -2300,8 +2294,8 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seg_q: 
             if c is None or c.dtype != torch.int32 or c.shape != (m, 4):
                 raise ValueError(f"a distance bias needs {name}: int32 [{m}, 4]")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if not 1e-6 <= scale <= 1e6:
+        raise ValueError(f"scale must lie in [1e-6, 1e6], got {scale}")
     require_device(q)
     fit = lambda t: None if t is None else _aligned(t)
     with torch.cuda.device(dev):

@@ -20,13 +20,12 @@ def test_bucket_cells_name_every_distance_s_bucket(ops):
     for edges in (ops.distance_edges(32, 100, 16), ops.distance_edges(48, 120, 8), ops.distance_edges(2, 100, 1), ops.distance_edges(3, 50, 0.5), (), (1,),
                   (1, 2, 3, 4, 5, 9, 1 << 22)):
         cells = ops.bucket_cells(edges)
-        edge = cells[:, 0].contiguous().view(torch.float32)
         d2 = sorted({0, 1, 2, 3, 3 * 65535 ** 2} | {max(0, e + o) for e in edges for o in (-1, 0, 1)} | {rng.randrange(1 << 24) for _ in range(400)})
         f = torch.tensor(d2, dtype=torch.float64).float()
         at = ((f.view(torch.int32) >> 18) - ((127 << 5) - 1)).clamp(0, cells.shape[0] - 1)
-        got = cells[at, 1] + (f >= edge[at]).int()
+        got = (cells[at] & 255) + ((f.view(torch.int32) & ((1 << 18) - 1)) >= (cells[at] >> 8)).int()
         assert got.tolist() == [sum(e <= v for e in edges) for v in d2]
-        assert int(cells[:, 1].max()) <= len(edges)
+        assert int((cells & 255).max()) <= len(edges)
 
 
 def test_edges_are_refused(ops):
@@ -63,7 +62,7 @@ def test_attention_refusals(ops):
                 dict(bias=table, coords_q=c, coords_k=c), dict(edges=(1, 4)), dict(bias=table, edges=(1,), coords_q=c, coords_k=c),
                 dict(bias=table, edges=(1, 4), coords_q=c.long(), coords_k=c), dict(bias=table, edges=(1, 4), coords_q=c[:5], coords_k=c),
                 dict(bias=torch.zeros(49, 4), edges=tuple(range(1, 49)), coords_q=c, coords_k=c), dict(bias=table.t(), edges=(1, 4), coords_q=c, coords_k=c),
-                dict(bias=table, edges=(1, 4), slopes=torch.ones(4), coords_q=c, coords_k=c), dict(scale=math.inf), dict(scale=math.nan)):
+                dict(bias=table, edges=(1, 4), slopes=torch.ones(4), coords_q=c, coords_k=c), dict(scale=math.inf), dict(scale=math.nan), dict(scale=0.0), dict(scale=-1.0)):
         with pytest.raises(ValueError):
             ops.segment_attention(**{**ok, **bad})
     with pytest.raises(RuntimeError, match="GPU only"):
@@ -94,23 +93,23 @@ def test_library_refuses_before_it_launches():
                      (dict(x=ctypes.c_void_p(4100)), "misaligned"), (dict(rows=2 ** 31), "rows")):
         rc, msg = norm(**kw)
         assert rc == 1 and word in msg, (kw, msg)
-    base = dict(q=P(), k=P(2), v=P(3), strides=[128, 32] * 3, cq=P(4), ck=P(5), sq=P(6), sk=P(7), nseg=1, mq=8, mk=8, h=4, hk=4, d=32, dtype=0, mode=0, slopes=None,
+    base = dict(q=P(), k=P(2), v=P(3), strides=[128, 32] * 3, cq=P(4), ck=P(5), sq=P(6), sk=P(7), nseg=1, mq=8, mk=8, h=4, hk=4, d=32, dtype=0, mode=0, scale=0.1, slopes=None,
                 table=None, cells=None, buckets=0, out=P(8))
     def attend(**kw):
         a = {**base, **kw}
         rc = lib.lidiff_segment_attention(a["q"], a["k"], a["v"], (ctypes.c_int64 * 6)(*a["strides"]), a["cq"], a["ck"], a["sq"], a["sk"], a["nseg"], a["mq"], a["mk"],
-                                          a["h"], a["hk"], a["d"], a["dtype"], 0.1, a["mode"], a["slopes"], a["table"], a["cells"], a["buckets"], a["out"], None, 0,
+                                          a["h"], a["hk"], a["d"], a["dtype"], a["scale"], a["mode"], a["slopes"], a["table"], a["cells"], a["buckets"], a["out"], None, 0,
                                           None, None, None)
         return rc, lib.lidiff_last_error().decode()
     for kw, word in ((dict(q=None), "null"), (dict(k=None), "null"), (dict(sq=None), "together"), (dict(nseg=0), "segments"), (dict(mq=0), "rows"), (dict(mk=-1), "rows"),
                      (dict(mq=2 ** 31), "rows"), (dict(hk=3), "divide"), (dict(d=36), "head dimension"), (dict(d=256), "head dimension"), (dict(dtype=7), "dtype"),
                      (dict(mode=3), "bias"), (dict(mode=1), "null"), (dict(mode=1, cq=None, slopes=P()), "coordinates"), (dict(mode=2, buckets=49), "buckets"),
-                     (dict(mode=2, buckets=8), "null"), (dict(strides=[127, 32] * 3), "16-byte"), (dict(strides=[-128, 32] * 3), "16-byte"),
+                     (dict(mode=2, buckets=8), "null"), (dict(strides=[127, 32] * 3), "16-byte"), (dict(strides=[-128, 32] * 3), "16-byte"), (dict(strides=[1 << 22, 32] * 3), "row stride"), (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"),
                      (dict(q=ctypes.c_void_p(4104)), "misaligned"), (dict(mk=5000), "workspace missing")):
         rc, msg = attend(**kw)
         assert rc == 1 and word in msg, (kw, msg)
-    assert lib.lidiff_segment_attention_workspace_bytes(8, 5000, 1, 4, 4, 32, 0) > 0
-    assert lib.lidiff_segment_attention_workspace_bytes(8, 5000, 1, 4, 3, 32, 0) == 0
-    assert lib.lidiff_segment_attention_bwd_workspace_bytes(8, 8, 1, 4, 4, 32, 2, 16, 1) >= 8 * 4 * 4
+    assert lib.lidiff_segment_attention_workspace_bytes(8, 5000, 1, 4, 4, 32, 1, 0) > 0
+    assert lib.lidiff_segment_attention_workspace_bytes(8, 5000, 1, 4, 3, 32, 1, 0) == 0
+    assert lib.lidiff_segment_attention_bwd_workspace_bytes(8, 8, 1, 4, 4, 32, 1, 2, 16, 1) >= 8 * 4 * 4
     rc = lib.lidiff_batch_segments(P(), 2 ** 30, None, 4, 4, P(2), P(3), None)
     assert rc == 1 and "2^31" in lib.lidiff_last_error().decode()
