@@ -23,7 +23,7 @@ typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* at_lds_t;
 
-constexpr int kAtBlock = 256;      // 4 waves
+constexpr int kAtBlock = 256;      // 4 waves; two a SIMD (at_waves): with at most 256 registers the matrix results stay in vector registers
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // -- operands -----------------------------------------------------------------------------------------------------------------------
@@ -33,6 +33,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // are rounded to an fp16 operand and the sums divided by it -- exact, and an addend of an exponent that is formed anyway.
 struct AtPieces { bf16x8 p[3]; };
 template <typename T> struct AtType;
+// waves a SIMD the kernels are compiled for (the widest fp32 rows need more than 256 registers)
+constexpr int at_waves(int bytes, int width) { return bytes == 4 && width == 128 ? 1 : 2; }
 template <> struct AtType<__bf16> { typedef bf16x8 Frag; typedef bf16x4 Quad; typedef __bf16 Elem; static constexpr int kPlanes = 1, kLift = 0; };
 template <> struct AtType<_Float16> { typedef f16x8 Frag; typedef f16x4 Quad; typedef _Float16 Elem; static constexpr int kPlanes = 1, kLift = 15; };
 template <> struct AtType<float> { typedef AtPieces Frag; typedef f32x4 Quad; typedef __bf16 Elem; static constexpr int kPlanes = 3, kLift = 0; };
@@ -43,6 +45,23 @@ __device__ __forceinline__ void at_mma(f32x4& acc, const f16x8& a, const f16x8& 
 __device__ __forceinline__ void at_mma(f32x4& acc, const AtPieces& a, const AtPieces& b) {
     at_mma(acc, a.p[0], b.p[2]); at_mma(acc, a.p[1], b.p[1]); at_mma(acc, a.p[2], b.p[0]);
     at_mma(acc, a.p[0], b.p[1]); at_mma(acc, a.p[1], b.p[0]); at_mma(acc, a.p[0], b.p[0]);
+}
+
+// the same with the parts joined by ordinary additions: the matrix pipe rounds a chain of sums to one side, which a sum over 10^8 values
+// that cancel does not forgive
+template <typename F>
+__device__ __forceinline__ void at_mma_apart(f32x4& acc, const F& a, const F& b) {
+    f32x4 part = {0.f, 0.f, 0.f, 0.f};
+    at_mma(part, a, b);
+    acc += part;
+}
+__device__ __forceinline__ void at_mma_apart(f32x4& acc, const AtPieces& a, const AtPieces& b) {
+    f32x4 low = {0.f, 0.f, 0.f, 0.f}, part = low;
+    at_mma(low, a.p[0], b.p[2]); at_mma(low, a.p[1], b.p[1]); at_mma(low, a.p[2], b.p[0]);
+    at_mma(low, a.p[0], b.p[1]); at_mma(low, a.p[1], b.p[0]);
+    at_mma(part, a.p[0], b.p[0]);
+    acc += low;
+    acc += part;
 }
 
 // x into its pieces; a value that is not finite goes into the first alone (so that it stays what it is), and one that rounds beyond
@@ -88,6 +107,13 @@ __device__ __forceinline__ void at_pack_rest(F& rest, const F& piece, const f32x
     at_pack(rest, v - __builtin_convertvector(piece, f32x8));
 }
 
+// a value that only the branch it stands in knows: keeps a rarely taken branch a branch (the compiler would turn it into selections that
+// every pass pays for)
+__device__ __forceinline__ int at_here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // A probability is exp2(s scale2 - base) with one rounding (fma).  Where the base is so large that the rounding of base alone is a factor
 // (|base| > 2^20: differences of such scores are whole powers of two anyway) the product is rounded first, so that the scores the base was
 // formed from give 1.  Returns the factor that is left for the fma.
@@ -95,10 +121,11 @@ constexpr float kHuge = 1048576.f;
 template <int N>
 __device__ __forceinline__ float at_scale(f32x4 (&s)[N], float scale2, bool huge) {
     if (!huge) return scale2;
+    const float f = __builtin_bit_cast(float, at_here(__builtin_bit_cast(int, scale2)));
 #pragma unroll
     for (int b = 0; b < N; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[b][e] = __fmul_rn(s[b][e], scale2);
+        for (int e = 0; e < 4; ++e) s[b][e] = __fmul_rn(s[b][e], f);
     return 1.f;
 }
 __device__ __forceinline__ bool at_huge(float base) { return __any(fabsf(base) > kHuge && fabsf(base) < INFINITY); }

@@ -70,9 +70,26 @@ inline int at_bwd_heads(int most, int heads, int share, int mode) {      // whol
     return mode != kNone && heads % most == 0 && (share == 1 || share % most == 0) ? most : 1;
 }
 
+// Adds four values to words bucket[e] * 64 of a lane's own column.  (LDS float atomics take some 240 cycles a wave: 15.9 ms of the
+// gradient of 3 10^8 pairs x 8 heads; plain reads and writes of a private column need no atomic.)  Writes of a wave happen in order, so
+// of equal buckets the last one has to hold the sum of them all.
+__device__ __forceinline__ void at_hist(float* __restrict__ column, const int (&bucket)[4], const f32x4& v) {
+    float old[4], sum[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) old[e] = column[bucket[e] * 64];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        sum[e] = v[e];
+#pragma unroll
+        for (int f = 0; f < e; ++f) sum[e] += bucket[f] == bucket[e] ? v[f] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) column[bucket[e] * 64] = old[e] + sum[e];
+}
+
 // one workgroup: 64 queries of one scan x HG heads: dq, delta, and its part of the table's gradient
 template <typename T, int DP, int HG, int SLOTS, int BIAS, bool GRAD, int ROWS, int NBUF>
-__global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
+__global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_kernel(const AtBwd a) {
     constexpr int DC = DP / 32, DB = DP / 16;
     typedef AtTile<T, DP, SLOTS, ROWS> Tile;
     typedef typename AtType<T>::Frag Frag;
@@ -104,7 +121,9 @@ __global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
     Frag qf[HG][DC], gf[HG][DC];
     float lse[HG], slope[HG], unlift[HG];
     bool huge[HG];
-    f32x4 down[HG];                                            // -delta, what the products do . v start from
+    // -delta: what the products do . v start from.  (With the table's gradient it is added behind them: the matrix pipe rounds sums to one
+    // side, and what is the same for every pair does not cancel in a sum over 10^8 of them -- 1.9e-5 of the gradient against 1.2e-6.)
+    f32x4 down[HG];
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
         float sum = 0.f, g2 = 0.f;
@@ -211,12 +230,13 @@ __global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         s[b] = pairs[b].start(slope[h], table + h * a.bias.buckets);
-                        dp[b] = down[h];
+                        dp[b] = GRAD ? f32x4{0.f, 0.f, 0.f, 0.f} : down[h];
 #pragma unroll
                         for (int c = 0; c < DC; ++c) {
                             const int at = Tile::at_rows(slot, 2 * j + b, c);
                             at_mma(s[b], Tile::frag(kt, at), qf[h][c]);
-                            at_mma(dp[b], Tile::frag(vt, at), gf[h][c]);
+                            if (GRAD) at_mma_apart(dp[b], Tile::frag(vt, at), gf[h][c]);
+                            else at_mma(dp[b], Tile::frag(vt, at), gf[h][c]);
                         }
                     }
                     const float factor = at_scale(s, scale2, huge[h]);
@@ -224,13 +244,24 @@ __global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
                     for (int b = 0; b < 2; ++b) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            float p = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][e], factor, -lse[h]));
-                            if (left < ROWS && 32 * j + 16 * b + 4 * g + e >= left) p = 0.f;
-                            s[b][e] = p * dp[b][e];
-                            if (GRAD)
-                                __hip_atomic_fetch_add(mine + (pairs[b].b[e] + h * a.bias.buckets) * 64, kLifted ? s[b][e] * unlift[h] : s[b][e], __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_WORKGROUP);
+                            s[b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][e], factor, -lse[h]));
                         }
+                    }
+                    if (left < ROWS) {
+                        const int end = at_here(left);
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (32 * j + 16 * b + 4 * g + e >= end) s[b][e] = 0.f;
+                    }
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[b][e] *= GRAD ? dp[b][e] + down[h][e] : dp[b][e];
+                        }
+                        if (GRAD) at_hist(mine + h * a.bias.buckets * 64, pairs[b].b, kLifted ? s[b] * unlift[h] : s[b]);
                     }
                     Frag p;
                     at_pack(p, at_join(s[0], s[1]));
@@ -264,7 +295,7 @@ __global__ __launch_bounds__(kAtBlock) void at_bwd_q_kernel(const AtBwd a) {
 
 // one workgroup: 64 keys of one scan x SLOTS key heads x one share of the queries: dk, dv
 template <typename T, int DP, int HG, int SLOTS, int BIAS, int NBUF>
-__global__ __launch_bounds__(kAtBlock) void at_bwd_kv_kernel(const AtBwd a) {
+__global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_kv_kernel(const AtBwd a) {
     constexpr int ROWS = 64, DC = DP / 32, DB = DP / 16;
     typedef AtTile<T, DP, HG, ROWS> Tile;
     typedef typename AtType<T>::Frag Frag;
@@ -400,12 +431,21 @@ __global__ __launch_bounds__(kAtBlock) void at_bwd_kv_kernel(const AtBwd a) {
                             const float factor = at_scale(one, scale2, huge);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                float p = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][e], factor, -lse[e]));
-                                if (left < ROWS && 32 * j + 16 * b + 4 * g + e >= left) p = 0.f;
-                                s[b][e] = p;
-                                dp[b][e] = p * dp[b][e];
-                                if (kLifted) dp[b][e] *= ds_lift[slot];
+                                s[b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][e], factor, -lse[e]));
                             }
+                        }
+                        if (left < ROWS) {
+                            const int end = at_here(left);
+#pragma unroll
+                            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (32 * j + 16 * b + 4 * g + e >= end) s[b][e] = 0.f;
+                        }
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            dp[b] *= s[b];
+                            if (kLifted) dp[b] *= ds_lift[slot];
                         }
                         Frag p, ds;
                         at_pack(p, at_join(s[0], s[1]));

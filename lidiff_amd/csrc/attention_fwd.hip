@@ -48,13 +48,13 @@ inline int at_fwd_heads(int most, int heads, int share, int mode) {      // whol
 // rest.  d table sums ds over millions of pairs whose rows cancel to zero through delta = do . out, so an output from probabilities of 8 or
 // 11 bits costs it more than fp32 sums do.
 template <typename T, int DP, int HG, int SLOTS, int BIAS, int QB, int NBUF, bool EXACT>
-__global__ __launch_bounds__(kAtBlock) void at_fwd_kernel(const AtFwd a) {
+__global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kernel(const AtFwd a) {
     constexpr int ROWS = kFwdRows, DC = DP / 32, DB = DP / 16, KB = ROWS / 16;
     typedef AtTile<T, DP, SLOTS, ROWS> Tile;
     typedef typename AtType<T>::Frag Frag;
     // (7, not 15: a probability may exceed the base's by 2^8)
     constexpr float kLift = AtType<T>::kLift ? 7.f : 0.f, kUnlift = AtType<T>::kLift ? 1.f / 128.f : 1.f, kSlack = 8.f;
-    constexpr bool kOnes = sizeof(T) == 2;
+    constexpr bool kOnes = sizeof(T) == 2 && !EXACT, kTwoLevels = sizeof(T) == 4 || EXACT;
     extern __shared__ __align__(16) char at_sm[];
     char* const ks = at_sm;                                                       // [NBUF] keys, [NBUF] values
     char* const vs = ks + NBUF * Tile::kBytes;
@@ -174,13 +174,14 @@ __global__ __launch_bounds__(kAtBlock) void at_fwd_kernel(const AtFwd a) {
                     }
                 }
                 if (left < ROWS) {
+                    const int end = at_here(left);
 #pragma unroll
                     for (int n = 0; n < QB; ++n)
 #pragma unroll
                         for (int b = 0; b < KB; ++b)
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                if (16 * b + 4 * g + e >= left) s[n][b][e] = -INFINITY;
+                                if (16 * b + 4 * g + e >= end) s[n][b][e] = -INFINITY;
                 }
                 constexpr int PIECES = EXACT ? 2 : 1;
                 Frag p[QB][KB / 2][PIECES];
@@ -221,6 +222,12 @@ __global__ __launch_bounds__(kAtBlock) void at_fwd_kernel(const AtFwd a) {
                         }
                     }
                 }
+                // (kTwoLevels: the matrix pipe rounds a long chain of sums to one side; where fp32 is asked for, a tile is summed by itself)
+                f32x4 part[QB][DB];
+#pragma unroll
+                for (int n = 0; n < QB; ++n)
+#pragma unroll
+                    for (int b = 0; b < DB; ++b) part[n][b] = kTwoLevels ? f32x4{0.f, 0.f, 0.f, 0.f} : o[n][h][b];
 #pragma unroll
                 for (int j = 0; j < KB / 2; ++j)
 #pragma unroll
@@ -229,8 +236,12 @@ __global__ __launch_bounds__(kAtBlock) void at_fwd_kernel(const AtFwd a) {
 #pragma unroll
                         for (int n = 0; n < QB; ++n)
 #pragma unroll
-                            for (int i = 0; i < PIECES; ++i) at_mma(o[n][h][b], vf, p[n][j][i]);
+                            for (int i = 0; i < PIECES; ++i) at_mma(part[n][b], vf, p[n][j][i]);
                     }
+#pragma unroll
+                for (int n = 0; n < QB; ++n)
+#pragma unroll
+                    for (int b = 0; b < DB; ++b) o[n][h][b] = kTwoLevels ? o[n][h][b] + part[n][b] : part[n][b];
             }
         }
         if (NBUF == 1 && tile + 1 < last) {
