@@ -11,6 +11,9 @@ Symbols (reference call sites, paths relative to /root/reference/lidiff):
   ME.MinkowskiReLU, ME.cat                minkunet.py:24,464
   ME.SparseTensorQuantizationMode, ME.MinkowskiAlgorithm   pipeline:77-78
 
+Beyond the reference (named and used as its neighbours are): ME.MinkowskiGroupNorm, ME.MinkowskiAttention -- statistics and attention
+per scan of a batch.
+
 Everything runs on the GPU through the C ABI in include/lidiff_amd.h (hand-written HIP
 kernels); there is no CPU path.  Row order is deterministic: first occurrence in point
 order (level 0) / in finer-row order (strided maps) -- SURVEY.md Appendix A.7.
@@ -91,6 +94,7 @@ class CoordinateManager:
         self.hints = None               # [rows of levels 0 .. 4, tail pairs of levels 0, 1] believed by the host
         self.exact_rows = None          # strides whose rows must come out EXACTLY as hinted (the condition's latent), checked later
         self.hint_lag = False           # exact sizes, but kernel choices from `hints` (the A/B twin of read_free: same choices)
+        self.batches = None             # batch indices lie in [0, batches): set where it is known, else read once (n_batches)
         self.lane_up_orders = True      # a pyramid built in lanes also builds the decoder's offset-grouped pair lists (up_order)
 
     def rows(self, ts: int) -> int:
@@ -108,6 +112,31 @@ class CoordinateManager:
     def count(self, ts: int):
         """int32 [1] device tensor with the valid rows of a read-free map, None for a map of exact size."""
         return self.maps[ts].count
+
+    def n_batches(self) -> int:
+        """How many batch indices the field's rows may have (the largest one + 1).  Read from the device once per manager, unless whoever
+        made the field knew it (`batches`); rows that are not grouped by ascending batch index raise ValueError there."""
+        if self.batches is None:
+            from .. import _lib
+            self._acquire(1)
+            _lib.join_pending()
+            m = self.maps[1]
+            seg = ops.batch_segments(m.coords, None, d_rows=m.count)
+            self.batches = seg.shape[0]
+            if m.count is None:
+                self.aux[("segments", 1, 1, self.batches)] = seg
+        return self.batches
+
+    def segments(self, ts: int, replicas: int = 1, n_batches: int | None = None):
+        """int32 [replicas * batches, 2]: the rows of every scan on the map of stride ts (ops.batch_segments), once per map."""
+        n = max(self.n_batches(), n_batches or 0)
+        key = ("segments", ts, replicas, n)
+        hit = self.aux.get(key)
+        if hit is None:
+            self._acquire(ts)
+            m = self.maps[ts]
+            hit = self.aux[key] = ops.batch_segments(m.coords, n, d_rows=m.count, replicas=replicas, status=self.status)
+        return hit
 
     def tail_rows(self, ts: int):
         """Believed pair count of the tail map of stride ts (profiler bookkeeping only)."""
@@ -468,6 +497,8 @@ class CoordinateManager:
             raise RuntimeError("coordinate hash table overflow")
         if s & ops.STATUS_BOUND:
             raise RuntimeError("a device-side count exceeded the bound of a host-read-free step (the step must be redone)")
+        if s & ops.STATUS_BATCH_ORDER:
+            raise RuntimeError("rows of a coordinate map are not grouped by ascending batch index")
 
 
 # ----------------------------------------------------------------------------------------
@@ -684,6 +715,10 @@ class SparseTensor:
             other = other.F
         return self._like(self._F + other)
 
+    def segments(self, n_batches: int | None = None) -> torch.Tensor:
+        """The rows of every scan (and replica) of this tensor: int32 [replicas * batches, 2], first row and the row behind the last."""
+        return self.coordinate_manager.segments(self.tensor_stride, self.replicas, n_batches)
+
     def slice(self, field: TensorField) -> TensorField:
         """F_vox[inverse_mapping] -> per-point features (minkunet.py:497,619)."""
         if field.coordinate_manager is not self.coordinate_manager or self.tensor_stride != 1:
@@ -853,3 +888,87 @@ class MinkowskiReLU(nn.Module):
 
     def forward(self, x: SparseTensor) -> SparseTensor:
         return x._like(torch.relu(x.F))
+
+
+class MinkowskiGroupNorm(nn.Module):
+    """Group normalisation of the features per scan of the batch (ops.group_norm), with an optional fused activation (None, "relu",
+    "silu").  Unlike MinkowskiBatchNorm it has no running estimates and no dependence on the other scans of a batch or on other ranks:
+    training and inference are the same function.  Parameters `weight`, `bias` as nn.GroupNorm names them."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation=None):
+        super().__init__()
+        if num_groups < 1 or num_channels % num_groups:
+            raise ValueError(f"{num_groups} groups do not divide {num_channels} channels")
+        if activation not in (None, "relu", "silu"):
+            raise ValueError(f"activation must be None, 'relu' or 'silu', got {activation!r}")
+        self.num_groups, self.num_channels, self.eps, self.activation = num_groups, num_channels, eps, activation
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+
+    def forward(self, x: SparseTensor) -> SparseTensor:
+        return x._like(ops.group_norm(x.F, self.num_groups, self.weight, self.bias, segments=x.segments(), eps=self.eps,
+                                      activation=self.activation))
+
+    def extra_repr(self):
+        return f"{self.num_groups}, {self.num_channels}, eps={self.eps}, activation={self.activation}"
+
+
+class MinkowskiAttention(nn.Module):
+    """The attention block of diffusion UNets on voxel rows: x + proj(attention(q(norm(x)), kv(norm(context)))), then x + feed(silu norm(x)).
+    A row attends to the rows of its own scan -- of x itself, or (context_channels) of a second tensor on a map of its own, e.g. the
+    latent of the partial scan -- with a learned bias by distance buckets (ops.segment_attention; `unit`: the bucket width in voxels,
+    the tensor stride of the block's map).  Both branches start at zero: a new block is the identity."""
+
+    def __init__(self, channels, num_heads, context_channels=None, num_kv_heads=None, num_groups=32, num_buckets=32, reach=100, unit=1):
+        super().__init__()
+        kv_heads = num_kv_heads or num_heads
+        if channels % num_heads or num_heads % kv_heads:
+            raise ValueError(f"{num_heads} heads ({kv_heads} key heads) do not divide {channels} channels")
+        self.num_heads, self.kv_heads, self.dim = num_heads, kv_heads, channels // num_heads
+        if self.dim % 8 or self.dim > 128:
+            raise ValueError(f"the head dimension must be a multiple of 8 up to 128, got {self.dim}")
+        self.edges = ops.distance_edges(num_buckets, reach, unit)
+        norm = lambda c, act=None: MinkowskiGroupNorm(math.gcd(num_groups, c), c, activation=act)
+        self.norm = norm(channels)
+        self.norm_context = None if context_channels is None else norm(context_channels)
+        self.to_q = nn.Linear(channels, channels, bias=False)
+        self.to_kv = nn.Linear(channels if context_channels is None else context_channels, 2 * kv_heads * self.dim, bias=False)
+        self.proj = nn.Linear(channels, channels)
+        self.distance_bias = nn.Parameter(torch.zeros(num_buckets, num_heads))
+        self.norm_feed = norm(channels, "silu")
+        self.feed = nn.Linear(channels, channels)
+        for lin in (self.proj, self.feed):
+            nn.init.zeros_(lin.weight)
+            nn.init.zeros_(lin.bias)
+
+    def forward(self, x: SparseTensor, context=None) -> SparseTensor:
+        """context: a SparseTensor, or a tuple of them, one per replica of x (a guidance pair)."""
+        if (context is None) != (self.norm_context is None):
+            raise ValueError("this block was built " + ("without" if self.norm_context is None else "with") + " a context")
+        parts = () if context is None else tuple(context) if isinstance(context, (tuple, list)) else (context,)
+        if parts and len(parts) != x.replicas:
+            raise ValueError(f"{x.replicas} replicas need as many contexts, got {len(parts)}")
+        n = max(t.coordinate_manager.n_batches() for t in (x,) + parts)
+        seg_q = x.segments(n)
+        coords_q = x.C if x.replicas == 1 else x.C.repeat(x.replicas, 1)
+        h = self.norm(x).F
+        if parts:
+            rows = [t.F.shape[0] for t in parts]
+            segs = [t.segments(n) for t in parts]
+            normed = [self.norm_context(t).F for t in parts]
+            starts = [sum(rows[:i]) for i in range(len(rows))]
+            seg_k = segs[0] if len(parts) == 1 else torch.cat([s + lo for s, lo in zip(segs, starts)])
+            coords_k = parts[0].C if len(parts) == 1 else torch.cat([t.C for t in parts])
+            source = normed[0] if len(parts) == 1 else torch.cat(normed)
+        else:
+            seg_k, coords_k, source = seg_q, coords_q, h
+        # bf16 training: the projections' GEMMs and the attention take bf16 operands, sums and statistics stay fp32
+        low = ops.TRAIN_OPERANDS == "bf16" and torch.is_grad_enabled() and x.F.is_cuda
+        with torch.autocast("cuda", dtype=torch.bfloat16) if low else contextlib.nullcontext():
+            q = self.to_q(h).view(-1, self.num_heads, self.dim)
+            k, v = self.to_kv(source).view(-1, 2, self.kv_heads, self.dim).unbind(1)
+            out = ops.segment_attention(q, k, v, seg_q, seg_k, coords_q=coords_q, coords_k=coords_k, bias=self.distance_bias, edges=self.edges)
+            y = x._like(x.F + self.proj(out.flatten(1)).float())
+        fed = self.norm_feed(y).F
+        with torch.autocast("cuda", dtype=torch.bfloat16) if low else contextlib.nullcontext():
+            return y._like(y.F + self.feed(fed).float())

@@ -67,7 +67,8 @@ class DiffusionPoints(nn.Module):
         self.dpm_scheduler.set_timesteps(self.s_steps)
         out_dim = self.hparams["model"]["out_dim"]
         self.partial_enc = minknet.MinkGlobalEnc(in_channels=3, out_channels=out_dim)
-        self.model = minknet.MinkUNetDiff(in_channels=3, out_channels=out_dim)
+        self.model = minknet.MinkUNetDiff(in_channels=3, out_channels=out_dim,
+                                          attention_heads=self.hparams["model"].get("attention_heads", 0))
         self.w_uncond = self.hparams["train"]["uncond_w"]
         self.to(self.device)
 
@@ -182,7 +183,8 @@ class RefineDiffusion(nn.Module):
         super().__init__()
         self.hparams = _merge(REFINE_HPARAMS, hparams or {})
         self.device = torch.device(device)
-        self.model_refine = minknet.MinkUNet(in_channels=3, out_channels=3 * self.hparams["train"]["up_factor"])
+        self.model_refine = minknet.MinkUNet(in_channels=3, out_channels=3 * self.hparams["train"]["up_factor"],
+                                             attention_heads=self.hparams.get("model", {}).get("attention_heads", 0))
         self.to(self.device)
 
     def forward_refine(self, x):

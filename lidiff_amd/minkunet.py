@@ -8,6 +8,9 @@ unchanged), same forward semantics:
   BasicDeconvolutionBlock minkunet.py:32-46      MinkUNetDiff    minkunet.py:144-497
   ResidualBlock           minkunet.py:49-80      MinkUNet        minkunet.py:500-619
 
+Both UNets take attention_heads (default 0: the reference's networks, same state dict): an attention block at the coarsest level
+(ME.MinkowskiAttention), on the partial scan's latent in MinkUNetDiff.
+
 What is different is the execution plan in eval mode under ``torch.no_grad()`` (the default):
   * eval-mode BatchNorm, ReLU and the residual add are folded into the sparse-conv epilogue
     (one HBM round trip per conv instead of four);
@@ -412,6 +415,10 @@ class MinkUNetDiff(_Base):
                 j = i - 4
                 setattr(self, name, _up(cs[4 + j], cs[5 + j], cs[3 - j], self.D))
         self.last = _mlp(cs[8], 20, 3)
+        # beyond the reference: attention_heads > 0 puts an attention block behind stage4 -- every stride-16 voxel reads the whole latent
+        # of its scan, weighted by content and distance, where the conditioning takes the nearest part voxel only
+        heads = kwargs.get("attention_heads", 0)
+        self.attention = ME.MinkowskiAttention(cs[4], heads, context_channels=lat, unit=16) if heads else None
         self.weight_initialization()
 
     # -- minkunet.py:390-401 --------------------------------------------------------------
@@ -648,6 +655,8 @@ class MinkUNetDiff(_Base):
             feats.append(getattr(self, name)(cond))
             mark(f"unet: {name}")
         y = feats[4]
+        if self.attention is not None:
+            y = self.attention(y, part_feats)
         for j, name in enumerate(_LEVELS[4:]):
             y = _run_up(getattr(self, name), self._condition(name, y, part_feats, temp_emb), feats[3 - j])
         if _fusable(self):
@@ -678,6 +687,8 @@ class MinkUNet(_Base):
         for j in range(4):
             setattr(self, f"up{j + 1}", _up(cs[4 + j], cs[5 + j], cs[3 - j], self.D))
         self.last = _mlp(cs[8], 20, kwargs.get("out_channels", 3), tail=nn.Tanh())
+        heads = kwargs.get("attention_heads", 0)              # beyond the reference: self-attention of the stride-16 rows, 0: none
+        self.attention = ME.MinkowskiAttention(cs[4], heads, unit=16) if heads else None
         self.weight_initialization()
         self.dropout = nn.Dropout(0.3, True)
 
@@ -686,6 +697,8 @@ class MinkUNet(_Base):
         for n in (1, 2, 3, 4):
             feats.append(getattr(self, f"stage{n}")(feats[-1]))
         y = feats[4]
+        if self.attention is not None:
+            y = self.attention(y)
         for j in range(4):
             y = _run_up(getattr(self, f"up{j + 1}"), y, feats[3 - j])
         if _fusable(self):

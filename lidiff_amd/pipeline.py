@@ -42,8 +42,10 @@ class DiffCompletion(nn.Module):
             f"The number of denoising steps cannot be bigger than T={self.hparams['diff']['t_steps']}"
         out_dim = self.hparams["model"]["out_dim"]
         self.partial_enc = minknet.MinkGlobalEnc(in_channels=3, out_channels=out_dim)
-        self.model = minknet.MinkUNetDiff(in_channels=3, out_channels=out_dim)
-        self.model_refine = minknet.MinkUNet(in_channels=3, out_channels=3 * 6)
+        self.model = minknet.MinkUNetDiff(in_channels=3, out_channels=out_dim,
+                                          attention_heads=self.hparams["model"].get("attention_heads", 0))
+        self.model_refine = minknet.MinkUNet(in_channels=3, out_channels=3 * 6,
+                                             attention_heads=self.hparams["model"].get("refine_attention_heads", 0))
         if ckpt_diff is not None:
             self.load_state_dict(ckpt_diff["state_dict"], strict=False)
         if refine_path:
@@ -141,16 +143,18 @@ class DiffCompletion(nn.Module):
                 and points.shape[2] == 3 and points.dtype in (torch.float32, torch.float64)):
             from . import ops
             feats, coords = ops.points_to_field(points.detach(), self.hparams["data"]["resolution"], scale_batch_column=True)
-            return self._make_field(feats, coords, role)
+            return self._make_field(feats, coords, role, scans=points.shape[0])
         x_feats = ME.utils.batched_coordinates(list(points[:]), dtype=torch.float32, device=self.device)
         x_coord = torch.round(x_feats / self.hparams["data"]["resolution"])
-        return self._make_field(x_feats[:, 1:], x_coord, role)
+        return self._make_field(x_feats[:, 1:], x_coord, role, scans=len(points))
 
-    def _make_field(self, feats, coords, role=None):
+    def _make_field(self, feats, coords, role=None, scans=None):
         field = ME.TensorField(features=feats, coordinates=coords,
                                quantization_mode=ME.SparseTensorQuantizationMode.UNWEIGHTED_AVERAGE,
                                minkowski_algorithm=ME.MinkowskiAlgorithm.SPEED_OPTIMIZED, device=self.device)
         mgr = field.coordinate_manager
+        if scans == 1:
+            mgr.batches = 1              # (known here: no host read for the scans' row ranges; several scans: CoordinateManager.n_batches)
         mgr.pyramid = self.single_read and field.F.device.type == "cuda"
         if (role is not None and mgr.pyramid and (self.read_free or self.hint_lag) and self.pair_cfg and minknet._FUSION
                 and not self.training and feats.shape[0] >= 1):
@@ -563,7 +567,7 @@ class DiffCompletion(nn.Module):
             x0, feats, coords = ops.cfg_dpm_step(e_cond, e_uncond, self.w_uncond, x_t.F, x_init, sch.step_plan(t_int), noise,
                                                  self.hparams["data"]["resolution"], scale_batch_column=True)
             sch.commit(x0)
-            return self._make_field(feats, coords, "x_t")
+            return self._make_field(feats, coords, "x_t", scans=x_init.shape[0])
         noise_t = e_uncond + self.w_uncond * (e_cond - e_uncond)
         input_noise = x_t.F.reshape(x_init.shape[0], -1, 3) - x_init
         x_new = x_init + sch.step(noise_t, t_int, input_noise, noise=noise)["prev_sample"]

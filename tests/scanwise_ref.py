@@ -146,3 +146,37 @@ def assert_within(got, val, bnd, floor, what):
     off = (got - val).abs() - bnd - floor
     worst = off.max().item() if off.numel() else -1.0
     assert worst <= 0, f"{what}: {worst:.3e} beyond its bound (largest error {(got - val).abs().max().item():.3e})"
+
+
+# -- the operators as differentiable 64-bit torch code, with ops' signatures (stand-ins inside a model) ---------------------------------------
+def plain_group_norm(x, num_groups, weight=None, bias=None, segments=None, eps=1e-5, activation=None):
+    out = torch.zeros_like(x, dtype=torch.float64)
+    for lo, hi in [(0, x.shape[0])] if segments is None else segments.tolist():
+        if hi <= lo:
+            continue
+        g = x[lo:hi].double().reshape(hi - lo, num_groups, -1)
+        z = ((g - g.mean((0, 2), keepdim=True)) / torch.sqrt(g.var((0, 2), unbiased=False, keepdim=True) + eps)).flatten(1)
+        z = z * (1 if weight is None else weight.double()) + (0 if bias is None else bias.double())
+        rows = torch.arange(lo, hi, device=x.device)
+        out = out.index_copy(0, rows, {None: z, "relu": z.relu(), "silu": z * torch.sigmoid(z)}[activation])
+    return out.to(x.dtype)
+
+
+def plain_segment_attention(q, k, v, seg_q=None, seg_k=None, *, coords_q=None, coords_k=None, slopes=None, bias=None, edges=None, scale=None):
+    heads, share = q.shape[1], q.shape[1] // k.shape[1]
+    scale = 1 / math.sqrt(q.shape[2]) if scale is None else scale
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    for (q0, q1), (k0, k1) in zip([(0, q.shape[0])] if seg_q is None else seg_q.tolist(), [(0, k.shape[0])] if seg_k is None else seg_k.tolist()):
+        if q1 <= q0 or k1 <= k0:
+            continue
+        Q, K, V = (t.double().transpose(0, 1).contiguous() for t in (q[q0:q1], k[k0:k1].repeat_interleave(share, 1), v[k0:k1].repeat_interleave(share, 1)))
+        s = torch.matmul(Q, K.transpose(1, 2).contiguous()) * scale
+        if slopes is not None or bias is not None:
+            d2 = distance2(coords_q[q0:q1], coords_k[k0:k1])
+            if slopes is not None:
+                s = s - slopes.double()[:, None, None] * d2.double().sqrt()
+            else:
+                s = s + bias.double()[torch.bucketize(d2, torch.tensor(edges, dtype=torch.int64, device=q.device), right=True)].permute(2, 0, 1)
+        o = torch.matmul(torch.softmax(s, 2), V).transpose(0, 1)
+        out = out.index_copy(0, torch.arange(q0, q1, device=q.device), o)
+    return out.to(q.dtype)
