@@ -113,6 +113,7 @@ __device__ __forceinline__ int at_here(int v) {
     asm volatile("" : "+v"(v));
     return v;
 }
+__device__ __forceinline__ void at_here(f32x4& v) { asm volatile("" : "+v"(v)); }
 
 // A probability is exp2(s scale2 - base) with one rounding (fma).  Where the base is so large that the rounding of base alone is a factor
 // (|base| > 2^20: differences of such scores are whole powers of two anyway) the product is rounded first, so that the scores the base was
@@ -124,8 +125,11 @@ __device__ __forceinline__ float at_scale(f32x4 (&s)[N], float scale2, bool huge
     const float f = __builtin_bit_cast(float, at_here(__builtin_bit_cast(int, scale2)));
 #pragma unroll
     for (int b = 0; b < N; ++b)
+    {
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[b][e] = __fmul_rn(s[b][e], f);
+        at_here(s[b]);
+    }
     return 1.f;
 }
 __device__ __forceinline__ bool at_huge(float base) { return __any(fabsf(base) > kHuge && fabsf(base) < INFINITY); }
@@ -158,19 +162,20 @@ struct AtTile {
 
     __device__ static __forceinline__ int swz(int row) { return (row / RP) & (CH - 1); }
 
-    // Requests rows [lo, lo + left) of heads h0 .. h0 + SLOTS - 1 straight into LDS (no registers, no waiting: at_arrive()).  The
+    // Requests `left` rows from `at` (the first row of the tile's first head) straight into LDS: no registers, no waiting (AT_ARRIVE).  The
     // descriptor ends with the last of these rows and pieces beyond `dim` are addressed out of its range: both arrive as zeros.
-    __device__ static __forceinline__ void request(const AtRows& src, int h0, int dim, int lo, int left, unsigned lds) {
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
+    __device__ static __forceinline__ void request(const AtRows& src, const char* at, int dim, int left, unsigned lds) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), end = (left - 1) * (int)src.row + dim * 2;
 #pragma unroll
         for (int n = 0; n < (N + kAtBlock - 1) / kAtBlock; ++n) {
             const int first = n * kAtBlock + wave * kWave;
             if (N % kAtBlock && first >= N) break;
-            const int ps = first / (CH * ROWS), slot = ps % SLOTS, plane = ps / SLOTS;
+            // (kAtBlock pieces are a whole number of a head's rows, or a head's rows are fewer: then two waves share one)
+            const int ps = ROWS * CH >= kAtBlock ? n * kAtBlock / (CH * ROWS) : first / (CH * ROWS), slot = ps % SLOTS, plane = ps / SLOTS;
             const int row = (first + lane) / CH % ROWS, c = (lane % CH) ^ swz(row);
-            const uint64_t base = (uint64_t)(uintptr_t)src.p + (int64_t)lo * src.row + (int64_t)(h0 + slot) * src.head + plane * src.plane;
+            const uint64_t base = (uint64_t)(uintptr_t)at + slot * src.head + plane * src.plane;
             const int voff = c * 8 < dim ? row * (int)src.row + c * 16 : (int)0x80000000;
-            i32x4 rsrc = {(int)(uint32_t)base, (int)(uint32_t)((base >> 32) & 0xffffu), (left - 1) * (int)src.row + dim * 2, 0x00020000};
+            i32x4 rsrc = {(int)(uint32_t)base, (int)(uint32_t)((base >> 32) & 0xffffu), end, 0x00020000};
 #pragma unroll
             for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
             asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
@@ -178,39 +183,43 @@ struct AtTile {
         }
     }
 
-    // byte offset of lane's part of rows 16 b + (lane & 15), elements 32 c + 8 g ..: the A operand of a product over the elements
-    __device__ static __forceinline__ int at_rows(int slot, int b, int c) {
-        const int lane = lane_id(), row = 16 * b + (lane & 15);
-        return ((slot * ROWS + row) * CH + ((4 * c + (lane >> 4)) ^ swz(row))) * 16;
-    }
-    __device__ static __forceinline__ Frag frag(const char* tile, int off) {
-        if constexpr (P == 1) return *reinterpret_cast<const Frag*>(tile + off);
+    // A lane's places in any tile, formed once: blocks, heads and planes are constant distances from them (the swizzle of rows 16 b + r is
+    // that of r, and of rows 16 b + 4 g + r that of 4 g + r).
+    struct Lane {
+        int rows[DP / 32], turned[DP / 16];
+        __device__ __forceinline__ Lane() {
+            const int lane = lane_id(), i = lane & 15, g = lane >> 4, r = 4 * g + i / 4;
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) rows[c] = (i * CH + ((4 * c + g) ^ swz(i))) * 16;
+#pragma unroll
+            for (int b = 0; b < DP / 16; ++b) turned[b] = (r * CH + ((2 * b + (i % 4) / 2) ^ swz(r))) * 16 + (i & 1) * 8;
+        }
+    };
+    // rows 16 b + (lane & 15), elements 32 c + 8 g ..: the A operand of a product over the elements
+    __device__ static __forceinline__ Frag frag(const char* tile, const Lane& l, int slot, int b, int c) {
+        const char* p = tile + (slot * ROWS + 16 * b) * CH * 16 + l.rows[c];
+        if constexpr (P == 1) return *reinterpret_cast<const Frag*>(p);
         else {
             Frag f;
 #pragma unroll
-            for (int i = 0; i < P; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(tile + i * kPlane + off);
+            for (int i = 0; i < P; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(p + i * kPlane);
             return f;
         }
     }
-    // the A operand of a product over rows 32 j ..: elements 16 b + (lane & 15).  Sixteen lanes read four rows of sixteen elements,
-    // lane i row i / 4 and elements 4 (i % 4) .., and receive element i of each row.
-    __device__ static __forceinline__ i16x8 turned(const char* tile, int slot, int j, int b) {
-        const int lane = lane_id(), i = lane & 15, g = lane >> 4;
-        i16x4 r[2];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int row = 32 * j + 16 * half + 4 * g + i / 4, c = 2 * b + (i % 4) / 2;
-            const char* p = tile + ((slot * ROWS + row) * CH + (c ^ swz(row))) * 16 + (i & 1) * 8;
-            r[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(at_lds_t)p);
-        }
-        return __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    // The A operand of a product over rows 32 j ..: elements 16 b + (lane & 15).  Sixteen lanes read four rows of sixteen elements, lane i
+    // row i / 4 and elements 4 (i % 4) .., and receive element i of each row.
+    __device__ static __forceinline__ i16x8 turned(const char* p) {
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(at_lds_t)p);
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(at_lds_t)(p + 16 * CH * 16));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
-    __device__ static __forceinline__ Frag frag_turned(const char* tile, int slot, int j, int b) {
-        if constexpr (P == 1) return __builtin_bit_cast(Frag, turned(tile, slot, j, b));
+    __device__ static __forceinline__ Frag frag_turned(const char* tile, const Lane& l, int slot, int j, int b) {
+        const char* p = tile + (slot * ROWS + 32 * j) * CH * 16 + l.turned[b];
+        if constexpr (P == 1) return __builtin_bit_cast(Frag, turned(p));
         else {
             Frag f;
 #pragma unroll
-            for (int i = 0; i < P; ++i) f.p[i] = __builtin_bit_cast(bf16x8, turned(tile + i * kPlane, slot, j, b));
+            for (int i = 0; i < P; ++i) f.p[i] = __builtin_bit_cast(bf16x8, turned(p + i * kPlane));
             return f;
         }
     }

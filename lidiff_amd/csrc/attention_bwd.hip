@@ -57,13 +57,15 @@ __global__ __launch_bounds__(256) void at_bound_kernel(const T* __restrict__ src
     if (lane_id() == 0) atomicMax(bound + blockIdx.y / share, __builtin_bit_cast(unsigned, sum));
 }
 
-// what a workgroup takes: heads at a time (the distances of a pair are the same for every head), rows of a tile, buffers of it
+// What a workgroup takes: heads at a time (the distances of a pair are the same for every head), rows of a tile.  One buffer per tile, as in
+// the forward kernel (41 157 x 5 824 x 2, bf16, dq: 1.43 against 1.69 ms).
 template <typename T, int DP> struct AtBwdPlan {
     static constexpr int kHeads = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 ? 2 : 1;
+    static constexpr int kKeyHeads = kHeads > 2 ? 2 : kHeads;         // dk / dv: twice the accumulators (four waves a SIMD: 1.56 against 1.71 ms)
     static constexpr int kGradHeads = sizeof(T) == 4 ? 1 : DP == 32 ? 2 : 1;      // with the table's gradient: a histogram of 256 bytes a wave, bucket and head
     static constexpr int kGradRows = 32;
     static constexpr int kRows = 64;
-    static constexpr int kBuf = sizeof(T) == 4 ? 1 : 2;
+    static constexpr int kKeyWaves = sizeof(T) == 2 && DP == 32 ? 4 : at_waves(sizeof(T), DP);
 };
 
 inline int at_bwd_heads(int most, int heads, int share, int mode) {      // whole groups of one key head, or key heads of their own
@@ -88,7 +90,7 @@ __device__ __forceinline__ void at_hist(float* __restrict__ column, const int (&
 }
 
 // one workgroup: 64 queries of one scan x HG heads: dq, delta, and its part of the table's gradient
-template <typename T, int DP, int HG, int SLOTS, int BIAS, bool GRAD, int ROWS, int NBUF>
+template <typename T, int DP, int HG, int SLOTS, int BIAS, bool GRAD, int ROWS>
 __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_kernel(const AtBwd a) {
     constexpr int DC = DP / 32, DB = DP / 16;
     typedef AtTile<T, DP, SLOTS, ROWS> Tile;
@@ -96,8 +98,8 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
     constexpr bool kLifted = AtType<T>::kLift != 0;
     extern __shared__ __align__(16) char at_sm[];
     char* const ks = at_sm;
-    char* const vs = ks + NBUF * Tile::kBytes;
-    float* const cs = reinterpret_cast<float*>(vs + NBUF * Tile::kBytes);
+    char* const vs = ks + Tile::kBytes;
+    float* const cs = reinterpret_cast<float*>(vs + Tile::kBytes);
     unsigned* const cells = reinterpret_cast<unsigned*>(cs + 2 * 3 * ROWS);
     float* const table = reinterpret_cast<float*>(cells + (BIAS == kTable ? kCells : 0));
     float* const hist = table + (BIAS == kTable ? a.bias.buckets * HG : 0);              // [wave][HG][bucket][64 lanes]: a lane adds to words of its own
@@ -193,11 +195,15 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
         float* c = cs + (tile & 1) * 3 * ROWS + threadIdx.x;
         c[0] = (float)kc.y; c[ROWS] = (float)kc.z; c[2 * ROWS] = (float)kc.w;
     };
-    auto request = [&](int tile) {
-        const int lo = k_lo + tile * ROWS, left = min(ROWS, k_hi - lo), at = (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
-        Tile::request(a.ks, kv0, a.dim, lo, left, ks_at + at);
-        Tile::request(a.vs, kv0, a.dim, lo, left, vs_at + at);
+    const char *k_at = a.ks.p + (int64_t)k_lo * a.ks.row + kv0 * a.ks.head, *v_at = a.vs.p + (int64_t)k_lo * a.vs.row + kv0 * a.vs.head;
+    auto request = [&](int tile) {                             // (tile after tile)
+        const int left = min(ROWS, k_hi - (k_lo + tile * ROWS));
+        Tile::request(a.ks, k_at, a.dim, left, ks_at);
+        Tile::request(a.vs, v_at, a.dim, left, vs_at);
+        k_at += ROWS * a.ks.row;
+        v_at += ROWS * a.vs.row;
     };
+    const typename Tile::Lane place;
     if (last > 0) {
         coords(0);
         put_coords(0);
@@ -206,14 +212,11 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
     }
     for (int tile = 0; tile < last; ++tile) {
         AT_ARRIVE();
-        if (NBUF == 2 && tile + 1 < last) request(tile + 1);
         if (tile + 1 < last) {
             put_coords(tile + 1);
             coords(tile + 2);
         }
         if (q0 < t.hi) {
-            const char* const kt = ks + (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
-            const char* const vt = vs + (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
             const float* const ct = cs + (tile & 1) * 3 * ROWS;
             const int left = k_hi - (k_lo + tile * ROWS);
 #pragma unroll
@@ -233,10 +236,9 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                         dp[b] = GRAD ? f32x4{0.f, 0.f, 0.f, 0.f} : down[h];
 #pragma unroll
                         for (int c = 0; c < DC; ++c) {
-                            const int at = Tile::at_rows(slot, 2 * j + b, c);
-                            at_mma(s[b], Tile::frag(kt, at), qf[h][c]);
-                            if (GRAD) at_mma_apart(dp[b], Tile::frag(vt, at), gf[h][c]);
-                            else at_mma(dp[b], Tile::frag(vt, at), gf[h][c]);
+                            at_mma(s[b], Tile::frag(ks, place, slot, 2 * j + b, c), qf[h][c]);
+                            if (GRAD) at_mma_apart(dp[b], Tile::frag(vs, place, slot, 2 * j + b, c), gf[h][c]);
+                            else at_mma(dp[b], Tile::frag(vs, place, slot, 2 * j + b, c), gf[h][c]);
                         }
                     }
                     const float factor = at_scale(s, scale2, huge[h]);
@@ -250,10 +252,12 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                     if (left < ROWS) {
                         const int end = at_here(left);
 #pragma unroll
-                        for (int b = 0; b < 2; ++b)
+                        for (int b = 0; b < 2; ++b) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
                                 if (32 * j + 16 * b + 4 * g + e >= end) s[b][e] = 0.f;
+                            at_here(s[b]);
+                        }
                     }
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
@@ -266,11 +270,11 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                     Frag p;
                     at_pack(p, at_join(s[0], s[1]));
 #pragma unroll
-                    for (int b = 0; b < DB; ++b) at_mma(dq[h][b], Tile::frag_turned(kt, slot, j, b), p);
+                    for (int b = 0; b < DB; ++b) at_mma(dq[h][b], Tile::frag_turned(ks, place, slot, j, b), p);
                 }
             }
         }
-        if (NBUF == 1 && tile + 1 < last) {
+        if (tile + 1 < last) {
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the tile has been read
             request(tile + 1);
         }
@@ -294,17 +298,17 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
 }
 
 // one workgroup: 64 keys of one scan x SLOTS key heads x one share of the queries: dk, dv
-template <typename T, int DP, int HG, int SLOTS, int BIAS, int NBUF>
-__global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_kv_kernel(const AtBwd a) {
+template <typename T, int DP, int HG, int SLOTS, int BIAS>
+__global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bwd_kv_kernel(const AtBwd a) {
     constexpr int ROWS = 64, DC = DP / 32, DB = DP / 16;
     typedef AtTile<T, DP, HG, ROWS> Tile;
     typedef typename AtType<T>::Frag Frag;
     constexpr bool kLifted = AtType<T>::kLift != 0;
     extern __shared__ __align__(16) char at_sm[];
     char* const qs = at_sm;
-    char* const gs = qs + NBUF * Tile::kBytes;
-    float* const st = reinterpret_cast<float*>(gs + NBUF * Tile::kBytes);          // [NBUF][2][HG][64] lse, -delta
-    float* const cs = st + NBUF * 2 * HG * ROWS;
+    char* const gs = qs + Tile::kBytes;
+    float* const st = reinterpret_cast<float*>(gs + Tile::kBytes);                 // [2][HG][64] lse, -delta
+    float* const cs = st + 2 * HG * ROWS;
     unsigned* const cells = reinterpret_cast<unsigned*>(cs + 2 * 3 * ROWS);
     float* const table = reinterpret_cast<float*>(cells + (BIAS == kTable ? kCells : 0));
     const unsigned qs_at = (unsigned)(uintptr_t)(at_lds_t)qs, gs_at = (unsigned)(uintptr_t)(at_lds_t)gs, st_at = (unsigned)(uintptr_t)(at_lds_t)st;
@@ -352,6 +356,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_kv_k
     if (BIAS == kTable)
         for (int i = threadIdx.x; i < kCells; i += kAtBlock) cells[i] = a.bias.cells[i];
 
+    const typename Tile::Lane place;
     // the query heads that read these key heads, HG at a time
     for (int h0 = kv0 * a.share; h0 < (kv0 + SLOTS) * a.share; h0 += HG) {
         float slope[HG];
@@ -367,17 +372,20 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_kv_k
             float* c = cs + (tile & 1) * 3 * ROWS + threadIdx.x;
             c[0] = (float)qc.y; c[ROWS] = (float)qc.z; c[2 * ROWS] = (float)qc.w;
         };
-        auto request = [&](int tile) {
-            const int lo = q_lo + tile * ROWS, left = min(ROWS, q_hi - lo), buf = NBUF == 2 ? tile & 1 : 0;
-            Tile::request(a.qs, h0, a.dim, lo, left, qs_at + buf * Tile::kBytes);
-            Tile::request(a.gs, h0, a.dim, lo, left, gs_at + buf * Tile::kBytes);
+        const char *q_at = a.qs.p + (int64_t)(q_lo + first * ROWS) * a.qs.row + h0 * a.qs.head, *g_at = a.gs.p + (int64_t)(q_lo + first * ROWS) * a.gs.row + h0 * a.gs.head;
+        auto request = [&](int tile) {                         // (tile after tile)
+            const int lo = q_lo + tile * ROWS, left = min(ROWS, q_hi - lo);
+            Tile::request(a.qs, q_at, a.dim, left, qs_at);
+            Tile::request(a.gs, g_at, a.dim, left, gs_at);
+            q_at += ROWS * a.qs.row;
+            g_at += ROWS * a.gs.row;
             for (int i = wave; i < 2 * HG; i += 4) {           // lse and -delta: 64 words a head
                 const uint64_t base = (uint64_t)(uintptr_t)(a.stat + ((int64_t)(i / HG) * a.heads + h0 + i % HG) * a.mq + lo);
                 i32x4 rsrc = {(int)(uint32_t)base, (int)(uint32_t)((base >> 32) & 0xffffu), left * 4, 0x00020000};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) rsrc[k] = __builtin_amdgcn_readfirstlane(rsrc[k]);
                 asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                             :: "s"(__builtin_amdgcn_readfirstlane(st_at + (buf * 2 * HG + i) * ROWS * 4)), "v"(lane * 4), "s"(rsrc) : "memory");
+                             :: "s"(__builtin_amdgcn_readfirstlane(st_at + i * ROWS * 4)), "v"(lane * 4), "s"(rsrc) : "memory");
             }
         };
         __syncthreads();                                       // the chunk of heads before has been read
@@ -392,16 +400,14 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_kv_k
         }
         for (int tile = first; tile < last; ++tile) {
             AT_ARRIVE();
-            if (NBUF == 2 && tile + 1 < last) request(tile + 1);
-            if (tile + 1 < last) {
+                if (tile + 1 < last) {
                 put_coords(tile + 1);
                 coords(tile + 2);
             }
             if (k0 < t.hi) {
-                const int buf = NBUF == 2 ? tile & 1 : 0;
-                const char* const qt = qs + buf * Tile::kBytes;
-                const char* const gt = gs + buf * Tile::kBytes;
-                const float* const lt = st + buf * 2 * HG * ROWS;
+                bool huge[HG];
+#pragma unroll
+                for (int h = 0; h < HG; ++h) huge[h] = at_huge(st[h * ROWS + lane]);
                 const float* const ct = cs + (tile & 1) * 3 * ROWS;
                 const int left = q_hi - (q_lo + tile * ROWS);
 #pragma unroll
@@ -415,20 +421,18 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_kv_k
                     for (int h = 0; h < HG; ++h) {
                         const int slot = SLOTS == 1 ? 0 : h;
                         f32x4 s[2], dp[2];
-                        const bool huge = at_huge(lt[h * ROWS + lane]);
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
-                            const f32x4 lse = *reinterpret_cast<const f32x4*>(lt + h * ROWS + 32 * j + 16 * b + 4 * g);
+                            const f32x4 lse = *reinterpret_cast<const f32x4*>(st + h * ROWS + 32 * j + 16 * b + 4 * g);
                             s[b] = pairs[b].start(slope[h], table + h * a.bias.buckets);
-                            dp[b] = *reinterpret_cast<const f32x4*>(lt + (HG + h) * ROWS + 32 * j + 16 * b + 4 * g);
+                            dp[b] = *reinterpret_cast<const f32x4*>(st + (HG + h) * ROWS + 32 * j + 16 * b + 4 * g);
 #pragma unroll
                             for (int c = 0; c < DC; ++c) {
-                                const int at = Tile::at_rows(h, 2 * j + b, c);
-                                at_mma(s[b], Tile::frag(qt, at), kf[slot][c]);
-                                at_mma(dp[b], Tile::frag(gt, at), vf[slot][c]);
+                                at_mma(s[b], Tile::frag(qs, place, h, 2 * j + b, c), kf[slot][c]);
+                                at_mma(dp[b], Tile::frag(gs, place, h, 2 * j + b, c), vf[slot][c]);
                             }
                             f32x4 (&one)[1] = reinterpret_cast<f32x4 (&)[1]>(s[b]);
-                            const float factor = at_scale(one, scale2, huge);
+                            const float factor = at_scale(one, scale2, huge[h]);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 s[b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][e], factor, -lse[e]));
@@ -437,10 +441,12 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_kv_k
                         if (left < ROWS) {
                             const int end = at_here(left);
 #pragma unroll
-                            for (int b = 0; b < 2; ++b)
+                            for (int b = 0; b < 2; ++b) {
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)
                                     if (32 * j + 16 * b + 4 * g + e >= end) s[b][e] = 0.f;
+                                at_here(s[b]);
+                            }
                         }
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
@@ -452,13 +458,13 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_kv_k
                         at_pack(ds, at_join(dp[0], dp[1]));
 #pragma unroll
                         for (int b = 0; b < DB; ++b) {
-                            at_mma(dv[slot][b], Tile::frag_turned(gt, h, j, b), p);
-                            at_mma(dk[slot][b], Tile::frag_turned(qt, h, j, b), ds);
+                            at_mma(dv[slot][b], Tile::frag_turned(gs, place, h, j, b), p);
+                            at_mma(dk[slot][b], Tile::frag_turned(qs, place, h, j, b), ds);
                         }
                     }
                 }
             }
-            if (NBUF == 1 && tile + 1 < last) {
+            if (tile + 1 < last) {
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 request(tile + 1);
             }
@@ -507,11 +513,11 @@ __global__ __launch_bounds__(kWave) void at_table_kernel(const float* __restrict
 template <typename T, int DP, int HG, int SLOTS, int BIAS, bool GRAD>
 static hipError_t at_bwd_q_launch(const AtBwd& a, hipStream_t st) {
     typedef AtBwdPlan<T, DP> Plan;
-    constexpr int ROWS = GRAD ? Plan::kGradRows : Plan::kRows, NBUF = GRAD ? 1 : Plan::kBuf;
-    size_t lds = (size_t)2 * NBUF * AtTile<T, DP, SLOTS, ROWS>::kBytes + 2 * 3 * ROWS * sizeof(float);
+    constexpr int ROWS = GRAD ? Plan::kGradRows : Plan::kRows;
+    size_t lds = (size_t)2 * AtTile<T, DP, SLOTS, ROWS>::kBytes + 2 * 3 * ROWS * sizeof(float);
     if (BIAS == kTable) lds += (kCells + a.bias.buckets * HG) * sizeof(float);
     if (GRAD) lds += (size_t)4 * a.bias.buckets * HG * 64 * sizeof(float);
-    auto kern = at_bwd_q_kernel<T, DP, HG, SLOTS, BIAS, GRAD, ROWS, NBUF>;
+    auto kern = at_bwd_q_kernel<T, DP, HG, SLOTS, BIAS, GRAD, ROWS>;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return e;
     kern<<<(unsigned)((int64_t)a.tiles * (a.heads / HG)), kAtBlock, lds, st>>>(a);
@@ -520,10 +526,9 @@ static hipError_t at_bwd_q_launch(const AtBwd& a, hipStream_t st) {
 
 template <typename T, int DP, int HG, int SLOTS, int BIAS>
 static hipError_t at_bwd_kv_launch(const AtBwd& a, hipStream_t st) {
-    constexpr int NBUF = AtBwdPlan<T, DP>::kBuf;
-    size_t lds = (size_t)2 * NBUF * AtTile<T, DP, HG, 64>::kBytes + (NBUF * 2 * HG + 2 * 3) * 64 * sizeof(float);
+    size_t lds = (size_t)2 * AtTile<T, DP, HG, 64>::kBytes + (2 * HG + 2 * 3) * 64 * sizeof(float);
     if (BIAS == kTable) lds += (kCells + a.bias.buckets * HG) * sizeof(float);
-    auto kern = at_bwd_kv_kernel<T, DP, HG, SLOTS, BIAS, NBUF>;
+    auto kern = at_bwd_kv_kernel<T, DP, HG, SLOTS, BIAS>;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return e;
     const int64_t wg = seg_tiles_bound(a.mk, 64, a.seg_k, a.nseg) * (a.heads / a.share / SLOTS);
@@ -551,7 +556,7 @@ static hipError_t at_bwd_kv_bias(const AtBwd& a, int mode, hipStream_t st) {
 
 template <typename T, int DP>
 static hipError_t at_bwd_width(const AtBwd& a, int mode, hipStream_t st) {
-    constexpr int most = AtBwdPlan<T, DP>::kHeads, grad = AtBwdPlan<T, DP>::kGradHeads;
+    constexpr int most = AtBwdPlan<T, DP>::kHeads, grad = AtBwdPlan<T, DP>::kGradHeads, keys = AtBwdPlan<T, DP>::kKeyHeads;
     const bool wide = most > 1 && at_bwd_heads(most, a.heads, a.share, mode) == most, one = a.share > 1;
     hipError_t e;
     if (a.part_t) {
@@ -564,7 +569,7 @@ static hipError_t at_bwd_width(const AtBwd& a, int mode, hipStream_t st) {
     } else if (wide) e = one ? at_bwd_q_bias<T, DP, most, 1>(a, mode, st) : at_bwd_q_bias<T, DP, most, most>(a, mode, st);
     else e = at_bwd_q_bias<T, DP, 1, 1>(a, mode, st);
     if (e != hipSuccess || a.dk == nullptr) return e;
-    if (wide) return one ? at_bwd_kv_bias<T, DP, most, 1>(a, mode, st) : at_bwd_kv_bias<T, DP, most, most>(a, mode, st);
+    if (keys > 1 && at_bwd_heads(keys, a.heads, a.share, mode) == keys) return one ? at_bwd_kv_bias<T, DP, keys, 1>(a, mode, st) : at_bwd_kv_bias<T, DP, keys, keys>(a, mode, st);
     return at_bwd_kv_bias<T, DP, 1, 1>(a, mode, st);
 }
 
@@ -572,7 +577,7 @@ static hipError_t at_bwd_width(const AtBwd& a, int mode, hipStream_t st) {
 // large part of the time, each with at least two tiles of an average scan's queries.
 template <typename T, int DP>
 static int at_bwd_splits(int64_t mq, int64_t mk, int64_t nseg, int heads, int kv_heads, int mode) {
-    const int share = heads / kv_heads, slots = share > 1 ? 1 : at_bwd_heads(AtBwdPlan<T, DP>::kHeads, heads, share, mode);
+    const int share = heads / kv_heads, slots = share > 1 ? 1 : at_bwd_heads(AtBwdPlan<T, DP>::kKeyHeads, heads, share, mode);
     const int64_t wg = (ceil_div(mk > 0 ? mk : 1, 64) + nseg - 1) * (kv_heads / slots);
     if (wg >= 2048) return 1;
     const int64_t want = ceil_div(2048, wg), most = ceil_div(mq, nseg) / 128;

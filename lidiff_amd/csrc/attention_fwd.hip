@@ -7,11 +7,6 @@
 // the sum of the probabilities comes from the matrix pipe too (a row of ones), of the values that multiply v.
 #include "attention.h"
 
-#ifndef AT_FWD_QB
-#define AT_FWD_QB 1
-#define AT_FWD_BUF 2
-#endif
-
 namespace lidiff {
 
 struct AtFwd {
@@ -31,12 +26,15 @@ struct AtFwd {
     float *part_o, *part_ml;                                  // splits > 1: [splits][mq][heads][dim], [splits][2][heads][mq]
 };
 
-// What a workgroup takes: QB x 16 queries a wave, HG heads, tiles of 64 keys in NBUF buffers.
+// What a workgroup takes: QB x 16 queries a wave, HG heads, tiles of 64 keys.
 // HG: the distances of a (query, key) pair are the same for every head, so a wave takes as many heads as its registers hold.
+// One buffer per tile: three workgroups of a compute unit cover each other's waits better than two with a second buffer do (41 157 x 5 824
+// x 2, bf16: 1.23 against 1.48 ms).  fp32 operands are three times the LDS reads: two blocks of queries share them (0.38 against 0.42 ms
+// at 5 824 x 5 824; bf16: 1.41 against 1.23, for the registers).
 template <typename T, int DP> struct AtFwdPlan {
     static constexpr int kHeads = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 ? 2 : 1;
-    static constexpr int kQB = AT_FWD_QB;
-    static constexpr int kBuf = sizeof(T) == 4 ? 1 : AT_FWD_BUF;
+    static constexpr int kExactHeads = kHeads > 2 ? 2 : kHeads;      // (the second pieces take the registers of two heads: 1.63 against 1.91 ms)
+    static constexpr int kQB = sizeof(T) == 4 && DP <= 64 ? 2 : 1;
 };
 constexpr int kFwdRows = 64;
 
@@ -47,7 +45,7 @@ inline int at_fwd_heads(int most, int heads, int share, int mode) {      // whol
 // EXACT (16-bit operands, when the table's gradient is wanted): probabilities enter the product with the values in pieces, rounding and
 // rest.  d table sums ds over millions of pairs whose rows cancel to zero through delta = do . out, so an output from probabilities of 8 or
 // 11 bits costs it more than fp32 sums do.
-template <typename T, int DP, int HG, int SLOTS, int BIAS, int QB, int NBUF, bool EXACT>
+template <typename T, int DP, int HG, int SLOTS, int BIAS, int QB, bool EXACT>
 __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kernel(const AtFwd a) {
     constexpr int ROWS = kFwdRows, DC = DP / 32, DB = DP / 16, KB = ROWS / 16;
     typedef AtTile<T, DP, SLOTS, ROWS> Tile;
@@ -56,9 +54,9 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
     constexpr float kLift = AtType<T>::kLift ? 7.f : 0.f, kUnlift = AtType<T>::kLift ? 1.f / 128.f : 1.f, kSlack = 8.f;
     constexpr bool kOnes = sizeof(T) == 2 && !EXACT, kTwoLevels = sizeof(T) == 4 || EXACT;
     extern __shared__ __align__(16) char at_sm[];
-    char* const ks = at_sm;                                                       // [NBUF] keys, [NBUF] values
-    char* const vs = ks + NBUF * Tile::kBytes;
-    float* const cs = reinterpret_cast<float*>(vs + NBUF * Tile::kBytes);         // [2][x, y, z] of the tile's keys
+    char* const ks = at_sm;
+    char* const vs = ks + Tile::kBytes;
+    float* const cs = reinterpret_cast<float*>(vs + Tile::kBytes);                // [2][x, y, z] of the tile's keys
     unsigned* const cells = reinterpret_cast<unsigned*>(cs + 2 * 3 * ROWS);
     float* const table = reinterpret_cast<float*>(cells + (BIAS == kTable ? kCells : 0));      // [HG][buckets]
     const unsigned ks_at = (unsigned)(uintptr_t)(at_lds_t)ks, vs_at = (unsigned)(uintptr_t)(at_lds_t)vs;
@@ -103,11 +101,13 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
 
     f32x4 o[QB][HG][DB], l[QB][HG];
     float base[QB][HG];                                        // in units of log 2; -inf: nothing seen yet
+    bool huge[QB][HG];
 #pragma unroll
     for (int n = 0; n < QB; ++n)
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
             base[n][h] = -INFINITY;
+            huge[n][h] = false;
             l[n][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int b = 0; b < DB; ++b) o[n][h][b] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -128,11 +128,15 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
         float* c = cs + (tile & 1) * 3 * ROWS + threadIdx.x;
         c[0] = (float)kc.y; c[ROWS] = (float)kc.z; c[2 * ROWS] = (float)kc.w;
     };
-    auto request = [&](int tile) {
-        const int lo = k_lo + tile * ROWS, left = min(ROWS, k_hi - lo), at = (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
-        Tile::request(a.k, kv0, a.dim, lo, left, ks_at + at);
-        Tile::request(a.v, kv0, a.dim, lo, left, vs_at + at);
+    const char *k_at = a.k.p + (int64_t)(k_lo + first * ROWS) * a.k.row + kv0 * a.k.head, *v_at = a.v.p + (int64_t)(k_lo + first * ROWS) * a.v.row + kv0 * a.v.head;
+    auto request = [&](int tile) {                             // (tile after tile)
+        const int left = min(ROWS, k_hi - (k_lo + tile * ROWS));
+        Tile::request(a.k, k_at, a.dim, left, ks_at);
+        Tile::request(a.v, v_at, a.dim, left, vs_at);
+        k_at += ROWS * a.k.row;
+        v_at += ROWS * a.v.row;
     };
+    const typename Tile::Lane place;
     if (first < last) {
         coords(first);
         put_coords(first);
@@ -141,14 +145,11 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
     }
     for (int tile = first; tile < last; ++tile) {
         AT_ARRIVE();
-        if (NBUF == 2 && tile + 1 < last) request(tile + 1);
         if (tile + 1 < last) {
             put_coords(tile + 1);
             coords(tile + 2);
         }
         if (q0 < t.hi) {                                       // (a wave without queries only takes part in the requests)
-            const char* const kt = ks + (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
-            const char* const vt = vs + (NBUF == 2 ? tile & 1 : 0) * Tile::kBytes;
             const float* const ct = cs + (tile & 1) * 3 * ROWS;
             const int left = k_hi - (k_lo + tile * ROWS);      // keys of this tile, 64 except at the end
             AtPairs<BIAS> pairs[QB][KB];
@@ -168,7 +169,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
                     for (int n = 0; n < QB; ++n) s[n][b] = pairs[n][b].start(slope[h], table + h * a.bias.buckets);
 #pragma unroll
                     for (int c = 0; c < DC; ++c) {
-                        const Frag kf = Tile::frag(kt, Tile::at_rows(slot, b, c));
+                        const Frag kf = Tile::frag(ks, place, slot, b, c);
 #pragma unroll
                         for (int n = 0; n < QB; ++n) at_mma(s[n][b], kf, qf[n][h][c]);
                     }
@@ -178,10 +179,12 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
 #pragma unroll
                     for (int n = 0; n < QB; ++n)
 #pragma unroll
-                        for (int b = 0; b < KB; ++b)
+                        for (int b = 0; b < KB; ++b) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
                                 if (16 * b + 4 * g + e >= end) s[n][b][e] = -INFINITY;
+                            at_here(s[n][b]);
+                        }
                 }
                 constexpr int PIECES = EXACT ? 2 : 1;
                 Frag p[QB][KB / 2][PIECES];
@@ -198,12 +201,13 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
                         top = fmaxf(top, __shfl_xor(top, 32));
                         const float now = fmaxf(base[n][h], top), fade = __builtin_amdgcn_exp2f(base[n][h] - (now == -INFINITY ? 0.f : now));
                         base[n][h] = now;
+                        huge[n][h] = at_huge(now);
                         l[n][h] *= fade;
 #pragma unroll
                         for (int b = 0; b < DB; ++b) o[n][h][b] *= fade;
                     }
                     const float down = base[n][h] == -INFINITY ? 0.f : kLift - base[n][h];
-                    const float factor = at_scale(s[n], scale2, at_huge(base[n][h]));
+                    const float factor = at_scale(s[n], scale2, huge[n][h]);
 #pragma unroll
                     for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
                 for (int j = 0; j < KB / 2; ++j)
 #pragma unroll
                     for (int b = 0; b < DB; ++b) {
-                        const Frag vf = Tile::frag_turned(vt, slot, j, b);
+                        const Frag vf = Tile::frag_turned(vs, place, slot, j, b);
 #pragma unroll
                         for (int n = 0; n < QB; ++n)
 #pragma unroll
@@ -244,7 +248,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
                     for (int b = 0; b < DB; ++b) o[n][h][b] = kTwoLevels ? o[n][h][b] + part[n][b] : part[n][b];
             }
         }
-        if (NBUF == 1 && tile + 1 < last) {
+        if (tile + 1 < last) {
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the tile has been read
             request(tile + 1);
         }
@@ -315,11 +319,11 @@ __global__ void at_join_kernel(const AtFwd a) {
 template <typename T, int DP, int HG, int SLOTS, int BIAS, bool EXACT = false>
 static hipError_t at_fwd_launch(const AtFwd& a, hipStream_t st) {
     typedef AtFwdPlan<T, DP> Plan;
-    constexpr int QB = Plan::kQB, NBUF = Plan::kBuf;
+    constexpr int QB = Plan::kQB;
     const int64_t wg = seg_tiles_bound(a.mq, 64 * QB, a.seg_q, a.nseg) * (a.heads / HG);
-    size_t lds = (size_t)2 * NBUF * AtTile<T, DP, SLOTS, kFwdRows>::kBytes + 2 * 3 * kFwdRows * sizeof(float);
+    size_t lds = (size_t)2 * AtTile<T, DP, SLOTS, kFwdRows>::kBytes + 2 * 3 * kFwdRows * sizeof(float);
     if (BIAS == kTable) lds += (kCells + a.bias.buckets * HG) * sizeof(float);
-    auto kern = at_fwd_kernel<T, DP, HG, SLOTS, BIAS, QB, NBUF, EXACT>;
+    auto kern = at_fwd_kernel<T, DP, HG, SLOTS, BIAS, QB, EXACT>;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return e;
     kern<<<dim3((unsigned)wg, (unsigned)a.splits), kAtBlock, lds, st>>>(a);
@@ -329,8 +333,6 @@ static hipError_t at_fwd_launch(const AtFwd& a, hipStream_t st) {
 
 template <typename T, int DP, int HG, int SLOTS>
 static hipError_t at_fwd_bias(const AtFwd& a, int mode, hipStream_t st) {
-    if constexpr (sizeof(T) == 2)
-        if (mode == kTable && a.exact) return at_fwd_launch<T, DP, HG, SLOTS, kTable, true>(a, st);
     if (mode == kTable) return at_fwd_launch<T, DP, HG, SLOTS, kTable>(a, st);
     if (mode == kSlope) return at_fwd_launch<T, DP, HG, SLOTS, kSlope>(a, st);
     if constexpr (HG == 1) return at_fwd_launch<T, DP, HG, SLOTS, kNone>(a, st);
@@ -339,7 +341,15 @@ static hipError_t at_fwd_bias(const AtFwd& a, int mode, hipStream_t st) {
 
 template <typename T, int DP>
 static hipError_t at_fwd_width(const AtFwd& a, int mode, hipStream_t st) {
-    constexpr int most = AtFwdPlan<T, DP>::kHeads;
+    constexpr int most = AtFwdPlan<T, DP>::kHeads, exact = AtFwdPlan<T, DP>::kExactHeads;
+    if constexpr (sizeof(T) == 2) {
+        if (mode == kTable && a.exact) {
+            if constexpr (exact > 1)
+                if (at_fwd_heads(exact, a.heads, a.share, mode) == exact)
+                    return a.share > 1 ? at_fwd_launch<T, DP, exact, 1, kTable, true>(a, st) : at_fwd_launch<T, DP, exact, exact, kTable, true>(a, st);
+            return at_fwd_launch<T, DP, 1, 1, kTable, true>(a, st);
+        }
+    }
     if constexpr (most > 1)
         if (at_fwd_heads(most, a.heads, a.share, mode) == most) return a.share > 1 ? at_fwd_bias<T, DP, most, 1>(a, mode, st) : at_fwd_bias<T, DP, most, most>(a, mode, st);
     return at_fwd_bias<T, DP, 1, 1>(a, mode, st);
