@@ -248,13 +248,24 @@ struct AtBias {
     int buckets;
 };
 
+// The cells and the table of HG heads as they stand in LDS: table[HG][kTableRow], already divided by the scale (neighbouring buckets in
+// neighbouring banks), and cells whose bucket is a byte offset into a row (low 10 bits), so that a pair's one address serves every head.
+constexpr int kTableRow = 64;
+__device__ __forceinline__ void at_put_cells(unsigned* __restrict__ cells, const unsigned* __restrict__ src) {
+    for (int i = threadIdx.x; i < kCells; i += kAtBlock) cells[i] = (src[i] >> 8 << 10) | (src[i] & 255u) * 4;
+}
+template <int HG>
+__device__ __forceinline__ void at_put_table(float* __restrict__ table, const AtBias& bias, int heads, int h0, float scale) {
+    for (int i = threadIdx.x; i < bias.buckets * HG; i += kAtBlock)
+        table[i / bias.buckets * kTableRow + i % bias.buckets] = bias.table[(int64_t)(i % bias.buckets) * heads + h0 + i / bias.buckets] / scale;
+}
 __device__ __forceinline__ int at_bucket(const unsigned* cells, float d2) {
     const int bits = __builtin_bit_cast(int, d2);
     const unsigned c = cells[min(max(bits >> kCellRest, kCellFirst), kCellFirst + kCells - 1) - kCellFirst];
-    return (int)(c & 255u) + ((unsigned)(bits & ((1 << kCellRest) - 1)) >= (c >> 8) ? 1 : 0);
+    return (int)(c & 1023u) + ((unsigned)(bits & ((1 << kCellRest) - 1)) >= (c >> 10) ? 4 : 0);
 }
 
-// what the heads of a wave share about four pairs: distances, or buckets
+// what the heads of a wave share about four pairs: distances, or their buckets' places in the table
 template <int BIAS>
 struct AtPairs {
     float d[4];
@@ -268,13 +279,13 @@ struct AtPairs {
             if (BIAS == kTable) b[e] = at_bucket(cells, d2);
         }
     }
-    // the accumulator a head's block starts from; slope: -slope / scale, table: this head's column divided by the scale
-    __device__ __forceinline__ f32x4 start(float slope, const float* table) const {
+    // the accumulator head h's block starts from
+    __device__ __forceinline__ f32x4 start(float slope, const float* table, int h) const {
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (BIAS == kSlope) s[e] = slope * d[e];
-            if (BIAS == kTable) s[e] = table[b[e]];
+            if (BIAS == kTable) s[e] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(table + h * kTableRow) + b[e]);
         }
         return s;
     }

@@ -50,7 +50,11 @@ __global__ __launch_bounds__(256) void at_bound_kernel(const T* __restrict__ src
     float sum = 0.f;
     if (row < rows) {
         const T* p = src + row * row_stride + (int64_t)blockIdx.y * head_stride;
-        for (int d = 0; d < dim; ++d) sum += (float)p[d] * (float)p[d];
+        for (int d = 0; d < dim; d += 8) {
+            const f32x8 v = __builtin_convertvector(at_load8(p + d), f32x8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += v[e] * v[e];
+        }
     }
     if (!(sum < INFINITY)) sum = 0.f;
     for (int off = kWave / 2; off > 0; off >>= 1) sum = fmaxf(sum, __shfl_xor(sum, off));
@@ -64,7 +68,8 @@ template <typename T, int DP> struct AtBwdPlan {
     static constexpr int kKeyHeads = kHeads > 2 ? 2 : kHeads;         // dk / dv: twice the accumulators (four waves a SIMD: 1.56 against 1.71 ms)
     static constexpr int kGradHeads = sizeof(T) == 4 ? 1 : DP == 32 ? 2 : 1;      // with the table's gradient: a histogram of 256 bytes a wave, bucket and head
     static constexpr int kGradRows = 32;
-    static constexpr int kRows = 64;
+    static constexpr int kGradQB = sizeof(T) == 2 && DP == 32 ? 2 : 1;      // blocks of 16 queries a wave (2.58 against 2.81 ms; fp32: 1.14 against 0.97)
+    static constexpr int kRows = 64, kQB = 1;                         // (two blocks: 1.33 against 1.26 ms)
     static constexpr int kKeyWaves = sizeof(T) == 2 && DP == 32 ? 4 : at_waves(sizeof(T), DP);
 };
 
@@ -72,25 +77,34 @@ inline int at_bwd_heads(int most, int heads, int share, int mode) {      // whol
     return mode != kNone && heads % most == 0 && (share == 1 || share % most == 0) ? most : 1;
 }
 
-// Adds four values to words bucket[e] * 64 of a lane's own column.  (LDS float atomics take some 240 cycles a wave: 15.9 ms of the
-// gradient of 3 10^8 pairs x 8 heads; plain reads and writes of a private column need no atomic.)  Writes of a wave happen in order, so
-// of equal buckets the last one has to hold the sum of them all.
-__device__ __forceinline__ void at_hist(float* __restrict__ column, const int (&bucket)[4], const f32x4& v) {
-    float old[4], sum[4];
+// Adds the score gradients of four pairs and HG heads to the words of a lane's own column, [bucket][HG][64 lanes] (place: byte offsets
+// of a row of the table, four per bucket).  LDS float atomics take some 240 cycles a wave (15.9 ms of the gradient of 3 10^8
+// pairs x 8 heads); plain reads and writes of a private column need no atomic.  A wave's accesses happen in order: two pairs at a time, for
+// all heads, are read and written; if their buckets are the same the second, written last, holds both.
+template <int HG>
+__device__ __forceinline__ void at_hist(char* __restrict__ column, const int (&place)[4], const f32x4 (&v)[HG]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) old[e] = column[bucket[e] * 64];
+    for (int e = 0; e < 4; e += 2) {
+        float* const one = reinterpret_cast<float*>(column + place[e] * (64 * HG));
+        float* const two = reinterpret_cast<float*>(column + place[e + 1] * (64 * HG));
+        const bool same = place[e] == place[e + 1];
+        float a[HG], b[HG];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        sum[e] = v[e];
+        for (int h = 0; h < HG; ++h) { a[h] = one[h * 64]; b[h] = two[h * 64]; }
 #pragma unroll
-        for (int f = 0; f < e; ++f) sum[e] += bucket[f] == bucket[e] ? v[f] : 0.f;
+        for (int h = 0; h < HG; ++h) {
+            a[h] += v[h][e];
+            b[h] = (same ? a[h] : b[h]) + v[h][e + 1];
+        }
+#pragma unroll
+        for (int h = 0; h < HG; ++h) one[h * 64] = a[h];
+#pragma unroll
+        for (int h = 0; h < HG; ++h) two[h * 64] = b[h];
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) column[bucket[e] * 64] = old[e] + sum[e];
 }
 
-// one workgroup: 64 queries of one scan x HG heads: dq, delta, and its part of the table's gradient
-template <typename T, int DP, int HG, int SLOTS, int BIAS, bool GRAD, int ROWS>
+// one workgroup: 64 QB queries of one scan x HG heads: dq, delta, and its part of the table's gradient
+template <typename T, int DP, int HG, int SLOTS, int BIAS, bool GRAD, int ROWS, int QB>
 __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_kernel(const AtBwd a) {
     constexpr int DC = DP / 32, DB = DP / 16;
     typedef AtTile<T, DP, SLOTS, ROWS> Tile;
@@ -102,12 +116,12 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
     float* const cs = reinterpret_cast<float*>(vs + Tile::kBytes);
     unsigned* const cells = reinterpret_cast<unsigned*>(cs + 2 * 3 * ROWS);
     float* const table = reinterpret_cast<float*>(cells + (BIAS == kTable ? kCells : 0));
-    float* const hist = table + (BIAS == kTable ? a.bias.buckets * HG : 0);              // [wave][HG][bucket][64 lanes]: a lane adds to words of its own
+    float* const hist = table + (BIAS == kTable ? kTableRow * HG : 0);              // [wave][bucket][HG][64 lanes]: a lane adds to words of its own
     const unsigned ks_at = (unsigned)(uintptr_t)(at_lds_t)ks, vs_at = (unsigned)(uintptr_t)(at_lds_t)vs;
 
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int groups = a.heads / HG, h0 = (blockIdx.x % groups) * HG, kv0 = h0 / a.share, tile_id = blockIdx.x / groups;
-    const SegTile t = find_seg_tile(a.seg_q, a.nseg, a.mq, 64, tile_id);
+    const SegTile t = find_seg_tile(a.seg_q, a.nseg, a.mq, 64 * QB, tile_id);
     if (t.lo >= t.hi) {
         if (GRAD)
             for (int i = threadIdx.x; i < HG * a.bias.buckets; i += kAtBlock)
@@ -116,74 +130,80 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
     }
     const int2 kr = t.seg >= 0 ? seg_range(a.seg_k, t.seg, a.mk) : make_int2(0, 0);
     const int k_lo = __builtin_amdgcn_readfirstlane(kr.x), k_hi = __builtin_amdgcn_readfirstlane(kr.y), last = (k_hi - k_lo + ROWS - 1) / ROWS;
-    const int q0 = t.lo + wave * 16, qi = q0 + col;
-    const bool have = qi < t.hi;
+    const int q0 = t.lo + wave * 16 * QB;
     const float scale2 = a.scale * kLog2e;
 
-    Frag qf[HG][DC], gf[HG][DC];
-    float lse[HG], slope[HG], unlift[HG];
-    bool huge[HG];
+    Frag qf[QB][HG][DC], gf[QB][HG][DC];
+    float lse[QB][HG], slope[HG], unlift[QB][HG], qx[QB], qy[QB], qz[QB];
+    bool huge[QB][HG];
     // -delta: what the products do . v start from.  (With the table's gradient it is added behind them: the matrix pipe rounds sums to one
     // side, and what is the same for every pair does not cancel in a sum over 10^8 of them -- 1.9e-5 of the gradient against 1.2e-6.)
-    f32x4 down[HG];
+    float less[QB][HG];
 #pragma unroll
-    for (int h = 0; h < HG; ++h) {
-        float sum = 0.f, g2 = 0.f;
+    for (int n = 0; n < QB; ++n) {
+        const int qi = q0 + 16 * n + col;
+        const bool have = qi < t.hi;
 #pragma unroll
-        for (int c = 0; c < DC; ++c) {
-            const int d = 32 * c + 8 * g;
-            qf[h][c] = gf[h][c] = Frag{};
-            if (have && d < a.dim) {
-                const T* go = (const T*)a.go + (int64_t)qi * a.go_row + (int64_t)(h0 + h) * a.go_head + d;
-                qf[h][c] = at_load8((const T*)a.q + (int64_t)qi * a.q_row + (int64_t)(h0 + h) * a.q_head + d);
-                gf[h][c] = at_load8(go);
-                const float* o = a.out32 + ((int64_t)qi * a.heads + h0 + h) * a.dim + d;
+        for (int h = 0; h < HG; ++h) {
+            float sum = 0.f, g2 = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    sum += (float)go[e] * o[e];
-                    if (kLifted) g2 += (float)go[e] * (float)go[e];
+            for (int c = 0; c < DC; ++c) {
+                const int d = 32 * c + 8 * g;
+                qf[n][h][c] = gf[n][h][c] = Frag{};
+                if (have && d < a.dim) {
+                    const T* go = (const T*)a.go + (int64_t)qi * a.go_row + (int64_t)(h0 + h) * a.go_head + d;
+                    qf[n][h][c] = at_load8((const T*)a.q + (int64_t)qi * a.q_row + (int64_t)(h0 + h) * a.q_head + d);
+                    gf[n][h][c] = at_load8(go);
+                    const float* o = a.out32 + ((int64_t)qi * a.heads + h0 + h) * a.dim + d;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        sum += (float)go[e] * o[e];
+                        if (kLifted) g2 += (float)go[e] * (float)go[e];
+                    }
                 }
             }
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            less[n][h] = -sum;
+            lse[n][h] = have ? a.lse[(int64_t)(h0 + h) * a.mq + qi] : INFINITY;
+            if (have && g == 0) {
+                a.stat[(int64_t)(h0 + h) * a.mq + qi] = lse[n][h] - AtType<T>::kLift;
+                a.stat[(int64_t)(a.heads + h0 + h) * a.mq + qi] = -sum;
+            }
+            unlift[n][h] = 1.f;
+            if (kLifted) {
+                g2 += __shfl_xor(g2, 16);
+                g2 += __shfl_xor(g2, 32);
+                const int kv_heads = a.heads / a.share;
+                const float lift = at_lift(g2, __builtin_bit_cast(float, a.bound[kv_heads + (h0 + h) / a.share]));
+                lse[n][h] -= lift;                             // p, and with it ds, carries the power of two
+                unlift[n][h] = __builtin_amdgcn_exp2f(-lift);
+            }
+            huge[n][h] = at_huge(lse[n][h]);
         }
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        down[h] = f32x4{-sum, -sum, -sum, -sum};
-        lse[h] = have ? a.lse[(int64_t)(h0 + h) * a.mq + qi] : INFINITY;
-        if (have && g == 0) {
-            a.stat[(int64_t)(h0 + h) * a.mq + qi] = lse[h] - AtType<T>::kLift;
-            a.stat[(int64_t)(a.heads + h0 + h) * a.mq + qi] = -sum;
+        qx[n] = qy[n] = qz[n] = 0.f;
+        if (BIAS != kNone && have) {
+            const int4 c = a.cq[qi];
+            qx[n] = (float)c.y; qy[n] = (float)c.z; qz[n] = (float)c.w;
         }
-        unlift[h] = 1.f;
-        if (kLifted) {
-            g2 += __shfl_xor(g2, 16);
-            g2 += __shfl_xor(g2, 32);
-            const int kv_heads = a.heads / a.share;
-            const float lift = at_lift(g2, __builtin_bit_cast(float, a.bound[kv_heads + (h0 + h) / a.share]));
-            lse[h] -= lift;                                    // p, and with it ds, carries the power of two
-            unlift[h] = __builtin_amdgcn_exp2f(-lift);
-        }
-        slope[h] = BIAS == kSlope ? -a.bias.slopes[h0 + h] / a.scale : 0.f;
-        huge[h] = at_huge(lse[h]);
     }
-    float qx = 0.f, qy = 0.f, qz = 0.f;
-    if (BIAS != kNone && have) {
-        const int4 c = a.cq[qi];
-        qx = (float)c.y; qy = (float)c.z; qz = (float)c.w;
-    }
+#pragma unroll
+    for (int h = 0; h < HG; ++h) slope[h] = BIAS == kSlope ? -a.bias.slopes[h0 + h] / a.scale : 0.f;
     if (BIAS == kTable) {
-        for (int i = threadIdx.x; i < a.bias.buckets * HG; i += kAtBlock)
-            table[i] = a.bias.table[(int64_t)(i % a.bias.buckets) * a.heads + h0 + i / a.bias.buckets] / a.scale;
-        for (int i = threadIdx.x; i < kCells; i += kAtBlock) cells[i] = a.bias.cells[i];
+        at_put_table<HG>(table, a.bias, a.heads, h0, a.scale);
+        at_put_cells(cells, a.bias.cells);
         if (GRAD)
             for (int i = threadIdx.x; i < 4 * a.bias.buckets * HG * 64; i += kAtBlock) hist[i] = 0.f;
     }
-    float* const mine = hist + wave * a.bias.buckets * HG * 64 + lane;
+    char* const mine = reinterpret_cast<char*>(hist + wave * a.bias.buckets * HG * 64 + lane);
 
-    f32x4 dq[HG][DB];
+    f32x4 dq[QB][HG][DB];
 #pragma unroll
-    for (int h = 0; h < HG; ++h)
+    for (int n = 0; n < QB; ++n)
 #pragma unroll
-        for (int b = 0; b < DB; ++b) dq[h][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int h = 0; h < HG; ++h)
+#pragma unroll
+            for (int b = 0; b < DB; ++b) dq[n][h][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     int4 kc = make_int4(0, 0, 0, 0);                           // the coordinates one tile further than the requests
     auto coords = [&](int tile) {
@@ -221,56 +241,73 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
             const int left = k_hi - (k_lo + tile * ROWS);
 #pragma unroll
             for (int j = 0; j < ROWS / 32; ++j) {              // 32 keys at a time
-                AtPairs<BIAS> pairs[2];
+                AtPairs<BIAS> pairs[QB][2];
+                f32x4 grads[QB][2][HG];
                 if (BIAS != kNone) {
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) pairs[b].form(ct, ROWS, 32 * j + 16 * b + 4 * g, qx, qy, qz, cells);
+                    for (int n = 0; n < QB; ++n)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) pairs[n][b].form(ct, ROWS, 32 * j + 16 * b + 4 * g, qx[n], qy[n], qz[n], cells);
                 }
 #pragma unroll
                 for (int h = 0; h < HG; ++h) {
                     const int slot = SLOTS == 1 ? 0 : h;
-                    f32x4 s[2], dp[2];
+                    f32x4 s[QB][2], dp[QB][2];
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        s[b] = pairs[b].start(slope[h], table + h * a.bias.buckets);
-                        dp[b] = GRAD ? f32x4{0.f, 0.f, 0.f, 0.f} : down[h];
+#pragma unroll
+                        for (int n = 0; n < QB; ++n) {
+                            s[n][b] = pairs[n][b].start(slope[h], table, h);
+                            dp[n][b] = GRAD ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{less[n][h], less[n][h], less[n][h], less[n][h]};
+                        }
 #pragma unroll
                         for (int c = 0; c < DC; ++c) {
-                            at_mma(s[b], Tile::frag(ks, place, slot, 2 * j + b, c), qf[h][c]);
-                            if (GRAD) at_mma_apart(dp[b], Tile::frag(vs, place, slot, 2 * j + b, c), gf[h][c]);
-                            else at_mma(dp[b], Tile::frag(vs, place, slot, 2 * j + b, c), gf[h][c]);
+                            const Frag kf = Tile::frag(ks, place, slot, 2 * j + b, c), vf = Tile::frag(vs, place, slot, 2 * j + b, c);
+#pragma unroll
+                            for (int n = 0; n < QB; ++n) {
+                                at_mma(s[n][b], kf, qf[n][h][c]);
+                                if (GRAD) at_mma_apart(dp[n][b], vf, gf[n][h][c]);
+                                else at_mma(dp[n][b], vf, gf[n][h][c]);
+                            }
                         }
                     }
-                    const float factor = at_scale(s, scale2, huge[h]);
+                    Frag p[QB];
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
+                    for (int n = 0; n < QB; ++n) {
+                        const float factor = at_scale(s[n], scale2, huge[n][h]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            s[b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][e], factor, -lse[h]));
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[n][b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[n][b][e], factor, -lse[n][h]));
+                        if (left < ROWS) {
+                            const int end = at_here(left);
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (32 * j + 16 * b + 4 * g + e >= end) s[n][b][e] = 0.f;
+                                at_here(s[n][b]);
+                            }
                         }
-                    }
-                    if (left < ROWS) {
-                        const int end = at_here(left);
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (32 * j + 16 * b + 4 * g + e >= end) s[b][e] = 0.f;
-                            at_here(s[b]);
+                            s[n][b] *= GRAD ? dp[n][b] + less[n][h] : dp[n][b];
+                            if (GRAD) grads[n][b][h] = kLifted ? s[n][b] * unlift[n][h] : s[n][b];
                         }
+                        at_pack(p[n], at_join(s[n][0], s[n][1]));
                     }
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
+                    for (int b = 0; b < DB; ++b) {
+                        const Frag kf = Tile::frag_turned(ks, place, slot, j, b);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            s[b][e] *= GRAD ? dp[b][e] + down[h][e] : dp[b][e];
-                        }
-                        if (GRAD) at_hist(mine + h * a.bias.buckets * 64, pairs[b].b, kLifted ? s[b] * unlift[h] : s[b]);
+                        for (int n = 0; n < QB; ++n) at_mma(dq[n][h][b], kf, p[n]);
                     }
-                    Frag p;
-                    at_pack(p, at_join(s[0], s[1]));
+                }
+                if (GRAD) {
 #pragma unroll
-                    for (int b = 0; b < DB; ++b) at_mma(dq[h][b], Tile::frag_turned(ks, place, slot, j, b), p);
+                    for (int n = 0; n < QB; ++n)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) at_hist<HG>(mine, pairs[n][b].b, grads[n][b]);
                 }
             }
         }
@@ -279,12 +316,15 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
             request(tile + 1);
         }
     }
-    if (have) {
+#pragma unroll
+    for (int n = 0; n < QB; ++n) {
+        const int qi = q0 + 16 * n + col;
+        if (qi >= t.hi) continue;
 #pragma unroll
         for (int h = 0; h < HG; ++h)
 #pragma unroll
             for (int b = 0; b < DB; ++b)
-                if (16 * b + 4 * g < a.dim) at_store4((T*)a.dq + ((int64_t)qi * a.heads + h0 + h) * a.dim + 16 * b + 4 * g, dq[h][b] * (a.scale * unlift[h]));
+                if (16 * b + 4 * g < a.dim) at_store4((T*)a.dq + ((int64_t)qi * a.heads + h0 + h) * a.dim + 16 * b + 4 * g, dq[n][h][b] * (a.scale * unlift[n][h]));
     }
     if (GRAD) {
         __syncthreads();
@@ -292,7 +332,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
             double u = 0;                                      // (the 4 x 64 lanes' sums in a fixed order)
             for (int w = 0; w < 4; ++w)
                 for (int l = 0; l < 64; ++l) u += hist[(w * HG * a.bias.buckets + i) * 64 + ((l + i) & 63)];
-            a.part_t[((int64_t)tile_id * a.heads + h0) * a.bias.buckets + i] = (float)u;
+            a.part_t[((int64_t)tile_id * a.heads + h0 + i % HG) * a.bias.buckets + i / HG] = (float)u;
         }
     }
 }
@@ -354,7 +394,7 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
         kx = (float)c.y; ky = (float)c.z; kz = (float)c.w;
     }
     if (BIAS == kTable)
-        for (int i = threadIdx.x; i < kCells; i += kAtBlock) cells[i] = a.bias.cells[i];
+        at_put_cells(cells, a.bias.cells);
 
     const typename Tile::Lane place;
     // the query heads that read these key heads, HG at a time
@@ -389,9 +429,7 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
             }
         };
         __syncthreads();                                       // the chunk of heads before has been read
-        if (BIAS == kTable)
-            for (int i = threadIdx.x; i < a.bias.buckets * HG; i += kAtBlock)
-                table[i] = a.bias.table[(int64_t)(i % a.bias.buckets) * a.heads + h0 + i / a.bias.buckets] / a.scale;
+        if (BIAS == kTable) at_put_table<HG>(table, a.bias, a.heads, h0, a.scale);
         if (first < last) {
             coords(first);
             put_coords(first);
@@ -424,7 +462,7 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
                             const f32x4 lse = *reinterpret_cast<const f32x4*>(st + h * ROWS + 32 * j + 16 * b + 4 * g);
-                            s[b] = pairs[b].start(slope[h], table + h * a.bias.buckets);
+                            s[b] = pairs[b].start(slope[h], table, h);
                             dp[b] = *reinterpret_cast<const f32x4*>(st + (HG + h) * ROWS + 32 * j + 16 * b + 4 * g);
 #pragma unroll
                             for (int c = 0; c < DC; ++c) {
@@ -513,21 +551,21 @@ __global__ __launch_bounds__(kWave) void at_table_kernel(const float* __restrict
 template <typename T, int DP, int HG, int SLOTS, int BIAS, bool GRAD>
 static hipError_t at_bwd_q_launch(const AtBwd& a, hipStream_t st) {
     typedef AtBwdPlan<T, DP> Plan;
-    constexpr int ROWS = GRAD ? Plan::kGradRows : Plan::kRows;
+    constexpr int ROWS = GRAD ? Plan::kGradRows : Plan::kRows, QB = GRAD ? Plan::kGradQB : Plan::kQB;
     size_t lds = (size_t)2 * AtTile<T, DP, SLOTS, ROWS>::kBytes + 2 * 3 * ROWS * sizeof(float);
-    if (BIAS == kTable) lds += (kCells + a.bias.buckets * HG) * sizeof(float);
+    if (BIAS == kTable) lds += (kCells + kTableRow * HG) * sizeof(float);
     if (GRAD) lds += (size_t)4 * a.bias.buckets * HG * 64 * sizeof(float);
-    auto kern = at_bwd_q_kernel<T, DP, HG, SLOTS, BIAS, GRAD, ROWS>;
+    auto kern = at_bwd_q_kernel<T, DP, HG, SLOTS, BIAS, GRAD, ROWS, QB>;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return e;
-    kern<<<(unsigned)((int64_t)a.tiles * (a.heads / HG)), kAtBlock, lds, st>>>(a);
+    kern<<<(unsigned)(seg_tiles_bound(a.mq, 64 * QB, a.seg_q, a.nseg) * (a.heads / HG)), kAtBlock, lds, st>>>(a);
     return hipGetLastError();
 }
 
 template <typename T, int DP, int HG, int SLOTS, int BIAS>
 static hipError_t at_bwd_kv_launch(const AtBwd& a, hipStream_t st) {
     size_t lds = (size_t)2 * AtTile<T, DP, HG, 64>::kBytes + (2 * HG + 2 * 3) * 64 * sizeof(float);
-    if (BIAS == kTable) lds += (kCells + a.bias.buckets * HG) * sizeof(float);
+    if (BIAS == kTable) lds += (kCells + kTableRow * HG) * sizeof(float);
     auto kern = at_bwd_kv_kernel<T, DP, HG, SLOTS, BIAS>;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return e;
@@ -585,6 +623,11 @@ static int at_bwd_splits(int64_t mq, int64_t mk, int64_t nseg, int heads, int kv
     return n < 1 ? 1 : (int)(n < 64 ? n : 64);
 }
 
+inline int at_grad_blocks(int dtype, int dim) {
+    return dtype == 0 ? (dim <= 32 ? AtBwdPlan<float, 32>::kGradQB : dim <= 64 ? AtBwdPlan<float, 64>::kGradQB : AtBwdPlan<float, 128>::kGradQB)
+                      : (dim <= 32 ? AtBwdPlan<__bf16, 32>::kGradQB : dim <= 64 ? AtBwdPlan<__bf16, 64>::kGradQB : AtBwdPlan<__bf16, 128>::kGradQB);
+}
+
 struct AtBwdLayout { int splits; int64_t bound, q, k, v, go, table, kv, bytes; };      // workspace; the row statistics come first
 
 template <typename T>
@@ -608,7 +651,7 @@ static AtBwdLayout at_bwd_layout(int64_t mq, int64_t mk, const void* seg, int64_
 template <typename T>
 static hipError_t at_bwd_run(AtBwd a, const AtBwdLayout& l, int mode, char* ws, hipStream_t st) {
     const int kv_heads = a.heads / a.share;
-    if (AtType<T>::kLift) {
+    if constexpr (AtType<T>::kLift != 0) {
         at_bound_clear_kernel<<<(unsigned)ceil_div(2 * kv_heads, 256), 256, 0, st>>>(a.bound, 2 * kv_heads);
         at_bound_kernel<T><<<dim3((unsigned)ceil_div(a.mq, 256), (unsigned)a.heads), 256, 0, st>>>((const T*)a.go, a.go_row, a.go_head, a.mq, a.dim, a.share, a.bound);
         if (a.mk > 0)
@@ -676,7 +719,7 @@ extern "C" int lidiff_segment_attention_bwd(const void* q, const void* k, const 
     a.bound = (unsigned*)(ws + l.bound);
     a.part_t = dtable ? (float*)(ws + l.table) : nullptr;
     a.part_kv = (float*)(ws + l.kv);
-    a.tiles = (int)seg_tiles_bound(mq, 64, seg_q, n_segments);
+    a.tiles = (int)seg_tiles_bound(mq, 64 * at_grad_blocks(dtype, dim), seg_q, n_segments);
     a.splits = l.splits;
     hipStream_t st = (hipStream_t)stream;
     LIDIFF_CHECK_HIP(dtype == 0 ? at_bwd_run<float>(a, l, bias_mode, ws, st) : dtype == 1 ? at_bwd_run<__bf16>(a, l, bias_mode, ws, st)

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
     char* const vs = ks + Tile::kBytes;
     float* const cs = reinterpret_cast<float*>(vs + Tile::kBytes);                // [2][x, y, z] of the tile's keys
     unsigned* const cells = reinterpret_cast<unsigned*>(cs + 2 * 3 * ROWS);
-    float* const table = reinterpret_cast<float*>(cells + (BIAS == kTable ? kCells : 0));      // [HG][buckets]
+    float* const table = reinterpret_cast<float*>(cells + (BIAS == kTable ? kCells : 0));      // [HG][kTableRow]
     const unsigned ks_at = (unsigned)(uintptr_t)(at_lds_t)ks, vs_at = (unsigned)(uintptr_t)(at_lds_t)vs;
 
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
@@ -94,9 +94,8 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
 #pragma unroll
     for (int h = 0; h < HG; ++h) slope[h] = BIAS == kSlope ? -a.bias.slopes[h0 + h] / a.scale : 0.f;
     if (BIAS == kTable) {
-        for (int i = threadIdx.x; i < a.bias.buckets * HG; i += kAtBlock)
-            table[i] = a.bias.table[(int64_t)(i % a.bias.buckets) * a.heads + h0 + i / a.bias.buckets] / a.scale;
-        for (int i = threadIdx.x; i < kCells; i += kAtBlock) cells[i] = a.bias.cells[i];
+        at_put_table<HG>(table, a.bias, a.heads, h0, a.scale);
+        at_put_cells(cells, a.bias.cells);
     }
 
     f32x4 o[QB][HG][DB], l[QB][HG];
@@ -166,7 +165,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
 #pragma unroll
-                    for (int n = 0; n < QB; ++n) s[n][b] = pairs[n][b].start(slope[h], table + h * a.bias.buckets);
+                    for (int n = 0; n < QB; ++n) s[n][b] = pairs[n][b].start(slope[h], table, h);
 #pragma unroll
                     for (int c = 0; c < DC; ++c) {
                         const Frag kf = Tile::frag(ks, place, slot, b, c);
@@ -290,30 +289,38 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
     }
 }
 
-// joins the shares of the keys: a thread takes four elements of one (query, head)
+// Joins the shares of the keys.  A (query, head) takes `width` lanes of four elements, times `lanes` that each add every lanes-th share; a
+// fixed butterfly joins those.  Many shares are read side by side (one lane walking over 45 of them: 23 us against 6), few by one lane
+// each (3 shares of 46 592 units: 7 us against 19).
 template <typename T>
-__global__ void at_join_kernel(const AtFwd a) {
-    const int quads = a.dim / 4;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, total = (int64_t)a.mq * a.heads * quads;
-    if (i >= total) return;
-    const int d = (int)(i % quads) * 4, head = (int)(i / quads % a.heads), qi = (int)(i / quads / a.heads);
+__global__ __launch_bounds__(256) void at_join_kernel(const AtFwd a, int width, int lanes) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, unit = i / (width * lanes);
+    if (unit >= (int64_t)a.mq * a.heads) return;              // (units are whole groups of lanes: a butterfly stays inside one)
+    const int head = (int)(unit % a.heads), qi = (int)(unit / a.heads), d = (int)(i % width) * 4, first = (int)(i / width % lanes);
+    const float* const ml = a.part_ml + (int64_t)head * a.mq + qi;
+    const int64_t plane = (int64_t)a.heads * a.mq;
     float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[((int64_t)(2 * s) * a.heads + head) * a.mq + qi]);
+    for (int s = first; s < a.splits; s += lanes) m = fmaxf(m, ml[2 * s * plane]);
+    for (int off = width * lanes / 2; off >= width; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
     const float base = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-        const float w = __builtin_amdgcn_exp2f(a.part_ml[((int64_t)(2 * s) * a.heads + head) * a.mq + qi] - base);
-        sum += w * a.part_ml[((int64_t)(2 * s + 1) * a.heads + head) * a.mq + qi];
-        const f32x4 p = *reinterpret_cast<const f32x4*>(a.part_o + (((int64_t)s * a.mq + qi) * a.heads + head) * a.dim + d);
-        o += w * p;
+    for (int s = first; s < a.splits; s += lanes) {
+        const float w = __builtin_amdgcn_exp2f(ml[2 * s * plane] - base);
+        sum += w * ml[(2 * s + 1) * plane];
+        if (d < a.dim) o += w * *reinterpret_cast<const f32x4*>(a.part_o + (((int64_t)s * a.mq + qi) * a.heads + head) * a.dim + d);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const f32x4 r = o * inv;
+    for (int off = width * lanes / 2; off >= width; off >>= 1) {
+        sum += __shfl_xor(sum, off);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off);
+    }
+    if (a.lse && d == 0 && first == 0) a.lse[(int64_t)head * a.mq + qi] = sum == 0.f ? INFINITY : m + log2f(sum);
+    if (first != 0 || d >= a.dim) return;
+    const f32x4 r = o * (sum == 0.f ? 0.f : 1.f / sum);
     const int64_t at = ((int64_t)qi * a.heads + head) * a.dim + d;
     at_store4((T*)a.out + at, r);
     if (a.out32) at_store4(a.out32 + at, r);
-    if (a.lse && d == 0) a.lse[(int64_t)head * a.mq + qi] = sum == 0.f ? INFINITY : m + log2f(sum);
 }
 
 template <typename T, int DP, int HG, int SLOTS, int BIAS, bool EXACT = false>
@@ -322,12 +329,15 @@ static hipError_t at_fwd_launch(const AtFwd& a, hipStream_t st) {
     constexpr int QB = Plan::kQB;
     const int64_t wg = seg_tiles_bound(a.mq, 64 * QB, a.seg_q, a.nseg) * (a.heads / HG);
     size_t lds = (size_t)2 * AtTile<T, DP, SLOTS, kFwdRows>::kBytes + 2 * 3 * kFwdRows * sizeof(float);
-    if (BIAS == kTable) lds += (kCells + a.bias.buckets * HG) * sizeof(float);
+    if (BIAS == kTable) lds += (kCells + kTableRow * HG) * sizeof(float);
     auto kern = at_fwd_kernel<T, DP, HG, SLOTS, BIAS, QB, EXACT>;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return e;
     kern<<<dim3((unsigned)wg, (unsigned)a.splits), kAtBlock, lds, st>>>(a);
-    if (a.splits > 1) at_join_kernel<T><<<(unsigned)ceil_div((int64_t)a.mq * a.heads * (a.dim / 4), 256), 256, 0, st>>>(a);
+    if (a.splits > 1) {
+        const int width = DP / 4, lanes = a.splits > 8 ? kWave / width : 1;
+        at_join_kernel<T><<<(unsigned)ceil_div((int64_t)a.mq * a.heads * width * lanes, 256), 256, 0, st>>>(a, width, lanes);
+    }
     return hipGetLastError();
 }
 
