@@ -12,7 +12,13 @@ namespace lidiff {
 
 constexpr int kGnBlock = 256;
 constexpr int kGnSlabs = 1024;           // workgroups of a reduction over all scans together (4 per compute unit)
-constexpr int kGnRowsPerThread = 16;     // rows a thread of the writing pass walks over
+constexpr int kGnRowsPerThread = 16;     // rows a thread of the writing pass walks over, fewer where that would leave compute units idle
+
+// rows of a workgroup of the writing pass (5 824 x 256, fp32: 8.2 us with 16 rows a thread, 7.5 with one)
+static int gn_tile(int rows, int rpb) {
+    const int n = rows / (rpb * kGnSlabs);
+    return rpb * (n < 1 ? 1 : n < kGnRowsPerThread ? n : kGnRowsPerThread);
+}
 
 typedef __bf16 gn_bf16;
 typedef _Float16 gn_f16;
@@ -124,10 +130,10 @@ __global__ __launch_bounds__(kWave) void gn_finish_kernel(const double* __restri
 
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnBlock) void gn_apply_kernel(const T* __restrict__ x, int rows, int c, int groups, const int32_t* __restrict__ seg, int nseg,
-                                                           const float2* __restrict__ stats, const float* __restrict__ w, const float* __restrict__ b,
+                                                           int tile, const float2* __restrict__ stats, const float* __restrict__ w, const float* __restrict__ b,
                                                            T* __restrict__ y) {
     const GnLane<V> at(c);
-    const SegTile t = find_seg_tile(seg, nseg, rows, at.rpb * kGnRowsPerThread, blockIdx.x);
+    const SegTile t = find_seg_tile(seg, nseg, rows, tile, blockIdx.x);
     if (!at.on) return;
     float mean[V], scale[V], shift[V];
     const int per = c / groups;
@@ -203,6 +209,7 @@ __global__ __launch_bounds__(256) void gn_bwd_finish_kernel(const double* __rest
     const int cols = (c2 + 15) / 16, s = blockIdx.x / cols, col = (blockIdx.x % cols) * 16 + (threadIdx.x & 15), l = threadIdx.x >> 4;
     double t = 0;
     if (col < c2)
+#pragma unroll 8
         for (int i = l; i < nblk; i += 16) t += part[((int64_t)s * nblk + i) * c2 + col];
     sm[l][threadIdx.x & 15] = t;
     __syncthreads();
@@ -216,12 +223,13 @@ __global__ __launch_bounds__(256) void gn_bwd_finish_kernel(const double* __rest
 // the last workgroup of the grid adds the scans' A_c / B_c to db / dw; the others write dx
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnBlock) void gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ dy, int rows, int c, int groups,
-                                                               const int32_t* __restrict__ seg, int nseg, const float2* __restrict__ stats,
+                                                               const int32_t* __restrict__ seg, int nseg, int tile, const float2* __restrict__ stats,
                                                                const double* __restrict__ chan, const float* __restrict__ w, const float* __restrict__ b,
                                                                T* __restrict__ dx, float* __restrict__ dw, float* __restrict__ db) {
     if (blockIdx.x == gridDim.x - 1) {
         for (int ch = threadIdx.x; ch < c; ch += kGnBlock) {
             double a = 0, bb = 0;
+#pragma unroll 16
             for (int s = 0; s < nseg; ++s) { a += chan[(int64_t)s * 2 * c + ch]; bb += chan[((int64_t)s * 2 + 1) * c + ch]; }
             if (db) db[ch] = (float)a;
             if (dw) dw[ch] = (float)bb;
@@ -230,7 +238,7 @@ __global__ __launch_bounds__(kGnBlock) void gn_bwd_apply_kernel(const T* __restr
     }
     __shared__ float sums[2 * 1024];                                    // per group: sum w A / n, sum w B / n
     const GnLane<V> at(c);
-    const SegTile t = find_seg_tile(seg, nseg, rows, at.rpb * kGnRowsPerThread, blockIdx.x);
+    const SegTile t = find_seg_tile(seg, nseg, rows, tile, blockIdx.x);
     if (t.lo >= t.hi) return;                                           // (the same for the whole workgroup)
     const int per = c / groups;
     if (t.seg >= 0) {
@@ -285,23 +293,23 @@ static int gn_slabs(int64_t rows, int c, int v, int64_t nseg) {
 template <typename T, int V, int ACT>
 static void gn_fwd_launch(const void* x, int rows, int c, int groups, const int32_t* seg, int nseg, const float* w, const float* b, float eps, void* y,
                           float2* stats, double* ws, hipStream_t st) {
-    const int nblk = gn_slabs(rows, c, V, nseg), rpb = kGnBlock / (c / V);
+    const int nblk = gn_slabs(rows, c, V, nseg), rpb = kGnBlock / (c / V), tile = gn_tile(rows, rpb);
     gn_stats_kernel<T, V><<<(unsigned)(nseg * nblk), kGnBlock, (size_t)rpb * c * 2 * sizeof(double), st>>>((const T*)x, rows, c, groups, seg, nblk, ws);
     gn_finish_kernel<<<(unsigned)(nseg * groups), kWave, 0, st>>>(ws, nblk, rows, c, groups, seg, eps, stats);
-    gn_apply_kernel<T, V, ACT><<<(unsigned)seg_tiles_bound(rows, rpb * kGnRowsPerThread, seg, nseg), kGnBlock, 0, st>>>(
-        (const T*)x, rows, c, groups, seg, nseg, stats, w, b, (T*)y);
+    gn_apply_kernel<T, V, ACT><<<(unsigned)seg_tiles_bound(rows, tile, seg, nseg), kGnBlock, 0, st>>>(
+        (const T*)x, rows, c, groups, seg, nseg, tile, stats, w, b, (T*)y);
 }
 
 template <typename T, int V, int ACT>
 static void gn_bwd_launch(const void* x, const void* dy, int rows, int c, int groups, const int32_t* seg, int nseg, const float2* stats, const float* w,
                           const float* b, void* dx, float* dw, float* db, double* ws, hipStream_t st) {
-    const int nblk = gn_slabs(rows, c, V, nseg), rpb = kGnBlock / (c / V);
+    const int nblk = gn_slabs(rows, c, V, nseg), rpb = kGnBlock / (c / V), tile = gn_tile(rows, rpb);
     double* chan = ws + (int64_t)nseg * nblk * 2 * c;
     gn_bwd_sums_kernel<T, V, ACT><<<(unsigned)(nseg * nblk), kGnBlock, (size_t)rpb * c * 2 * sizeof(double), st>>>((const T*)x, (const T*)dy, rows, c, groups, seg,
                                                                                                                 nblk, stats, w, b, ws);
     gn_bwd_finish_kernel<<<(unsigned)(nseg * ((2 * c + 15) / 16)), 256, 0, st>>>(ws, nblk, 2 * c, chan);
-    gn_bwd_apply_kernel<T, V, ACT><<<(unsigned)(seg_tiles_bound(rows, rpb * kGnRowsPerThread, seg, nseg) + 1), kGnBlock, 0, st>>>(
-        (const T*)x, (const T*)dy, rows, c, groups, seg, nseg, stats, chan, w, b, (T*)dx, dw, db);
+    gn_bwd_apply_kernel<T, V, ACT><<<(unsigned)(seg_tiles_bound(rows, tile, seg, nseg) + 1), kGnBlock, 0, st>>>(
+        (const T*)x, (const T*)dy, rows, c, groups, seg, nseg, tile, stats, chan, w, b, (T*)dx, dw, db);
 }
 
 // 16-byte accesses: 8 channels of a 16-bit type where C allows it, 4 otherwise

@@ -1998,6 +1998,18 @@ _ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2}
 _BIAS_NONE, _BIAS_SLOPES, _BIAS_TABLE = 0, 1, 2
 MAX_BUCKETS = 48
+_ON_CURRENT = contextlib.nullcontext()
+
+
+def _on(device):
+    """The context in which launches for tensors on `device` are made (its current stream; nothing to enter on the current device)."""
+    return _ON_CURRENT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream_of(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 MAX_EDGE = 1 << 22        # squared distances are exact in fp32 far beyond this (2^24)
 _CELL_BITS = 5            # kCellBits of attention.h
 
@@ -2025,11 +2037,11 @@ def batch_segments(coords: torch.Tensor, n_batches: int | None = None, d_rows: t
         n_batches = int(valid[:, 0].max().item()) + 1 if valid.shape[0] else 1
         if n_batches < 1:
             raise ValueError("batch indices must not be negative")
-    with torch.cuda.device(coords.device):
+    with _on(coords.device):
         seg = torch.zeros((replicas * n_batches, 2), dtype=torch.int32, device=coords.device)
         if status is None:
             status = torch.zeros(1, dtype=torch.int32, device=coords.device)
-        call("lidiff_batch_segments", ptr(coords), rows, ptr(d_rows), int(n_batches), int(replicas), ptr(seg), ptr(status), stream_ptr())
+        call("lidiff_batch_segments", ptr(coords), rows, ptr(d_rows), int(n_batches), int(replicas), ptr(seg), ptr(status), _stream_of(coords.device))
     if read and int(status.item()) & STATUS_BATCH_ORDER:
         raise ValueError("rows are not grouped by ascending batch index")
     return seg
@@ -2065,7 +2077,7 @@ class _GroupNorm(torch.autograd.Function):
         if m:
             ws = torch.empty(_lib.load().lidiff_group_norm_workspace_bytes(c, n_seg), dtype=torch.uint8, device=x.device)
             call("lidiff_group_norm", ptr(x), m, c, groups, _ROW_DTYPES[x.dtype], ptr(segments), n_seg, ptr(w), ptr(b), float(eps),
-                 act, ptr(y), ptr(stats), ptr(ws), stream_ptr())
+                 act, ptr(y), ptr(stats), ptr(ws), _stream_of(x.device))
         ctx.save_for_backward(x, weight, bias, segments, stats)
         ctx.args = (groups, act)
         return y
@@ -2083,14 +2095,14 @@ class _GroupNorm(torch.autograd.Function):
         dw = new(c, dtype=torch.float32, device=dev) if need_w else None
         db = new(c, dtype=torch.float32, device=dev) if need_b else None
         if m:
-            with torch.cuda.device(dev):
+            with _on(dev):
                 n_seg = stats.shape[0]
                 dy = _aligned(dy)
                 w = None if weight is None else _aligned(weight.detach().float())
                 b = None if bias is None else _aligned(bias.detach().float())
                 ws = torch.empty(_lib.load().lidiff_group_norm_workspace_bytes(c, n_seg), dtype=torch.uint8, device=dev)
                 call("lidiff_group_norm_bwd", ptr(x), ptr(dy), m, c, groups, _ROW_DTYPES[x.dtype], ptr(segments), n_seg, ptr(w), ptr(b),
-                     ptr(stats), act, ptr(dx), ptr(dw), ptr(db), ptr(ws), stream_ptr())
+                     ptr(stats), act, ptr(dx), ptr(dw), ptr(db), ptr(ws), _stream_of(dev))
         return (dx if ctx.needs_input_grad[0] else None, dw.to(weight.dtype) if need_w else None, db.to(bias.dtype) if need_b else None,
                 None, None, None, None)
 
@@ -2125,7 +2137,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
     _same_device(x.device, weight=weight, bias=bias)
     _check_segments("segments", segments, x.device)
     require_device(x)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         return _GroupNorm.apply(x, weight, bias, None if segments is None else segments.contiguous(), int(num_groups), float(eps),
                                 _ACTIVATIONS[activation])
 
@@ -2212,7 +2224,7 @@ class _SegmentAttention(torch.autograd.Function):
             call("lidiff_segment_attention", ptr(q), ptr(k), ptr(v), _strides(q, k, v), ptr(coords_q), ptr(coords_k), ptr(seg_q), ptr(seg_k),
                  n_seg, mq, mk, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], float(scale), mode, ptr(slopes), ptr(tab), ptr(cells),
                  0 if table is None else table.shape[0], ptr(out), ptr(out32) if out32 is not out else None,
-                 int(table is not None and ctx.needs_input_grad[3]), ptr(lse), ptr(ws), stream_ptr())
+                 int(table is not None and ctx.needs_input_grad[3]), ptr(lse), ptr(ws), _stream_of(dev))
         if grads:
             ctx.save_for_backward(q, k, v, table, seg_q, seg_k, coords_q, coords_k, slopes, out32, lse)
             ctx.edges, ctx.scale, ctx.mode = edges, scale, mode
@@ -2225,7 +2237,7 @@ class _SegmentAttention(torch.autograd.Function):
         (mq, heads, dim), (mk, kv_heads, _) = q.shape, k.shape
         dev = q.device
         need_kv, need_t = ctx.needs_input_grad[1] or ctx.needs_input_grad[2], table is not None and ctx.needs_input_grad[3]
-        with torch.cuda.device(dev):
+        with _on(dev):
             new = torch.empty if mq else torch.zeros
             dq = torch.empty((mq, heads, dim), dtype=q.dtype, device=dev)
             dk, dv = (new((mk, kv_heads, dim), dtype=q.dtype, device=dev) if need_kv else None for _ in range(2))
@@ -2240,7 +2252,7 @@ class _SegmentAttention(torch.autograd.Function):
                 call("lidiff_segment_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(go), _strides(q, k, v, go), ptr(coords_q), ptr(coords_k),
                      ptr(seg_q), ptr(seg_k), n_seg, mq, mk, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], float(ctx.scale), ctx.mode,
                      ptr(slopes), ptr(tab), ptr(None if table is None else _device_cells(ctx.edges, dev)), buckets, ptr(out32), ptr(lse),
-                     ptr(dq), ptr(dk), ptr(dv), ptr(dt), ptr(ws), stream_ptr())
+                     ptr(dq), ptr(dk), ptr(dv), ptr(dt), ptr(ws), _stream_of(dev))
         need = ctx.needs_input_grad
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dt.to(table.dtype) if need_t else None) + (None,) * 7
 
@@ -2298,7 +2310,7 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seg_q: 
         raise ValueError(f"scale must lie in [1e-6, 1e6], got {scale}")
     require_device(q)
     fit = lambda t: None if t is None else _aligned(t)
-    with torch.cuda.device(dev):
+    with _on(dev):
         biased = slopes is not None or bias is not None
         return _SegmentAttention.apply(q, k, v, bias, fit(seg_q), fit(seg_k), fit(coords_q) if biased else None, fit(coords_k) if biased else None,
                                        None if slopes is None else _aligned(slopes.float()), edges, scale)
