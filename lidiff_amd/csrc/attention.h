@@ -35,9 +35,9 @@ struct AtPieces { bf16x8 p[3]; };
 template <typename T> struct AtType;
 // waves a SIMD the kernels are compiled for (the widest fp32 rows need more than 256 registers)
 constexpr int at_waves(int bytes, int width) { return bytes == 4 && width == 128 ? 1 : 2; }
-template <> struct AtType<__bf16> { typedef bf16x8 Frag; typedef bf16x4 Quad; typedef __bf16 Elem; static constexpr int kPlanes = 1, kLift = 0; };
-template <> struct AtType<_Float16> { typedef f16x8 Frag; typedef f16x4 Quad; typedef _Float16 Elem; static constexpr int kPlanes = 1, kLift = 15; };
-template <> struct AtType<float> { typedef AtPieces Frag; typedef f32x4 Quad; typedef __bf16 Elem; static constexpr int kPlanes = 3, kLift = 0; };
+template <> struct AtType<__bf16> { typedef bf16x8 Frag; typedef bf16x4 Quad; typedef __bf16 Elem; static constexpr int kPlanes = 1, kLift = 0, kPieces = 3; };
+template <> struct AtType<_Float16> { typedef f16x8 Frag; typedef f16x4 Quad; typedef _Float16 Elem; static constexpr int kPlanes = 1, kLift = 15, kPieces = 2; };
+template <> struct AtType<float> { typedef AtPieces Frag; typedef f32x4 Quad; typedef __bf16 Elem; static constexpr int kPlanes = 3, kLift = 0, kPieces = 1; };
 
 // acc += A B over 32 terms: lane group g holds the terms 8 g .. 8 g + 7 of row (A) / column (B) lane & 15
 __device__ __forceinline__ void at_mma(f32x4& acc, const bf16x8& a, const bf16x8& b) { acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0); }
@@ -100,11 +100,11 @@ __device__ __forceinline__ void at_pack(AtPieces& f, const f32x8& v) {
     at_pack(f.p[1], r);
     at_pack(f.p[2], r - __builtin_convertvector(f.p[1], f32x8));
 }
-// what the rounding of at_pack left, as a second operand: two pieces carry 16 (bf16) or 22 (fp16) bits; a third one changed the table
-// gradient of 3 10^8 pairs by nothing (1.19e-6 against 1.18e-6)
+// what the rounding of at_pack left (v: the values on entry, what is still left on return), as a further operand
 template <typename F>
-__device__ __forceinline__ void at_pack_rest(F& rest, const F& piece, const f32x8& v) {
-    at_pack(rest, v - __builtin_convertvector(piece, f32x8));
+__device__ __forceinline__ void at_pack_rest(F& rest, const F& piece, f32x8& v) {
+    v -= __builtin_convertvector(piece, f32x8);
+    at_pack(rest, v);
 }
 
 // a value that only the branch it stands in knows: keeps a rarely taken branch a branch (the compiler would turn it into selections that

@@ -205,6 +205,27 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
 #pragma unroll
             for (int b = 0; b < DB; ++b) dq[n][h][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    // The columns' sums go over into doubles every kGather tiles: a word then holds a few hundred values, and its rounding does not show in
+    // the sum of 3 10^8 (5 10^-7 of it with 2 000 a word).
+    constexpr int kGather = 64, kSums = (4 * HG * 48 + kAtBlock - 1) / kAtBlock;
+    double sums[kSums] = {};
+    auto gather = [&]() {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) {
+            const int i = k * kAtBlock + threadIdx.x;
+            if (i >= 4 * HG * a.bias.buckets) continue;
+            double u = 0;                                      // (64 lanes in a fixed order; neighbouring threads in neighbouring banks)
+            for (int l = 0; l < 64; ++l) {
+                float& word = hist[i * 64 + ((l + i) & 63)];
+                u += word;
+                word = 0.f;
+            }
+            sums[k] += u;
+        }
+        __syncthreads();
+    };
+
     int4 kc = make_int4(0, 0, 0, 0);                           // the coordinates one tile further than the requests
     auto coords = [&](int tile) {
         const int row = k_lo + tile * ROWS + (int)threadIdx.x;
@@ -311,6 +332,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                 }
             }
         }
+        if (GRAD && (tile + 1) % kGather == 0) gather();       // (every wave is here)
         if (tile + 1 < last) {
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the tile has been read
             request(tile + 1);
@@ -327,11 +349,15 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                 if (16 * b + 4 * g < a.dim) at_store4((T*)a.dq + ((int64_t)qi * a.heads + h0 + h) * a.dim + 16 * b + 4 * g, dq[n][h][b] * (a.scale * unlift[n][h]));
     }
     if (GRAD) {
+        gather();
+        double* const wide = reinterpret_cast<double*>(hist);
+#pragma unroll
+        for (int k = 0; k < kSums; ++k)
+            if (k * kAtBlock + threadIdx.x < 4 * HG * a.bias.buckets) wide[k * kAtBlock + threadIdx.x] = sums[k];
         __syncthreads();
         for (int i = threadIdx.x; i < HG * a.bias.buckets; i += kAtBlock) {
-            double u = 0;                                      // (the 4 x 64 lanes' sums in a fixed order)
-            for (int w = 0; w < 4; ++w)
-                for (int l = 0; l < 64; ++l) u += hist[(w * HG * a.bias.buckets + i) * 64 + ((l + i) & 63)];
+            double u = 0;
+            for (int w = 0; w < 4; ++w) u += wide[w * HG * a.bias.buckets + i];
             a.part_t[((int64_t)tile_id * a.heads + h0 + i % HG) * a.bias.buckets + i / HG] = (float)u;
         }
     }

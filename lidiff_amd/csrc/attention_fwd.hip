@@ -33,7 +33,7 @@ struct AtFwd {
 // at 5 824 x 5 824; bf16: 1.41 against 1.23, for the registers).
 template <typename T, int DP> struct AtFwdPlan {
     static constexpr int kHeads = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 ? 2 : 1;
-    static constexpr int kExactHeads = kHeads > 2 ? 2 : kHeads;      // (the second pieces take the registers of two heads: 1.63 against 1.91 ms)
+    static constexpr int kExactHeads = kHeads > 2 ? 2 : kHeads;      // (the pieces take the registers of two heads: 1.63 against 1.91 ms)
     static constexpr int kQB = sizeof(T) == 4 && DP <= 64 ? 2 : 1;
 };
 constexpr int kFwdRows = 64;
@@ -43,8 +43,9 @@ inline int at_fwd_heads(int most, int heads, int share, int mode) {      // whol
 }
 
 // EXACT (16-bit operands, when the table's gradient is wanted): probabilities enter the product with the values in pieces, rounding and
-// rest.  d table sums ds over millions of pairs whose rows cancel to zero through delta = do . out, so an output from probabilities of 8 or
-// 11 bits costs it more than fp32 sums do.
+// rests (bf16 three: 24 bits, fp16 two: 22).  d table sums ds over millions of pairs whose rows cancel to zero through delta = do . out, so
+// the rounding of the probabilities behind out shows in it.  Of 2 x 12 809^2 pairs, bf16, against 64 bits: one piece 10^-3, two 1.2e-6,
+// three 0.8e-6, the same in fp32 torch operations 0.8e-6; two pieces take 1.67 ms, three 2.0.
 template <typename T, int DP, int HG, int SLOTS, int BIAS, int QB, bool EXACT>
 __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kernel(const AtFwd a) {
     constexpr int ROWS = kFwdRows, DC = DP / 32, DB = DP / 16, KB = ROWS / 16;
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
                             at_here(s[n][b]);
                         }
                 }
-                constexpr int PIECES = EXACT ? 2 : 1;
+                constexpr int PIECES = EXACT ? AtType<T>::kPieces : 1;
                 Frag p[QB][KB / 2][PIECES];
 #pragma unroll
                 for (int n = 0; n < QB; ++n) {
@@ -216,9 +217,12 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
                         }
 #pragma unroll
                     for (int j = 0; j < KB / 2; ++j) {
-                        const f32x8 v = at_join(s[n][2 * j], s[n][2 * j + 1]);
+                        f32x8 v = at_join(s[n][2 * j], s[n][2 * j + 1]);
                         at_pack(p[n][j][0], v);
-                        if constexpr (EXACT) at_pack_rest(p[n][j][1], p[n][j][0], v);
+                        if constexpr (PIECES > 1) {
+#pragma unroll
+                            for (int i = 1; i < PIECES; ++i) at_pack_rest(p[n][j][i], p[n][j][i - 1], v);
+                        }
                         if constexpr (kOnes) {
 #pragma unroll
                             for (int i = 0; i < PIECES; ++i) at_mma(l[n][h], ones, p[n][j][i]);
