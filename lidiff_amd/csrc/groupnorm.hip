@@ -331,6 +331,7 @@ static void gn_bwd_launch(const void* x, const void* dy, int rows, int c, int gr
 static const char* gn_check(int64_t rows, int c, int groups, int dtype, int64_t nseg, int act) {
     if (rows < 1 || rows > 0x7fffffff - 65536) return "need 1 <= rows < 2^31 - 65536";
     if (c < 4 || c > 1024 || c % 4) return "need a multiple of 4 channels in [4, 1024]";
+    if (rows * c > (int64_t)1 << 33) return "need rows x channels <= 2^33";                  // (one launch's workgroups)
     if (groups < 1 || c % groups) return "the groups must divide the channels";
     if (dtype < 0 || dtype > 2) return "dtype: 0 fp32, 1 bf16, 2 fp16";
     if (nseg < 1 || nseg > 1 << 20) return "need 1 <= segments <= 2^20";

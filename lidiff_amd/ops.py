@@ -2205,11 +2205,10 @@ class _SegmentAttention(torch.autograd.Function):
     """Attention within a scan with a distance bias (attention_fwd.hip, attention_bwd.hip)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, table, seg_q, seg_k, coords_q, coords_k, slopes, edges, scale):
+    def forward(ctx, q, k, v, table, seg_q, seg_k, coords_q, coords_k, slopes, edges, scale, grads):
         q, k, v = _heads_rows(q), _heads_rows(k), _heads_rows(v)
         (mq, heads, dim), (mk, kv_heads, _) = q.shape, k.shape
         dev = q.device
-        grads = any(ctx.needs_input_grad[:4])
         mode = _BIAS_TABLE if table is not None else _BIAS_SLOPES if slopes is not None else _BIAS_NONE
         tab = None if table is None else _aligned(table.detach().float())
         cells = None if table is None else _device_cells(edges, dev)
@@ -2224,7 +2223,7 @@ class _SegmentAttention(torch.autograd.Function):
             call("lidiff_segment_attention", ptr(q), ptr(k), ptr(v), _strides(q, k, v), ptr(coords_q), ptr(coords_k), ptr(seg_q), ptr(seg_k),
                  n_seg, mq, mk, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], float(scale), mode, ptr(slopes), ptr(tab), ptr(cells),
                  0 if table is None else table.shape[0], ptr(out), ptr(out32) if out32 is not out else None,
-                 int(table is not None and ctx.needs_input_grad[3]), ptr(lse), ptr(ws), _stream_of(dev))
+                 int(grads and table is not None and ctx.needs_input_grad[3]), ptr(lse), ptr(ws), _stream_of(dev))
         if grads:
             ctx.save_for_backward(q, k, v, table, seg_q, seg_k, coords_q, coords_k, slopes, out32, lse)
             ctx.edges, ctx.scale, ctx.mode = edges, scale, mode
@@ -2254,7 +2253,7 @@ class _SegmentAttention(torch.autograd.Function):
                      ptr(slopes), ptr(tab), ptr(None if table is None else _device_cells(ctx.edges, dev)), buckets, ptr(out32), ptr(lse),
                      ptr(dq), ptr(dk), ptr(dv), ptr(dt), ptr(ws), _stream_of(dev))
         need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dt.to(table.dtype) if need_t else None) + (None,) * 7
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dt.to(table.dtype) if need_t else None) + (None,) * 8
 
 
 def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seg_q: torch.Tensor | None = None,
@@ -2270,7 +2269,8 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seg_q: 
       bias [buckets, H]     a learned table: bias[b, h], b = number of `edges` (ascending whole squared distances, one less than
                             buckets: distance_edges) that |c_i - c_j|^2 reaches
     Gradients for q, k, v and bias; deterministic.  The backward pass keeps q, k, v, an fp32 copy of the output and one number per
-    query and head -- never the scores."""
+    query and head -- never the scores.  A first call with new `edges` copies a small table to the device: make one before capturing a
+    graph."""
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
         raise ValueError(f"need q [Mq, H, D] and k, v [Mk, Hkv, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if q.dtype not in _ROW_DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -2312,5 +2312,7 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seg_q: 
     fit = lambda t: None if t is None else _aligned(t)
     with _on(dev):
         biased = slopes is not None or bias is not None
+        # (a parameter under no_grad asks for nothing: no fp32 copy, no statistics, no second pieces)
+        grads = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias))
         return _SegmentAttention.apply(q, k, v, bias, fit(seg_q), fit(seg_k), fit(coords_q) if biased else None, fit(coords_k) if biased else None,
-                                       None if slopes is None else _aligned(slopes.float()), edges, scale)
+                                       None if slopes is None else _aligned(slopes.float()), edges, scale, grads)

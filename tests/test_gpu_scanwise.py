@@ -244,6 +244,38 @@ def test_attention_buckets_are_exact(ops):
             assert torch.allclose(g[:, 0].double(), torch.bincount(want[keys], ds, minlength=buckets), rtol=1e-4, atol=1e-5)
 
 
+def test_attention_keeps_nothing_where_no_gradient_is_asked_for(ops, monkeypatch):
+    """Parameters that require gradients, under no_grad: the inference call (no fp32 output, no statistics, one piece), same bits."""
+    gen = generator(15)
+    q, k, v = (rand(gen, 60, 4, 32, dtype=BF16) for _ in range(3))
+    kw = dict(coords_q=voxel_rows(gen, 60), coords_k=voxel_rows(gen, 60), edges=edges_of(ops, 16))
+    table = rand(gen, 16, 4)
+    want = ops.segment_attention(q, k, v, bias=table, **kw)
+    seen = []
+    real = ops.call
+    monkeypatch.setattr(ops, "call", lambda name, *a, **k: (seen.append(a), real(name, *a, **k))[1])
+    with torch.no_grad():
+        got = ops.segment_attention(q.clone().requires_grad_(), k, v, bias=table.clone().requires_grad_(), **kw)
+    assert torch.equal(got, want) and not got.requires_grad
+    assert seen[0][22:25] == (None, 0, None)                     # out_f32, exact, lse
+
+
+def test_attention_of_a_long_scan_with_the_table_s_gradient(ops):
+    """Keys beyond the 64 tiles after which the histogram's words are gathered, every width and type of that kernel, more queries than a
+    workgroup takes."""
+    for heads, dim, buckets in ((2, 32, 48), (1, 64, 33), (1, 128, 48), (3, 16, 8)):
+        for dtype in (F32, BF16, F16):
+            gen = generator(heads * dim)
+            a = dict(q=rand(gen, 140, heads, dim, dtype=dtype), k=rand(gen, 4300, heads, dim, dtype=dtype), v=rand(gen, 4300, heads, dim, dtype=dtype))
+            kw = dict(coords_q=voxel_rows(gen, 140), coords_k=voxel_rows(gen, 4300), bias=rand(gen, buckets, heads), edges=edges_of(ops, buckets))
+            go = rand(gen, 140, heads, dim, dtype=dtype)
+            val, bnd = reference(a, kw, go)
+            leaves = [a[n].requires_grad_() for n in "qkv"] + [kw["bias"].requires_grad_()]
+            out = ops.segment_attention(*leaves[:3], **kw)
+            for name, got in zip(("out", "dq", "dk", "dv", "dt"), (out.detach(),) + torch.autograd.grad(out, leaves, go)):
+                assert_within(got, val[name].detach(), bnd[name].detach(), 1e-30 if name == "dt" else TINY[dtype], f"{name} {heads} x {dim} {dtype}")
+
+
 def test_attention_layouts(ops):
     """Slices of one fused projection, heads first, one broadcast key row, misaligned storage: the values of contiguous copies."""
     gen = generator(8)

@@ -90,7 +90,8 @@ def test_library_refuses_before_it_launches():
         return rc, lib.lidiff_last_error().decode()
     for kw, word in ((dict(x=None), "null"), (dict(rows=0), "rows"), (dict(c=30), "multiple of 4"), (dict(c=2048), "multiple of 4"), (dict(groups=5), "divide"),
                      (dict(dtype=3), "dtype"), (dict(nseg=0), "segments"), (dict(nseg=2, seg=None), "one"), (dict(act=3), "activation"),
-                     (dict(x=ctypes.c_void_p(4100)), "misaligned"), (dict(rows=2 ** 31), "rows")):
+                     (dict(x=ctypes.c_void_p(4100)), "misaligned"), (dict(rows=2 ** 31), "rows"),
+                     (dict(rows=2 ** 30, c=512), "channels")):
         rc, msg = norm(**kw)
         assert rc == 1 and word in msg, (kw, msg)
     base = dict(q=P(), k=P(2), v=P(3), strides=[128, 32] * 3, cq=P(4), ck=P(5), sq=P(6), sk=P(7), nseg=1, mq=8, mk=8, h=4, hk=4, d=32, dtype=0, mode=0, scale=0.1, slopes=None,
@@ -102,7 +103,7 @@ def test_library_refuses_before_it_launches():
                                           None, None, None)
         return rc, lib.lidiff_last_error().decode()
     for kw, word in ((dict(q=None), "null"), (dict(k=None), "null"), (dict(sq=None), "together"), (dict(nseg=0), "segments"), (dict(mq=0), "rows"), (dict(mk=-1), "rows"),
-                     (dict(mq=2 ** 31), "rows"), (dict(hk=3), "divide"), (dict(d=36), "head dimension"), (dict(d=256), "head dimension"), (dict(dtype=7), "dtype"),
+                     (dict(mq=2 ** 31), "rows"), (dict(mq=2 ** 28), "2^26"), (dict(mk=2 ** 28), "2^26"), (dict(hk=3), "divide"), (dict(d=36), "head dimension"), (dict(d=256), "head dimension"), (dict(dtype=7), "dtype"),
                      (dict(mode=3), "bias"), (dict(mode=1), "null"), (dict(mode=1, cq=None, slopes=P()), "coordinates"), (dict(mode=2, buckets=49), "buckets"),
                      (dict(mode=2, buckets=8), "null"), (dict(strides=[127, 32] * 3), "16-byte"), (dict(strides=[-128, 32] * 3), "16-byte"), (dict(strides=[1 << 22, 32] * 3), "row stride"), (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"),
                      (dict(q=ctypes.c_void_p(4104)), "misaligned"), (dict(mk=5000), "workspace missing")):
