@@ -28,6 +28,9 @@ struct AtFwd {
 
 // What a workgroup takes: QB x 16 queries a wave, HG heads, tiles of 64 keys.
 // HG: the distances of a (query, key) pair are the same for every head, so a wave takes as many heads as its registers hold.
+// What bounds it: issue of vector instructions (bf16, 4 heads of 32, slopes: some 115 a head and 64 keys, 67 % of the time busy; matrix pipe
+// 17 %, LDS 30 %).  The next head's products started ahead of this head's probabilities gave nothing (1.19 against 1.18 ms; with the table
+// 2.0 against 1.5: a wave less): the other waves of the SIMD fill those cycles already.
 // One buffer per tile: three workgroups of a compute unit cover each other's waits better than two with a second buffer do (41 157 x 5 824
 // x 2, bf16: 1.23 against 1.48 ms).  fp32 operands are three times the LDS reads: two blocks of queries share them (0.38 against 0.42 ms
 // at 5 824 x 5 824; bf16: 1.41 against 1.23, for the registers).
