@@ -254,10 +254,15 @@ constexpr int kTableRow = 64;
 __device__ __forceinline__ void at_put_cells(unsigned* __restrict__ cells, const unsigned* __restrict__ src) {
     for (int i = threadIdx.x; i < kCells; i += kAtBlock) cells[i] = (src[i] >> 8 << 10) | (src[i] & 255u) * 4;
 }
+// A finite entry is cut to 2^14 in units of log 2: beside any other score it is zero (or everything) long before that, and a row whose keys
+// all carry the type's lowest value still has scores that differ and sums that fp32 resolves.
 template <int HG>
 __device__ __forceinline__ void at_put_table(float* __restrict__ table, const AtBias& bias, int heads, int h0, float scale) {
-    for (int i = threadIdx.x; i < bias.buckets * HG; i += kAtBlock)
-        table[i / bias.buckets * kTableRow + i % bias.buckets] = bias.table[(int64_t)(i % bias.buckets) * heads + h0 + i / bias.buckets] / scale;
+    const float most = 16384.f / kLog2e;
+    for (int i = threadIdx.x; i < bias.buckets * HG; i += kAtBlock) {
+        const float v = bias.table[(int64_t)(i % bias.buckets) * heads + h0 + i / bias.buckets];
+        table[i / bias.buckets * kTableRow + i % bias.buckets] = (fabsf(v) < INFINITY ? fminf(fmaxf(v, -most), most) : v) / scale;
+    }
 }
 __device__ __forceinline__ int at_bucket(const unsigned* cells, float d2) {
     const int bits = __builtin_bit_cast(int, d2);

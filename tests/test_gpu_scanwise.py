@@ -215,6 +215,37 @@ def test_attention_scores_at_the_ends_of_the_range(ops):
         assert torch.equal(lone, torch.full_like(out, 5.0))
 
 
+def test_attention_with_buckets_masked_by_the_lowest_value(ops):
+    """Table entries of -inf and of fp32's lowest value: such keys take no part beside others; a row that sees nothing else gives zeros
+    (-inf), or the softmax of its scores (the lowest value: the same offset for every key)."""
+    gen = generator(16)
+    n, edges = 200, (50 * 50,)
+    ck = torch.zeros(n, 4, dtype=torch.int32, device="cuda")
+    ck[:, 1] = torch.arange(n, device="cuda")                     # keys on a line; queries at 0 and far away from every key
+    cq = torch.zeros(6, 4, dtype=torch.int32, device="cuda")
+    cq[3:, 1] = 1000
+    for dtype in (F32, BF16, F16):
+        q, k, v = rand(gen, 6, 2, 32, dtype=dtype), rand(gen, n, 2, 32, dtype=dtype), rand(gen, n, 2, 32, dtype=dtype)
+        go = rand(gen, 6, 2, 32, dtype=dtype)
+        def both(far):
+            leaves = [t.detach().requires_grad_() for t in (q, k, v)] + [torch.tensor([[0.0, 0.5], [far, far]], device="cuda").requires_grad_()]
+            out = ops.segment_attention(*leaves[:3], coords_q=cq, coords_k=ck, bias=leaves[3], edges=edges)
+            return [out.detach()] + list(torch.autograd.grad(out, leaves, go))
+        near = ops.segment_attention(q[:3], k[:50], v[:50], coords_q=cq[:3], coords_k=ck[:50].contiguous(), bias=torch.tensor([[0.0, 0.5]], device="cuda"), edges=())
+        plain = both(0.0)
+        for far in (-math.inf, torch.finfo(F32).min, -1e9):
+            got = both(far)
+            assert all(torch.isfinite(t).all() for t in got)
+            # (the masked tiles add exact zeros; a table call of another length sums in another order: a few half steps)
+            assert (got[0][:3].double() - near.double()).abs().max() <= 8 * torch.finfo(dtype).eps * v.double().abs().max()
+            if far == -math.inf:
+                assert (got[0][3:] == 0).all() and (got[1][3:] == 0).all()
+            else:
+                # scores near 2^14 / log2 e / scale have steps of 2^-8 / 0.18 score units' worth: probabilities are off by 2 x 7e-4 at most
+                off = (got[0][3:].double() - plain[0][3:].double()).abs().max()
+                assert off <= (2 * 7e-4 + 4 * torch.finfo(dtype).eps) * 2 * v.double().abs().max()
+
+
 def test_attention_buckets_are_exact(ops):
     """A table that spells its bucket, one key per query: every lattice distance up to the last edge and far beyond it."""
     for buckets in (2, 16, 32, 48):
