@@ -22,6 +22,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* at_lds_t;
+typedef uint32_t at_words __attribute__((ext_vector_type(4)));
 
 constexpr int kAtBlock = 256;      // 4 waves; two a SIMD (at_waves): with at most 256 registers the matrix results stay in vector registers
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -62,6 +63,14 @@ __device__ __forceinline__ void at_mma_apart(f32x4& acc, const AtPieces& a, cons
     at_mma(part, a.p[0], b.p[0]);
     acc += low;
     acc += part;
+}
+
+// the operand with its signs turned where `mask` is 0x80008000
+__device__ __forceinline__ void at_turn(bf16x8& f, uint32_t mask) { f = __builtin_bit_cast(bf16x8, __builtin_bit_cast(at_words, f) ^ mask); }
+__device__ __forceinline__ void at_turn(f16x8& f, uint32_t mask) { f = __builtin_bit_cast(f16x8, __builtin_bit_cast(at_words, f) ^ mask); }
+__device__ __forceinline__ void at_turn(AtPieces& f, uint32_t mask) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) at_turn(f.p[i], mask);
 }
 
 // x into its pieces; a value that is not finite goes into the first alone (so that it stays what it is), and one that rounds beyond

@@ -141,6 +141,10 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
     // -delta: what the products do . v start from.  (With the table's gradient it is added behind them: the matrix pipe rounds sums to one
     // side, and what is the same for every pair does not cancel in a sum over 10^8 of them -- 1.9e-5 of the gradient against 1.2e-6.)
     float less[QB][HG];
+    // That side is the lower one also within one product (of fp16's 22 bits more than of bf16's 16 are cut): with do turned for every other
+    // query the cuts fall to both sides alike, for no instruction more (fp16,
+    // 15 158 x 3 082 pairs of 96: 1.2e-6 of the gradient against 1.3e-5; times as before).
+    const float sign = GRAD && (col & 1) ? -1.f : 1.f;
 #pragma unroll
     for (int n = 0; n < QB; ++n) {
         const int qi = q0 + 16 * n + col;
@@ -156,6 +160,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                     const T* go = (const T*)a.go + (int64_t)qi * a.go_row + (int64_t)(h0 + h) * a.go_head + d;
                     qf[n][h][c] = at_load8((const T*)a.q + (int64_t)qi * a.q_row + (int64_t)(h0 + h) * a.q_head + d);
                     gf[n][h][c] = at_load8(go);
+                    if (GRAD) at_turn(gf[n][h][c], col & 1 ? 0x80008000u : 0u);
                     const float* o = a.out32 + ((int64_t)qi * a.heads + h0 + h) * a.dim + d;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -314,7 +319,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                         }
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
-                            s[n][b] *= GRAD ? dp[n][b] + less[n][h] : dp[n][b];
+                            s[n][b] *= GRAD ? dp[n][b] * sign + less[n][h] : dp[n][b];
                             if (GRAD) grads[n][b][h] = kLifted ? s[n][b] * unlift[n][h] : s[n][b];
                         }
                         at_pack(p[n], at_join(s[n][0], s[n][1]));

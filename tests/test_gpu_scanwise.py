@@ -307,6 +307,23 @@ def test_attention_of_a_long_scan_with_the_table_s_gradient(ops):
                 assert_within(got, val[name].detach(), bnd[name].detach(), 1e-30 if name == "dt" else TINY[dtype], f"{name} {heads} x {dim} {dtype}")
 
 
+def test_table_gradient_s_entries_cancel_over_many_rows(ops):
+    """ds of one row sums to zero, so the entries of the table's gradient do: the roundings of 40 000 rows have to fall to both sides.
+
+    A row's own error, with t = sqrt(sum (do out)^2), the size of a partial sum of delta = do . out: 128 additions of delta round by
+    2^-24 t / sqrt(3) each (7 of them to the root), some fifty of out's tiles by as much a component (4 of them), the probabilities' pieces
+    and the products behind dp by less than one: 12 x 2^-24 t.  Rows are independent, so six times the root of the squares' sum bounds it."""
+    rows, dim = 40000, 128
+    for dtype in (F16, BF16, F32):
+        gen = generator(16)
+        q, k, v = (rand(gen, n, 1, dim, dtype=dtype) for n in (rows, 3100, 3100))
+        table, go = rand(gen, 32, 1).requires_grad_(), rand(gen, rows, 1, dim, dtype=dtype)
+        out = ops.segment_attention(q, k, v, coords_q=voxel_rows(gen, rows), coords_k=voxel_rows(gen, 3100), bias=table, edges=edges_of(ops, 32))
+        g, = torch.autograd.grad(out, [table], go)
+        root = (out.detach().double() * go.double()).square().sum().sqrt().item()
+        assert abs(g.double().sum().item()) <= 6 * 12 * 2.0 ** -24 * root, dtype
+
+
 def test_attention_layouts(ops):
     """Slices of one fused projection, heads first, one broadcast key row, misaligned storage: the values of contiguous copies."""
     gen = generator(8)
