@@ -187,8 +187,7 @@ struct AtTile {
             i32x4 rsrc = {(int)(uint32_t)base, (int)(uint32_t)((base >> 32) & 0xffffu), end, 0x00020000};
 #pragma unroll
             for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
-            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                         :: "s"(__builtin_amdgcn_readfirstlane(lds + first * 16)), "v"(voff), "s"(rsrc) : "memory");
+            lds_dma16(rsrc, __builtin_amdgcn_readfirstlane(lds + first * 16), voff, 0);
         }
     }
 

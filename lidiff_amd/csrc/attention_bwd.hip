@@ -457,8 +457,7 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
                 i32x4 rsrc = {(int)(uint32_t)base, (int)(uint32_t)((base >> 32) & 0xffffu), left * 4, 0x00020000};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) rsrc[k] = __builtin_amdgcn_readfirstlane(rsrc[k]);
-                asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                             :: "s"(__builtin_amdgcn_readfirstlane(st_at + i * ROWS * 4)), "v"(lane * 4), "s"(rsrc) : "memory");
+                lds_dma4(rsrc, __builtin_amdgcn_readfirstlane(st_at + i * ROWS * 4), lane * 4, 0);
             }
         };
         __syncthreads();                                       // the chunk of heads before has been read

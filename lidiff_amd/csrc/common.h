@@ -74,6 +74,21 @@ __device__ __forceinline__ int hash_find(const uint64_t* __restrict__ hkeys,
 
 __device__ __forceinline__ int lane_id() { return threadIdx.x & (kWave - 1); }
 
+// LDS-DMA: one request of a wave, 16 (or 4) bytes a lane from a raw buffer descriptor straight into LDS (lane l's at lds_addr + 16 l or + 4 l),
+// from inline asm: the compiler does not see LDS being written behind its back, so it puts no wait for all requests in front of every LDS
+// read; the callers wait before they read.  It does not look into the string either, so the string brings the wait states the hardware asks
+// software for: one between the write of M0 and the load, five between a vector instruction's write of a scalar operand (v_readfirstlane,
+// v_readlane of a spilled one) and the load -- the move and s_nop 3 are those five.
+typedef int dma_rsrc __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void lds_dma16(const dma_rsrc rsrc, const unsigned lds_addr, const int voff, const int soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :: "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
+}
+__device__ __forceinline__ void lds_dma4(const dma_rsrc rsrc, const unsigned lds_addr, const int voff, const int soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :: "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
+}
+
 // number of set bits of `mask` strictly below this lane
 __device__ __forceinline__ int popc_below(unsigned long long mask) {
     return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),

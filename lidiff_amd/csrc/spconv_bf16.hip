@@ -433,11 +433,6 @@ static int dispatch_bf16(const ConvParams& p, bool ks64, hipStream_t st) {
 // barriers alone.  Same pairs, products and order of sums per accumulator as the kernel above: bit-identical results.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ void dma16_to_lds(const i32x4 rsrc, const unsigned lds_addr, const int voff, const int soff) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 :: "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
-}
-
 template <int BM, int WC, int WR>
 __global__ __launch_bounds__(64 * WC * WR) void spconv_fwd_bf16_ring_kernel(const ConvParams p_launch) {
     constexpr int KS = 32, R = 4, D = 3;                    // channels per stage, stages in LDS, stages the requests run ahead
@@ -564,7 +559,7 @@ __global__ __launch_bounds__(64 * WC * WR) void spconv_fwd_bf16_ring_kernel(cons
 #pragma unroll
         for (int j = 0; j < TW; ++j) {
             const int b = (wave + NW * j) % WBLK;
-            dma16_to_lds(rsrc_w, w_base + slot * WBYTES + b * 1024, (((n0 >> 4) + b) * 64 + lane) * 16, ws);
+            lds_dma16(rsrc_w, w_base + slot * WBYTES + b * 1024, (((n0 >> 4) + b) * 64 + lane) * 16, ws);
         }
         const int k0 = slab * KS;
         const bool from_a = k0 < p.c_in_a;
@@ -575,7 +570,7 @@ __global__ __launch_bounds__(64 * WC * WR) void spconv_fwd_bf16_ring_kernel(cons
             const int r = RPI * tblk[j] + lane / NCHK;
             const int row = r < n ? in_list[k * BM + r] : -1;
             const int voff = row >= 0 ? row * cw + chb[j] : (int)0x80000000;          // out of range -> zero fill
-            dma16_to_lds(from_a ? rsrc_a : rsrc_b, a_base + slot * ABYTES + tblk[j] * 1024, voff, cb);
+            lds_dma16(from_a ? rsrc_a : rsrc_b, a_base + slot * ABYTES + tblk[j] * 1024, voff, cb);
         }
         if (++i_slab == nslab) { i_slab = 0; ++i_oi; }
     };
@@ -794,7 +789,7 @@ __global__ __launch_bounds__(512) void spconv_fwd_bf16_wide_kernel(const ConvPar
 #pragma unroll
         for (int j = 0; j < TW; ++j) {
             const int b = (wave + NW * j) % WBLK;
-            dma16_to_lds(rsrc_w, w_base + slot * WBYTES + b * 1024, (((n0 >> 4) + b) * 64 + lane) * 16, ws);
+            lds_dma16(rsrc_w, w_base + slot * WBYTES + b * 1024, (((n0 >> 4) + b) * 64 + lane) * 16, ws);
         }
         const int k0 = slab * KS;
         const bool from_a = k0 < p.c_in_a;
@@ -805,7 +800,7 @@ __global__ __launch_bounds__(512) void spconv_fwd_bf16_wide_kernel(const ConvPar
             const int t = wave + NW * j;
             const int row = live ? raw[k * BM + RPI * t + lane / NCHK] : -1;
             const int voff = row >= 0 ? row * cw + chb[j] : (int)0x80000000;          // no neighbour: zeros, no bytes moved
-            dma16_to_lds(from_a ? rsrc_a : rsrc_b, a_base + slot * ABYTES + t * 1024, voff, cb);
+            lds_dma16(from_a ? rsrc_a : rsrc_b, a_base + slot * ABYTES + t * 1024, voff, cb);
         }
         if (++i_slab == nslab) { i_slab = 0; ++i_oi; }
     };

@@ -47,11 +47,6 @@ __device__ __forceinline__ f32x4 s3_mfma(const f16x8 a, const f16x8 b, const f32
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ void s3_dma16(const i32x4 rsrc, const unsigned lds_addr, const int voff, const int soff) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 :: "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
-}
-
 // a wave-uniform value into a scalar register, whatever register class the compiler computed it in (the "s" operands of the
 // request above: `__builtin_amdgcn_readfirstlane` of a value the compiler has PROVED uniform is folded away, and the operand
 // then arrives in a vector register -- "invalid operand for instruction")
@@ -296,8 +291,7 @@ __global__ __launch_bounds__(512) void spconv_fwd_split3_kernel(const ConvParams
         // (entries behind the tile's last row are masked when they are read; the descriptor's range check keeps the request
         // inside the table)
         const int64_t e0 = (int64_t)k * p.m_out + row0 + 64 * wave;
-        asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds"
-                     :: "s"(rowbuf_base + (oi & 1) * (BM * 4) + wave * 256), "v"((int)(e0 * 4) + lane * 4), "s"(rsrc_n), "s"(0) : "memory");
+        lds_dma4(rsrc_n, rowbuf_base + (oi & 1) * (BM * 4) + wave * 256, (int)(e0 * 4) + lane * 4, 0);
     };
     auto take_rows = [&](int oi) {
 #pragma unroll
@@ -331,7 +325,7 @@ __global__ __launch_bounds__(512) void spconv_fwd_split3_kernel(const ConvParams
     auto issue_w = [&]() {
 #pragma unroll
         for (int b = rqw; b < WBLK; b += NRQ)
-            s3_dma16(rsrc_w, s_base + n_slot * STAGE + ABYTES + b * 1024, (((n0 >> 4) * NP + b) * 64 + lane) * 16, n_ws);
+            lds_dma16(rsrc_w, s_base + n_slot * STAGE + ABYTES + b * 1024, (((n0 >> 4) * NP + b) * 64 + lane) * 16, n_ws);
     };
     auto issue_a = [&]() {
         int soff[NP];
@@ -344,7 +338,7 @@ __global__ __launch_bounds__(512) void spconv_fwd_split3_kernel(const ConvParams
             const int voff = row_cur[j] >= 0 ? row_cur[j] * (NP * n_cw) + chb[j] : (int)0x80000000;   // no neighbour: zeros, no bytes moved
 #pragma unroll
             for (int q = 0; q < NP; ++q)
-                s3_dma16(n_from_a ? rsrc_a : rsrc_b, s_base + n_slot * STAGE + q * APLANE + t * 1024, voff, soff[q]);
+                lds_dma16(n_from_a ? rsrc_a : rsrc_b, s_base + n_slot * STAGE + q * APLANE + t * 1024, voff, soff[q]);
         }
     };
 #define LIDIFF_S3_BARRIER() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
