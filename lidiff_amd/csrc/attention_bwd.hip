@@ -8,9 +8,9 @@
 // sum to zero only as exactly as delta is known.
 //
 // fp16 operands.  A score gradient is a probability times a gradient and soon lies below fp16's range (2^-24), so it is multiplied by a
-// power of two before it is rounded and the sums are multiplied back, both exact: |ds| <= 2 |do_i| max_j |v_j|, and the power takes that
-// bound to 2^15.  dq: a power of each query; dk: one for all queries of a key head (a sum has one scale).  The norms' maxima come from a
-// pass of their own over do and v; values that are not finite take no part in them.
+// power of two before it is rounded and the sums are multiplied back, both exact.  Every sum (a query's dq, a key's dk) has a power of its
+// own that follows its largest score gradient so far, as a softmax's running maximum does (at_lift_to): no other row, of this scan or of
+// another, moves it.
 #include "attention.h"
 
 namespace lidiff {
@@ -31,37 +31,34 @@ struct AtBwd {
     float* part_kv;                                           // splits > 1: [splits][2][mk][heads / share][dim]
     float* part_t;                                            // [tiles][heads][buckets]
     int tiles;
-    unsigned* bound;                                          // fp16: [2][heads / share] bits of the largest |do|^2 and |v|^2 of a key head
 };
 
-// the power of two (its exponent) for score gradients bounded by 2 sqrt(g2 v2)
-__device__ __forceinline__ float at_lift(float g2, float v2) {
-    return fminf(fmaxf(floorf(14.f - 0.5f * (__builtin_amdgcn_logf(g2) + __builtin_amdgcn_logf(v2))), -100.f), 100.f);
-}
-
-__global__ void at_bound_clear_kernel(unsigned* bound, int n) {
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < n) bound[i] = 0u;
-}
-
-// largest |row|^2 of a head of src [rows][heads][dim], joined over `share` heads: a maximum of bit patterns, the same in any order
-template <typename T>
-__global__ __launch_bounds__(256) void at_bound_kernel(const T* __restrict__ src, int64_t row_stride, int64_t head_stride, int rows, int dim, int share,
-                                                      unsigned* __restrict__ bound) {
-    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    float sum = 0.f;
-    if (row < rows) {
-        const T* p = src + row * row_stride + (int64_t)blockIdx.y * head_stride;
-        for (int d = 0; d < dim; d += 8) {
-            const f32x8 v = __builtin_convertvector(at_load8(p + d), f32x8);
+// Multiplies a column's score gradients (its four lanes hold 4 N each) by the column's power of two `lift`; where the largest would leave
+// [0, 2^15] the power is lowered so that it comes to [2^10, 2^11) -- 2^4 of room for the next tiles' -- and the sums formed so far go along.
+// 2^-24 of the largest keeps all of fp16's bits, and what fp16 loses below is 2^-34 of it.  Values that are not finite make their sum so
+// and leave the power alone.
+constexpr float kLiftStart = 1152921504606846976.f;          // 2^60: within fp32 times the largest |ds| (2^41, with p's own lift 2^56), beyond 2^15 times any that matters
+template <int N, int DB>
+__device__ __forceinline__ void at_lift_to(float& lift, f32x4 (&ds)[N], f32x4 (&sums)[DB]) {
+    float top = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum += v[e] * v[e];
-        }
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(ds[b][e]));
+    if (__any(top * lift > 32768.f)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const int was = __builtin_bit_cast(int, lift) >> 23, most = 127 + 10 - ((__builtin_bit_cast(int, top) >> 23) - 127);
+        const bool lower = top * lift > 32768.f && top < INFINITY;
+        const float fade = __builtin_bit_cast(float, (lower ? most - was + 127 : 127) << 23);
+        lift *= fade;
+#pragma unroll
+        for (int b = 0; b < DB; ++b) sums[b] *= fade;
     }
-    if (!(sum < INFINITY)) sum = 0.f;
-    for (int off = kWave / 2; off > 0; off >>= 1) sum = fmaxf(sum, __shfl_xor(sum, off));
-    if (lane_id() == 0) atomicMax(bound + blockIdx.y / share, __builtin_bit_cast(unsigned, sum));
+#pragma unroll
+    for (int b = 0; b < N; ++b) ds[b] *= lift;
 }
+__device__ __forceinline__ float at_unlift(float lift) { return __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, lift)); }      // 1 / 2^n, exact
 
 // What a workgroup takes: heads at a time (the distances of a pair are the same for every head), rows of a tile.  One buffer per tile, as in
 // the forward kernel (41 157 x 5 824 x 2, bf16, dq: 1.43 against 1.69 ms).
@@ -136,7 +133,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
     const float scale2 = a.scale * kLog2e;
 
     Frag qf[QB][HG][DC], gf[QB][HG][DC];
-    float lse[QB][HG], slope[HG], unlift[QB][HG], qx[QB], qy[QB], qz[QB];
+    float lse[QB][HG], slope[HG], lift[QB][HG], qx[QB], qy[QB], qz[QB];
     bool huge[QB][HG];
     // -delta: what the products do . v start from.  (With the table's gradient it is added behind them: the matrix pipe rounds sums to one
     // side, and what is the same for every pair does not cancel in a sum over 10^8 of them -- 1.9e-5 of the gradient against 1.2e-6.)
@@ -151,7 +148,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
         const bool have = qi < t.hi;
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
-            float sum = 0.f, g2 = 0.f;
+            float sum = 0.f;
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
                 const int d = 32 * c + 8 * g;
@@ -163,10 +160,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                     if (GRAD) at_turn(gf[n][h][c], col & 1 ? 0x80008000u : 0u);
                     const float* o = a.out32 + ((int64_t)qi * a.heads + h0 + h) * a.dim + d;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        sum += (float)go[e] * o[e];
-                        if (kLifted) g2 += (float)go[e] * (float)go[e];
-                    }
+                    for (int e = 0; e < 8; ++e) sum += (float)go[e] * o[e];
                 }
             }
             sum += __shfl_xor(sum, 16);
@@ -177,15 +171,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                 a.stat[(int64_t)(h0 + h) * a.mq + qi] = lse[n][h] - AtType<T>::kLift;
                 a.stat[(int64_t)(a.heads + h0 + h) * a.mq + qi] = -sum;
             }
-            unlift[n][h] = 1.f;
-            if (kLifted) {
-                g2 += __shfl_xor(g2, 16);
-                g2 += __shfl_xor(g2, 32);
-                const int kv_heads = a.heads / a.share;
-                const float lift = at_lift(g2, __builtin_bit_cast(float, a.bound[kv_heads + (h0 + h) / a.share]));
-                lse[n][h] -= lift;                             // p, and with it ds, carries the power of two
-                unlift[n][h] = __builtin_amdgcn_exp2f(-lift);
-            }
+            lift[n][h] = kLiftStart;
             huge[n][h] = at_huge(lse[n][h]);
         }
         qx[n] = qy[n] = qz[n] = 0.f;
@@ -320,8 +306,9 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
                             s[n][b] *= GRAD ? dp[n][b] * sign + less[n][h] : dp[n][b];
-                            if (GRAD) grads[n][b][h] = kLifted ? s[n][b] * unlift[n][h] : s[n][b];
+                            if (GRAD) grads[n][b][h] = s[n][b];
                         }
+                        if constexpr (kLifted) at_lift_to(lift[n][h], s[n], dq[n][h]);
                         at_pack(p[n], at_join(s[n][0], s[n][1]));
                     }
 #pragma unroll
@@ -353,7 +340,8 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
         for (int h = 0; h < HG; ++h)
 #pragma unroll
             for (int b = 0; b < DB; ++b)
-                if (16 * b + 4 * g < a.dim) at_store4((T*)a.dq + ((int64_t)qi * a.heads + h0 + h) * a.dim + 16 * b + 4 * g, dq[n][h][b] * (a.scale * unlift[n][h]));
+                if (16 * b + 4 * g < a.dim)
+                    at_store4((T*)a.dq + ((int64_t)qi * a.heads + h0 + h) * a.dim + 16 * b + 4 * g, dq[n][h][b] * (kLifted ? a.scale * at_unlift(lift[n][h]) : a.scale));
     }
     if (GRAD) {
         gather();
@@ -398,7 +386,7 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
     const float scale2 = a.scale * kLog2e;
 
     Frag kf[SLOTS][DC], vf[SLOTS][DC];
-    float ds_lift[SLOTS], dk_unlift[SLOTS];
+    float lift[SLOTS];
     f32x4 dk[SLOTS][DB], dv[SLOTS][DB];
 #pragma unroll
     for (int h = 0; h < SLOTS; ++h) {
@@ -411,12 +399,7 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
                 vf[h][c] = at_load8((const T*)a.v + (int64_t)ki * a.v_row + (int64_t)(kv0 + h) * a.v_head + d);
             }
         }
-        ds_lift[h] = dk_unlift[h] = 1.f;
-        if (kLifted) {
-            const float lift = at_lift(__builtin_bit_cast(float, a.bound[kv0 + h]), __builtin_bit_cast(float, a.bound[kv_heads + kv0 + h]));
-            ds_lift[h] = __builtin_amdgcn_exp2f(lift - AtType<T>::kLift);             // (p carries kLift already)
-            dk_unlift[h] = __builtin_amdgcn_exp2f(-lift);
-        }
+        lift[h] = kLiftStart;
 #pragma unroll
         for (int b = 0; b < DB; ++b) dk[h][b] = dv[h][b] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -519,10 +502,8 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
                             }
                         }
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            dp[b] *= s[b];
-                            if (kLifted) dp[b] *= ds_lift[slot];
-                        }
+                        for (int b = 0; b < 2; ++b) dp[b] *= s[b];
+                        if constexpr (kLifted) at_lift_to(lift[slot], dp, dk[slot]);
                         Frag p, ds;
                         at_pack(p, at_join(s[0], s[1]));
                         at_pack(ds, at_join(dp[0], dp[1]));
@@ -542,20 +523,23 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
     }
     if (!have) return;
 #pragma unroll
-    for (int h = 0; h < SLOTS; ++h)
+    for (int h = 0; h < SLOTS; ++h) {
+        // (p, and with it ds, carries kLift already)
+        const float dk_unlift = kLifted ? at_unlift(lift[h]) * kUnlift : 1.f;
 #pragma unroll
         for (int b = 0; b < DB; ++b) {
             if (16 * b + 4 * g >= a.dim) continue;
             const int64_t at = ((int64_t)ki * kv_heads + kv0 + h) * a.dim + 16 * b + 4 * g;
             if (a.splits > 1) {
                 const int64_t plane = (int64_t)a.mk * kv_heads * a.dim;
-                at_store4(a.part_kv + (2 * split) * plane + at, dk[h][b] * dk_unlift[h]);
+                at_store4(a.part_kv + (2 * split) * plane + at, dk[h][b] * dk_unlift);
                 at_store4(a.part_kv + (2 * split + 1) * plane + at, dv[h][b] * kUnlift);
             } else {
-                at_store4((T*)a.dk + at, dk[h][b] * (a.scale * dk_unlift[h]));
+                at_store4((T*)a.dk + at, dk[h][b] * (a.scale * dk_unlift));
                 at_store4((T*)a.dv + at, dv[h][b] * kUnlift);
             }
         }
+    }
 }
 
 template <typename T>
@@ -660,7 +644,7 @@ inline int at_grad_blocks(int dtype, int dim) {
                       : (dim <= 32 ? AtBwdPlan<__bf16, 32>::kGradQB : dim <= 64 ? AtBwdPlan<__bf16, 64>::kGradQB : AtBwdPlan<__bf16, 128>::kGradQB);
 }
 
-struct AtBwdLayout { int splits; int64_t bound, q, k, v, go, table, kv, bytes; };      // workspace; the row statistics come first
+struct AtBwdLayout { int splits; int64_t q, k, v, go, table, kv, bytes; };      // workspace; the row statistics come first
 
 template <typename T>
 static AtBwdLayout at_bwd_layout(int64_t mq, int64_t mk, const void* seg, int64_t nseg, int heads, int kv_heads, int dim, int mode, int buckets, bool table_grad) {
@@ -669,8 +653,7 @@ static AtBwdLayout at_bwd_layout(int64_t mq, int64_t mk, const void* seg, int64_
     l.splits = dim <= 32 ? at_bwd_splits<T, 32>(mq, mk, nseg, heads, kv_heads, mode) : dim <= 64 ? at_bwd_splits<T, 64>(mq, mk, nseg, heads, kv_heads, mode)
                                                                                                : at_bwd_splits<T, 128>(mq, mk, nseg, heads, kv_heads, mode);
     const int64_t pq = sizeof(T) == 4 ? up(3 * at_plane_bytes(mq, heads, dim)) : 0, pk = sizeof(T) == 4 ? up(3 * at_plane_bytes(mk, kv_heads, dim)) : 0;
-    l.bound = up(2 * mq * heads * (int64_t)sizeof(float));
-    l.q = l.bound + up(2 * kv_heads * (int64_t)sizeof(float));
+    l.q = up(2 * mq * heads * (int64_t)sizeof(float));
     l.go = l.q + pq;
     l.k = l.go + pq;
     l.v = l.k + pk;
@@ -683,13 +666,6 @@ static AtBwdLayout at_bwd_layout(int64_t mq, int64_t mk, const void* seg, int64_
 template <typename T>
 static hipError_t at_bwd_run(AtBwd a, const AtBwdLayout& l, int mode, char* ws, hipStream_t st) {
     const int kv_heads = a.heads / a.share;
-    if constexpr (AtType<T>::kLift != 0) {
-        at_bound_clear_kernel<<<(unsigned)ceil_div(2 * kv_heads, 256), 256, 0, st>>>(a.bound, 2 * kv_heads);
-        at_bound_kernel<T><<<dim3((unsigned)ceil_div(a.mq, 256), (unsigned)a.heads), 256, 0, st>>>((const T*)a.go, a.go_row, a.go_head, a.mq, a.dim, a.share, a.bound);
-        if (a.mk > 0)
-            at_bound_kernel<T><<<dim3((unsigned)ceil_div(a.mk, 256), (unsigned)kv_heads), 256, 0, st>>>((const T*)a.v, a.v_row, a.v_head, a.mk, a.dim, 1,
-                                                                                                    a.bound + kv_heads);
-    }
     a.ks = at_stream<T>(a.k, a.k_row, a.k_head, a.mk, kv_heads, a.dim, ws + l.k, st);
     a.vs = at_stream<T>(a.v, a.v_row, a.v_head, a.mk, kv_heads, a.dim, ws + l.v, st);
     if (a.dk) {
@@ -748,7 +724,6 @@ extern "C" int lidiff_segment_attention_bwd(const void* q, const void* k, const 
     const AtBwdLayout l = at_bwd_layout_of(dtype, mq, mk, seg_q, n_segments, heads, kv_heads, dim, bias_mode, buckets, dtable != nullptr);
     char* ws = (char*)workspace;
     a.stat = (float*)ws;
-    a.bound = (unsigned*)(ws + l.bound);
     a.part_t = dtable ? (float*)(ws + l.table) : nullptr;
     a.part_kv = (float*)(ws + l.kv);
     a.tiles = (int)seg_tiles_bound(mq, 64 * at_grad_blocks(dtype, dim), seg_q, n_segments);

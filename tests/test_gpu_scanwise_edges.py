@@ -1,0 +1,76 @@
+"""The scan-wise operators at the edges: large finite values beside a scan, scores and table entries far out, means far from zero (MI355X, against
+64-bit forms; helpers and bounds of scanwise_ref)."""
+import math
+
+import pytest
+import torch
+
+from scanwise_ref import U32, assert_within, attention_ref, group_norm_ref, ranges
+from test_gpu_scanwise import BF16, F16, F32, TINY, edges_of, generator, rand, voxel_rows
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(device):
+    from lidiff_amd import ops
+    return ops
+
+
+def attend(ops, q, k, v, go, *segments, bias=None, **kw):
+    """Output and gradients of one call."""
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v) + (() if bias is None else (bias,))]
+    out = ops.segment_attention(*leaves[:3], *segments, **kw, **({} if bias is None else {"bias": leaves[3]}))
+    return (out.detach(),) + torch.autograd.grad(out, leaves, go)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("share", [1, 2])
+def test_large_finite_values_beside_a_scan_change_no_bit_of_it(ops, dtype, share):
+    """Another scan's rows and rows of no scan at 100 ... 60 000, in the values, the output's gradient, queries and keys."""
+    gen = generator(31)
+    seg, m = ranges([70, 50, 40], [3, 0, 2]).cuda(), 170
+    q, go = rand(gen, m, 4, 32, dtype=dtype), rand(gen, m, 4, 32, dtype=dtype)
+    k, v = rand(gen, m, 4 // share, 32, dtype=dtype), rand(gen, m, 4 // share, 32, dtype=dtype)
+    kw = dict(coords_q=voxel_rows(gen, m), coords_k=voxel_rows(gen, m), bias=rand(gen, 8, 4), edges=edges_of(ops, 8))
+    clean = attend(ops, q, k, v, go, seg, seg, **kw)
+    for big in (1e2, 1e4, 6e4):
+        q2, k2, v2, go2 = (t.clone() for t in (q, k, v, go))
+        for t in (v2, go2, q2, k2):
+            t[73:123], t[:3], t[123:125], t[165:] = big, big, big, big
+        for name, got, want in zip(("out", "dq", "dk", "dv"), attend(ops, q2, k2, v2, go2, seg, seg, **kw), clean):
+            assert torch.equal(got[3:73], want[3:73]) and torch.equal(got[125:165], want[125:165]), (name, big)
+
+
+@pytest.mark.parametrize("bias", [None, 8])
+def test_fp16_score_gradients_of_every_size(ops, bias):
+    """Gradients of rows that differ by 10^8 in size, and masked keys with values near fp16's end: each key's and query's sum keeps the bits
+    its own terms have."""
+    gen = generator(32)
+    nq, nk, h, d = 300, 400, 2, 32
+    q, k, v = rand(gen, nq, h, d, dtype=F16), rand(gen, nk, h, d, dtype=F16), rand(gen, nk, h, d, dtype=F16)
+    go = (rand(gen, nq, h, d) * 10.0 ** torch.randint(-4, 5, (nq, 1, 1), generator=gen, device="cuda")).clamp(-6e4, 6e4).to(F16)
+    kw = {}
+    if bias:
+        ck, cq = voxel_rows(gen, nk), voxel_rows(gen, nq)
+        ck[::7, 1] = 30000                                   # every seventh key is far away, in the last bucket: masked, its values huge
+        v[::7] = 6e4
+        table = rand(gen, bias, h)
+        table[-1] = -math.inf
+        cq[:, 1:] = cq[:, 1:].clamp(-200, 200)
+        kw = dict(coords_q=cq, coords_k=ck, bias=table, edges=edges_of(ops, bias))
+    got = attend(ops, q, k, v, go, **kw)
+    # the 64-bit form without the masked keys (its bounds do not hold infinities); no other pair is in the last bucket
+    seen = torch.arange(nk, device="cuda") % 7 != 0 if bias else torch.ones(nk, dtype=torch.bool, device="cuda")
+    ref = {}
+    if bias:
+        ref = dict(cq=cq, ck=ck[seen], bias=table.nan_to_num(neginf=0.0), edges=kw["edges"])
+        assert (cq[:, None, 1:] - ck[None, seen, 1:]).long().square().sum(-1).max() < kw["edges"][-1]
+    val, bnd = attention_ref(q, k[seen], v[seen], go=go, **ref)
+    for name, g in zip(("out", "dq", "dk", "dv"), (got[0], got[1], got[2][seen], got[3][seen])):
+        assert_within(g, val[name], bnd[name], TINY[F16], f"{name} {bias}")
+    if bias:
+        assert (got[2][::7] == 0).all() and (got[3][::7] == 0).all()
+    # small gradients alone: below fp16's normal range before they are lifted
+    tiny = attend(ops, q, k, v, (rand(gen, nq, h, d) * 1e-3).to(F16), **kw)
+    assert tiny[1].abs().max() > 0 and tiny[2].abs().max() > 0
