@@ -175,8 +175,8 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
             huge[n][h] = at_huge(lse[n][h]);
         }
         qx[n] = qy[n] = qz[n] = 0.f;
-        if (BIAS != kNone && have) {
-            const int4 c = a.cq[qi];
+        if (BIAS != kNone) {                                   // (a place without a query stands where the last one does: it meets no bucket that
+            const int4 c = a.cq[min(qi, t.hi - 1)];            // no query meets, whose entry may be infinite or NaN)
             qx[n] = (float)c.y; qy[n] = (float)c.z; qz[n] = (float)c.w;
         }
     }
@@ -293,6 +293,8 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                         for (int b = 0; b < 2; ++b)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) s[n][b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[n][b][e], factor, -lse[n][h]));
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) s[n][b] *= GRAD ? dp[n][b] * sign + less[n][h] : dp[n][b];
                         if (left < ROWS) {
                             const int end = at_here(left);
 #pragma unroll
@@ -304,10 +306,8 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                             }
                         }
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            s[n][b] *= GRAD ? dp[n][b] * sign + less[n][h] : dp[n][b];
+                        for (int b = 0; b < 2; ++b)
                             if (GRAD) grads[n][b][h] = s[n][b];
-                        }
                         if constexpr (kLifted) at_lift_to(lift[n][h], s[n], dq[n][h]);
                         at_pack(p[n], at_join(s[n][0], s[n][1]));
                     }

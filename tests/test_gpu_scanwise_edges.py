@@ -74,3 +74,22 @@ def test_fp16_score_gradients_of_every_size(ops, bias):
     # small gradients alone: below fp16's normal range before they are lifted
     tiny = attend(ops, q, k, v, (rand(gen, nq, h, d) * 1e-3).to(F16), **kw)
     assert tiny[1].abs().max() > 0 and tiny[2].abs().max() > 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("entry", [math.inf, math.nan, -math.inf])
+def test_a_bucket_that_no_pair_meets_has_no_gradient(ops, dtype, entry):
+    """Whatever its entry holds: the places of a workgroup's tile without a query, or without a key, meet no bucket of their own."""
+    gen = generator(33)
+    for heads in (1, 2, 4):
+        for nq, nk in ((5, 40), (70, 33), (128, 64)):
+            q, k, v, go = (rand(gen, n, heads, 32, dtype=dtype) for n in (nq, nk, nk, nq))
+            cq, ck = (torch.zeros(n, 4, dtype=torch.int32, device="cuda") for n in (nq, nk))
+            cq[:, 1], ck[:, 1] = 1000, 1000 + torch.arange(nk, device="cuda")          # (far from the origin, near each other)
+            table = rand(gen, 3, heads)
+            table[2] = entry
+            got = attend(ops, q, k, v, go, bias=table, edges=(400, 10000), coords_q=cq, coords_k=ck)
+            val, bnd = attention_ref(q, k, v, go=go, bias=table.nan_to_num(0.0, 0.0, 0.0), edges=(400, 10000), cq=cq, ck=ck)
+            assert (got[4][2] == 0).all()
+            for name, g in zip(("out", "dq", "dk", "dv", "dt"), got):
+                assert_within(g, val[name], bnd[name], 1e-30 if name == "dt" else TINY[dtype], f"{name} {heads} {nq}")
