@@ -118,11 +118,13 @@ def load() -> C.CDLL:
                 f"lidiff_amd HIP extension missing: {LIB_PATH}. Build it with "
                 "`python -m lidiff_amd.csrc.build` (needs hipcc); there is no CPU fallback.")
         lib = C.CDLL(LIB_PATH)
+        missing = [name for name in SIGNATURES if not hasattr(lib, name)]
+        if missing or lib.lidiff_abi_version() != ABI_VERSION:
+            raise RuntimeError(f"lidiff_amd ABI version mismatch: {LIB_PATH} was built from other sources"
+                               + (f" (it lacks {', '.join(missing)})" if missing else "") + "; run `python -m lidiff_amd.csrc.build`")
         for name, (res, args) in SIGNATURES.items():
-            fn = getattr(lib, name)          # AttributeError if the symbol is not exported
+            fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
-        if lib.lidiff_abi_version() != ABI_VERSION:
-            raise RuntimeError("lidiff_amd ABI version mismatch")
         _lib = lib
     return _lib
 
