@@ -511,6 +511,9 @@ int64_t lidiff_nn_dist_grid_workspace_bytes(int64_t n, int64_t m, int32_t elem_b
 int lidiff_nn_dist_grid(const void* a, int64_t n, const void* b, int64_t m, int32_t elem_bytes, double cell, void* d2, int64_t* idx,
                         void* workspace, void* stream);
 
+/* The layouts of what the scan-wise operators hand from a forward call to its backward call (stats, lse): 2. */
+int32_t lidiff_scanwise_version(void);
+
 /* ---- scan-wise operators: rows of the same scan share statistics / attend to each other -------------------------------------------
  * A batch of scans is ONE row matrix; `segments` (device int32 [n_segments][2]) holds the first row and the row behind the last one of
  * every scan, ascending and disjoint; NULL with n_segments = 1: all rows.  dtype: 0 fp32, 1 bf16, 2 fp16.  Rows of no segment come out
@@ -542,8 +545,9 @@ int lidiff_group_norm_bwd(const void* x, const void* dy, int64_t rows, int32_t c
  * bias_mode: 0 none; 1: -slopes[head] * |c_i - c_j|; 2: table[bucket][head], bucket = edges <= |c_i - c_j|^2 (table fp32
  * [buckets][heads], buckets <= 48; cells: the look-up table of the edges that ops.bucket_cells builds).  coords_q / coords_k: int32
  * [rows][4] = (batch, x, y, z); the batch column is not read.
- * out_f32 (unrounded copy) and lse ([heads][mq]: log2 of the sum of exponentials; +inf without keys) are kept for the backward pass;
- * either may be NULL.  exact: with a table and 16-bit operands, out_f32 from probabilities of twice the bits (for dtable).  workspace:
+ * out_f32 (unrounded copy) and lse ([2][heads][mq]: log2 of the sum of exponentials as two numbers whose sum it is; +inf and 0 without
+ * keys) are kept for the backward pass; either may be NULL.  exact: with a table and 16-bit operands, out_f32 from probabilities in
+ * pieces (bf16: 24 bits in three, fp16: 22 in two; for dtable).  workspace:
  * may be NULL where workspace_bytes says 0. */
 int64_t lidiff_segment_attention_workspace_bytes(int64_t mq, int64_t mk, int64_t n_segments, int32_t heads, int32_t kv_heads,
                                                  int32_t dim, int32_t dtype, int32_t bias_mode);

@@ -93,6 +93,7 @@ SIGNATURES = {
     "lidiff_nn_dist": (_i32, [_p, _i64, _p, _i64, _i32, _p, _p, _p, _p]),
     "lidiff_nn_dist_grid_workspace_bytes": (_i64, [_i64, _i64, _i32]),
     "lidiff_nn_dist_grid": (_i32, [_p, _i64, _p, _i64, _i32, C.c_double, _p, _p, _p, _p]),
+    "lidiff_scanwise_version": (_i32, []),
     "lidiff_batch_segments": (_i32, [_p, _i64, _p, _i32, _i32, _p, _p, _p]),
     "lidiff_group_norm_workspace_bytes": (_i64, [_i32, _i64]),
     "lidiff_group_norm": (_i32, [_p, _i64, _i32, _i32, _i32, _p, _i64, _p, _p, C.c_float, _i32, _p, _p, _p, _p]),
@@ -106,6 +107,7 @@ SIGNATURES = {
 }
 
 ABI_VERSION = 28
+SCANWISE_VERSION = 2          # layouts of what the scan-wise operators' forward calls hand to their backward calls
 _lib = None
 
 
@@ -119,7 +121,7 @@ def load() -> C.CDLL:
                 "`python -m lidiff_amd.csrc.build` (needs hipcc); there is no CPU fallback.")
         lib = C.CDLL(LIB_PATH)
         missing = [name for name in SIGNATURES if not hasattr(lib, name)]
-        if missing or lib.lidiff_abi_version() != ABI_VERSION:
+        if missing or lib.lidiff_abi_version() != ABI_VERSION or lib.lidiff_scanwise_version() != SCANWISE_VERSION:
             raise RuntimeError(f"lidiff_amd ABI version mismatch: {LIB_PATH} was built from other sources"
                                + (f" (it lacks {', '.join(missing)})" if missing else "") + "; run `python -m lidiff_amd.csrc.build`")
         for name, (res, args) in SIGNATURES.items():

@@ -124,24 +124,27 @@ __device__ __forceinline__ int at_here(int v) {
 }
 __device__ __forceinline__ void at_here(f32x4& v) { asm volatile("" : "+v"(v)); }
 
-// A probability is exp2(s scale2 - base) with one rounding (fma).  Where the base is so large that the rounding of base alone is a factor
-// (|base| > 2^20: differences of such scores are whole powers of two anyway) the product is rounded first, so that the scores the base was
-// formed from give 1.  Returns the factor that is left for the fma.
+// A probability is exp2(s scale2 - base) with one rounding (fma).  Where the base is so large (|base| > 2^20, where fp32 steps by 1/8) that
+// the rounding of the base alone is a factor, the product is rounded first, so that the scores the base was formed from give 1.
 constexpr float kHuge = 1048576.f;
-template <int N>
-__device__ __forceinline__ float at_scale(f32x4 (&s)[N], float scale2, bool huge) {
-    if (!huge) return scale2;
-    const float f = __builtin_bit_cast(float, at_here(__builtin_bit_cast(int, scale2)));
-#pragma unroll
-    for (int b = 0; b < N; ++b)
-    {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[b][e] = __fmul_rn(s[b][e], f);
-        at_here(s[b]);
-    }
-    return 1.f;
-}
 __device__ __forceinline__ bool at_huge(float base) { return __any(fabsf(base) > kHuge && fabsf(base) < INFINITY); }
+__device__ __forceinline__ float at_exponent(float s, float scale2, float base) {
+    float product = __fmul_rn(s, scale2);
+    asm volatile("" : "+v"(product));                          // (no fma of it and the subtraction)
+    return fabsf(base) > kHuge ? product - base : __fmaf_rn(s, scale2, -base);
+}
+
+// The log2 of a sum of exponentials is base + log2(sum), kept as two numbers whose sum is exact: one fp32 number steps by 2^-23 |base|, and a
+// probability rebuilt from it is off by that factor (13 equal scores of 2^14: 5e-4; of 2^22: 15 %).  The backward pass's exponent is
+// s scale2 - lse.  Up to |lse| = 2^6 the first number alone does (2^-19 of rounding: 1.3e-6 of the row's probabilities, alike for all of
+// them); beyond, in a wave that has such a row, the product less the first number is small, and the second one is subtracted from that.
+constexpr float kFar = 64.f;
+__device__ __forceinline__ bool at_far(float lse) { return __any(fabsf(lse) > kFar && fabsf(lse) < INFINITY); }
+__device__ __forceinline__ float at_two_sum(float a, float b, float& rest) {
+    const float sum = a + b, part = sum - a;
+    rest = fabsf(sum) < INFINITY ? (a - (sum - part)) + (b - part) : 0.f;
+    return sum;
+}
 
 // four consecutive outputs
 template <typename T>

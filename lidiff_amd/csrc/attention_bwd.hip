@@ -24,8 +24,8 @@ struct AtBwd {
     int nseg, mq, mk, heads, share, dim;
     float scale;
     AtBias bias;
-    const float *out32, *lse;                                 // [mq][heads][dim], [heads][mq]
-    float* stat;                                              // [2][heads][mq]: lse (less kLift) and -delta, for the dk / dv kernel
+    const float *out32, *lse;                                 // [mq][heads][dim], [2][heads][mq]
+    float* stat;                                              // [3][heads][mq]: lse (less kLift), -delta, lse's second number, for the dk / dv kernel
     void *dq, *dk, *dv;                                       // contiguous
     int splits;                                               // dk / dv: the queries of a scan are shared out over `splits` workgroups
     float* part_kv;                                           // splits > 1: [splits][2][mk][heads / share][dim]
@@ -69,7 +69,8 @@ template <typename T, int DP> struct AtBwdPlan {
     static constexpr int kGradRows = 32;
     static constexpr int kGradQB = sizeof(T) == 2 && DP == 32 ? 2 : 1;      // blocks of 16 queries a wave (2.58 against 2.81 ms; fp32: 1.14 against 0.97)
     static constexpr int kRows = 64, kQB = 1;                         // (two blocks: 1.33 against 1.26 ms)
-    static constexpr int kKeyWaves = sizeof(T) == 2 && DP == 32 ? 4 : at_waves(sizeof(T), DP);
+    // dk / dv, 128 wide: three waves with four registers spilled against two without, 949 : 995 us at 20 000 x 5 824, bf16, slopes, 2 heads, training
+    static constexpr int kKeyWaves = sizeof(T) == 2 ? (DP == 32 ? 4 : DP == 128 ? 3 : 2) : at_waves(sizeof(T), DP);
 };
 
 inline int at_bwd_heads(int most, int heads, int share, int mode) {      // whole groups of one key head, or key heads of their own
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
 
     Frag qf[QB][HG][DC], gf[QB][HG][DC];
     float lse[QB][HG], slope[HG], lift[QB][HG], qx[QB], qy[QB], qz[QB];
-    bool huge[QB][HG];
+    bool far[QB][HG];
     // -delta: what the products do . v start from.  (With the table's gradient it is added behind them: the matrix pipe rounds sums to one
     // side, and what is the same for every pair does not cancel in a sum over 10^8 of them -- 1.9e-5 of the gradient against 1.2e-6.)
     float less[QB][HG];
@@ -168,11 +169,13 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
             less[n][h] = -sum;
             lse[n][h] = have ? a.lse[(int64_t)(h0 + h) * a.mq + qi] : INFINITY;
             if (have && g == 0) {
-                a.stat[(int64_t)(h0 + h) * a.mq + qi] = lse[n][h] - AtType<T>::kLift;
+                float off;                                     // (the lift may not move lse's last bits either)
+                a.stat[(int64_t)(h0 + h) * a.mq + qi] = at_two_sum(lse[n][h], -(float)AtType<T>::kLift, off);
                 a.stat[(int64_t)(a.heads + h0 + h) * a.mq + qi] = -sum;
+                a.stat[(int64_t)(2 * a.heads + h0 + h) * a.mq + qi] = a.lse[(int64_t)(a.heads + h0 + h) * a.mq + qi] + off;
             }
             lift[n][h] = kLiftStart;
-            huge[n][h] = at_huge(lse[n][h]);
+            far[n][h] = at_far(lse[n][h]);
         }
         qx[n] = qy[n] = qz[n] = 0.f;
         if (BIAS != kNone) {                                   // (a place without a query stands where the last one does: it meets no bucket that
@@ -288,11 +291,23 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                     Frag p[QB];
 #pragma unroll
                     for (int n = 0; n < QB; ++n) {
-                        const float factor = at_scale(s[n], scale2, huge[n][h]);
+                        float factor = scale2, minus = lse[n][h];
+                        if (far[n][h]) {                       // (lse's second number from memory: the branch is rare, registers are not spent on it)
+                            const float f = __builtin_bit_cast(float, at_here(__builtin_bit_cast(int, scale2)));
+                            const float rest = a.lse[(int64_t)(a.heads + h0 + h) * a.mq + min(at_here(q0 + 16 * n + col), t.hi - 1)];
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) s[n][b][e] = at_exponent(s[n][b][e], f, lse[n][h]) - rest;
+                                at_here(s[n][b]);
+                            }
+                            factor = 1.f;
+                            minus = 0.f;
+                        }
 #pragma unroll
                         for (int b = 0; b < 2; ++b)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) s[n][b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[n][b][e], factor, -lse[n][h]));
+                            for (int e = 0; e < 4; ++e) s[n][b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[n][b][e], factor, -minus));
 #pragma unroll
                         for (int b = 0; b < 2; ++b) s[n][b] *= GRAD ? dp[n][b] * sign + less[n][h] : dp[n][b];
                         if (left < ROWS) {
@@ -458,9 +473,9 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
                 coords(tile + 2);
             }
             if (k0 < t.hi) {
-                bool huge[HG];
+                bool far[HG];
 #pragma unroll
-                for (int h = 0; h < HG; ++h) huge[h] = at_huge(st[h * ROWS + lane]);
+                for (int h = 0; h < HG; ++h) far[h] = at_far(st[h * ROWS + lane]);
                 const float* const ct = cs + (tile & 1) * 3 * ROWS;
                 const int left = q_hi - (q_lo + tile * ROWS);
 #pragma unroll
@@ -484,11 +499,15 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
                                 at_mma(s[b], Tile::frag(qs, place, h, 2 * j + b, c), kf[slot][c]);
                                 at_mma(dp[b], Tile::frag(gs, place, h, 2 * j + b, c), vf[slot][c]);
                             }
-                            f32x4 (&one)[1] = reinterpret_cast<f32x4 (&)[1]>(s[b]);
-                            const float factor = at_scale(one, scale2, huge[h]);
+                            if (far[h]) {                      // (lse's second numbers from memory, as above)
+                                const float f = __builtin_bit_cast(float, at_here(__builtin_bit_cast(int, scale2)));
+                                const float* const rest = a.stat + (int64_t)(2 * a.heads + h0 + h) * a.mq;
+                                const int row = at_here(q_lo + tile * ROWS + 32 * j + 16 * b + 4 * g);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                s[b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][e], factor, -lse[e]));
+                                for (int e = 0; e < 4; ++e) s[b][e] = __builtin_amdgcn_exp2f(at_exponent(s[b][e], f, lse[e]) - rest[min(row + e, q_hi - 1)]);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) s[b][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][e], scale2, -lse[e]));
                             }
                         }
                         if (left < ROWS) {
@@ -653,7 +672,7 @@ static AtBwdLayout at_bwd_layout(int64_t mq, int64_t mk, const void* seg, int64_
     l.splits = dim <= 32 ? at_bwd_splits<T, 32>(mq, mk, nseg, heads, kv_heads, mode) : dim <= 64 ? at_bwd_splits<T, 64>(mq, mk, nseg, heads, kv_heads, mode)
                                                                                                : at_bwd_splits<T, 128>(mq, mk, nseg, heads, kv_heads, mode);
     const int64_t pq = sizeof(T) == 4 ? up(3 * at_plane_bytes(mq, heads, dim)) : 0, pk = sizeof(T) == 4 ? up(3 * at_plane_bytes(mk, kv_heads, dim)) : 0;
-    l.q = up(2 * mq * heads * (int64_t)sizeof(float));
+    l.q = up(3 * mq * heads * (int64_t)sizeof(float));
     l.go = l.q + pq;
     l.k = l.go + pq;
     l.v = l.k + pk;

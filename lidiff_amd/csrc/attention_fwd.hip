@@ -22,9 +22,17 @@ struct AtFwd {
     void* out;                                                // [mq][heads][dim]
     float* out32;                                             // the same unrounded (for the backward pass), or null
     int exact;                                                // probabilities in pieces: out32 is wanted to fp32 precision
-    float* lse;                                               // [heads][mq]: log2 of the sum of exponentials, +inf for a row without keys; or null
+    float* lse;                                               // [2][heads][mq]: log2 of the sum of exponentials in two numbers, +inf and 0 for a row without keys; or null
     float *part_o, *part_ml;                                  // splits > 1: [splits][mq][heads][dim], [splits][2][heads][mq]
 };
+
+__device__ __forceinline__ void at_put_lse(const AtFwd& a, int head, int qi, float base, float sum, float lift) {
+    float rest;
+    const float lse = at_two_sum(base, log2f(sum) - lift, rest);
+    const bool none = sum == 0.f;
+    a.lse[(int64_t)head * a.mq + qi] = none ? INFINITY : lse;
+    a.lse[(int64_t)(a.heads + head) * a.mq + qi] = none ? 0.f : rest;
+}
 
 // What a workgroup takes: QB x 16 queries a wave, HG heads, tiles of 64 keys.
 // HG: the distances of a (query, key) pair are the same for every head, so a wave takes as many heads as its registers hold.
@@ -209,8 +217,18 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
 #pragma unroll
                         for (int b = 0; b < DB; ++b) o[n][h][b] *= fade;
                     }
-                    const float down = base[n][h] == -INFINITY ? 0.f : kLift - base[n][h];
-                    const float factor = at_scale(s[n], scale2, huge[n][h]);
+                    float down = base[n][h] == -INFINITY ? 0.f : kLift - base[n][h], factor = scale2;
+                    if (huge[n][h]) {                          // (the lift would be lost beside such a base as well)
+                        const float f = __builtin_bit_cast(float, at_here(__builtin_bit_cast(int, scale2))), from = base[n][h] == -INFINITY ? 0.f : base[n][h];
+#pragma unroll
+                        for (int b = 0; b < KB; ++b) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[n][b][e] = at_exponent(s[n][b][e], f, from);
+                            at_here(s[n][b]);
+                        }
+                        factor = 1.f;
+                        down = kLift;
+                    }
 #pragma unroll
                     for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -283,7 +301,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
                 continue;
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            if (a.lse && g == 0) a.lse[(int64_t)head * a.mq + qi] = sum == 0.f ? INFINITY : base[n][h] - kLift + log2f(sum);
+            if (a.lse && g == 0) at_put_lse(a, head, qi, base[n][h], sum, kLift);
 #pragma unroll
             for (int b = 0; b < DB; ++b) {
                 if (16 * b + 4 * g >= a.dim) continue;
@@ -322,7 +340,7 @@ __global__ __launch_bounds__(256) void at_join_kernel(const AtFwd a, int width, 
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off);
     }
-    if (a.lse && d == 0 && first == 0) a.lse[(int64_t)head * a.mq + qi] = sum == 0.f ? INFINITY : m + log2f(sum);
+    if (a.lse && d == 0 && first == 0) at_put_lse(a, head, qi, m, sum, 0.f);
     if (first != 0 || d >= a.dim) return;
     const f32x4 r = o * (sum == 0.f ? 0.f : 1.f / sum);
     const int64_t at = ((int64_t)qi * a.heads + head) * a.dim + d;

@@ -343,6 +343,8 @@ static const char* gn_check(int64_t rows, int c, int groups, int dtype, int64_t 
 
 using namespace lidiff;
 
+extern "C" int32_t lidiff_scanwise_version(void) { return 2; }
+
 extern "C" int64_t lidiff_group_norm_workspace_bytes(int32_t c, int64_t n_segments) {
     const int64_t slabs = n_segments > kGnSlabs ? n_segments : kGnSlabs;               // of all scans together (gn_slabs)
     return (slabs + n_segments) * 2 * c * (int64_t)sizeof(double);

@@ -2216,7 +2216,7 @@ class _SegmentAttention(torch.autograd.Function):
         out = torch.empty((mq, heads, dim), dtype=q.dtype, device=dev)
         # the backward pass needs the output as it was before its rounding (the rows of the score gradient sum to zero through it)
         out32 = None if not grads else out if q.dtype == torch.float32 else torch.empty((mq, heads, dim), dtype=torch.float32, device=dev)
-        lse = torch.empty((heads, mq), dtype=torch.float32, device=dev) if grads else None
+        lse = torch.empty((2, heads, mq), dtype=torch.float32, device=dev) if grads else None
         if mq:
             nbytes = _lib.load().lidiff_segment_attention_workspace_bytes(mq, mk, n_seg, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], mode)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
@@ -2269,7 +2269,7 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seg_q: 
       bias [buckets, H]     a learned table: bias[b, h], b = number of `edges` (ascending whole squared distances, one less than
                             buckets: distance_edges) that |c_i - c_j|^2 reaches
                             (an entry of -inf masks its bucket; finite entries beyond +-2^14 log 2 count as that)
-    Gradients for q, k, v and bias; deterministic.  The backward pass keeps q, k, v, an fp32 copy of the output and one number per
+    Gradients for q, k, v and bias; deterministic.  The backward pass keeps q, k, v, an fp32 copy of the output and two numbers per
     query and head -- never the scores.  A first call with new `edges` copies a small table to the device: make one before capturing a
     graph."""
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:

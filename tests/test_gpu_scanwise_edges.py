@@ -93,3 +93,31 @@ def test_a_bucket_that_no_pair_meets_has_no_gradient(ops, dtype, entry):
             assert (got[4][2] == 0).all()
             for name, g in zip(("out", "dq", "dk", "dv", "dt"), got):
                 assert_within(g, val[name], bnd[name], 1e-30 if name == "dt" else TINY[dtype], f"{name} {heads} {nq}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("power", [5, 10, 14, 18, 20, 22, 23, 24, 28])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_gradients_of_equal_scores_far_from_zero(ops, dtype, power, sign):
+    """Keys with one and the same score of +-2^power (in units of log 2): the rebuilt probabilities are 1 / keys whatever the score is.
+
+    The 64-bit form takes the scores 2^-power times as large: the same softmax, and its bounds then count the roundings of everything but the
+    (equal) scores; dq and dk carry the scale as a factor.  All factors are powers of two."""
+    gen = generator(34)
+    for nk, heads, table in ((13, 2, False), (13, 2, True), (1300, 4, False), (1300, 1, True)):
+        nq, d = 20, 32
+        q, k = rand(gen, nq, heads, d, dtype=dtype), torch.zeros(nk, heads, d, dtype=dtype, device="cuda")
+        q[..., 0], k[..., 0] = 2.0 ** (power // 2 - 1), sign * 2.0 ** (power - power // 2 - 1)
+        v, go = rand(gen, nk, heads, d, dtype=dtype), rand(gen, nq, heads, d, dtype=dtype)
+        kw = {}
+        if table:
+            c = lambda n: torch.zeros(n, 4, dtype=torch.int32, device="cuda")
+            kw = dict(bias=torch.zeros(1, heads, device="cuda"), edges=(), coords_q=c(nq), coords_k=c(nk))
+        scale = 4 * math.log(2)
+        got = attend(ops, q, k, v, go, scale=scale, **kw)
+        val, bnd = attention_ref(q, k, v, go=go, scale=scale * 2.0 ** -power, **{{"coords_q": "cq", "coords_k": "ck"}.get(n, n): t for n, t in kw.items()})
+        for name, g in zip(("out", "dq", "dk", "dv", "dt"), got):
+            more = 2.0 ** power if name in ("dq", "dk") else 1.0
+            within = (val[name].abs() + bnd[name]) * more < torch.finfo(g.dtype).max      # (fp16 at 2^28: a few values of dk are beyond its range)
+            assert within.all() or (dtype == F16 and power == 28 and name == "dk")
+            assert_within(g[within], val[name][within] * more, bnd[name][within] * more, 1e-30 if name == "dt" else TINY[dtype], f"{name} {nk} {heads}")
