@@ -265,14 +265,38 @@ constexpr int kTableRow = 64;
 __device__ __forceinline__ void at_put_cells(unsigned* __restrict__ cells, const unsigned* __restrict__ src) {
     for (int i = threadIdx.x; i < kCells; i += kAtBlock) cells[i] = (src[i] >> 8 << 10) | (src[i] & 255u) * 4;
 }
-// A finite entry is cut to 2^14 in units of log 2: beside any other score it is zero (or everything) long before that, and a row whose keys
-// all carry the type's lowest value still has scores that differ and sums that fp32 resolves.
+// A softmax only sees differences, and a score far enough below another is zero beside it.  So a head's finite entries keep their order and
+// their differences up to 2^14 in units of log 2; what is farther apart counts as that far, and the largest is brought to at most 2^14: a row
+// whose keys all carry the type's lowest value still has scores that differ and sums that fp32 resolves.  Entries within +-2^14 stay what
+// they are.  A wave takes a head, a lane a bucket.
 template <int HG>
 __device__ __forceinline__ void at_put_table(float* __restrict__ table, const AtBias& bias, int heads, int h0, float scale) {
     const float most = 16384.f / kLog2e;
-    for (int i = threadIdx.x; i < bias.buckets * HG; i += kAtBlock) {
-        const float v = bias.table[(int64_t)(i % bias.buckets) * heads + h0 + i / bias.buckets];
-        table[i / bias.buckets * kTableRow + i % bias.buckets] = (fabsf(v) < INFINITY ? fminf(fmaxf(v, -most), most) : v) / scale;
+    const int lane = lane_id();
+    for (int h = threadIdx.x >> 6; h < HG; h += kAtBlock / kWave) {
+        float v = lane < bias.buckets ? bias.table[(int64_t)lane * heads + h0 + h] : INFINITY;
+        const bool finite = fabsf(v) < INFINITY;
+        if (__any(finite && fabsf(v) > most)) {
+            auto largest = [&](bool of) {
+                float m = of ? v : -INFINITY;
+                for (int off = kWave / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+                return m;
+            };
+            // down the distinct values: `now` is what `at` becomes; from `top` on (as `put`) no two neighbours were too far apart
+            float at = largest(finite), now = fminf(fmaxf(at, -most), most), top = at, put = now, mine = v;
+            for (int n = 0; n < bias.buckets; ++n) {
+                if (finite && v == at) mine = now;
+                const float next = largest(finite && v < at);
+                if (next == -INFINITY) break;
+                if (at - next > most) {
+                    top = next;
+                    put = now = now - most;
+                } else now = put == top ? next : put - (top - next);
+                at = next;
+            }
+            v = mine;
+        }
+        if (lane < bias.buckets) table[h * kTableRow + lane] = v / scale;
     }
 }
 __device__ __forceinline__ int at_bucket(const unsigned* cells, float d2) {

@@ -2268,7 +2268,8 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seg_q: 
       slopes [H]            -slopes[h] * |c_i - c_j|, fixed (no gradient)
       bias [buckets, H]     a learned table: bias[b, h], b = number of `edges` (ascending whole squared distances, one less than
                             buckets: distance_edges) that |c_i - c_j|^2 reaches
-                            (an entry of -inf masks its bucket; finite entries beyond +-2^14 log 2 count as that)
+                            (an entry of -inf masks its bucket; finite entries of a head that are farther apart than 2^14 log 2 = 11 356
+                            count as that far: a finite mask holds against scores that differ by less)
     Gradients for q, k, v and bias; deterministic.  The backward pass keeps q, k, v, an fp32 copy of the output and two numbers per
     query and head -- never the scores.  A first call with new `edges` copies a small table to the device: make one before capturing a
     graph."""

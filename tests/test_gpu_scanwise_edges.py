@@ -121,3 +121,37 @@ def test_gradients_of_equal_scores_far_from_zero(ops, dtype, power, sign):
             within = (val[name].abs() + bnd[name]) * more < torch.finfo(g.dtype).max      # (fp16 at 2^28: a few values of dk are beyond its range)
             assert within.all() or (dtype == F16 and power == 28 and name == "dk")
             assert_within(g[within], val[name][within] * more, bnd[name][within] * more, 1e-30 if name == "dt" else TINY[dtype], f"{name} {nk} {heads}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_table_entries_far_out_keep_their_order(ops, dtype):
+    """Entries thousands to 10^38 apart: each key alone in its bucket, every pair of them visible to a query of its own -- the larger entry takes
+    everything.  (Some stand within fp32's steps of each other's size, none of them equal.)"""
+    for entries in ([-20000.0, -30000.0], [20000.0, 30000.0], [0.5, -1e4, -65504.0, torch.finfo(F32).min], [-1e9, -2e9, -3e38], [3e38, 1e38, 12000.0, 11000.0, -50.0],
+                    [-400.0 * i for i in range(48)], [-9000.0 * i * i for i in range(20)], [1e5, 2e5, -1e5, 0.0, 99000.0]):
+        n = len(entries)
+        edges = tuple(range(1, 30 * n, 30)[:n - 1]) if n <= 3 else ops.distance_edges(n, 100, 16)
+        # key b at a distance just inside bucket b, alone on a line from every query
+        at = torch.tensor([0] + [math.isqrt(e - 1) + 1 for e in edges], device="cuda")
+        assert [sum(e <= a * a for e in edges) for a in at.tolist()] == list(range(n))
+        ck = torch.zeros(n, 4, dtype=torch.int32, device="cuda")
+        ck[:, 1] = at
+        pairs = [(i, j) for i in range(n) for j in range(n) if i < j]
+        seg_q = torch.tensor([[p, p + 1] for p in range(len(pairs))], dtype=torch.int32)
+        keys = torch.tensor(pairs, device="cuda").reshape(-1)
+        gen = generator(35)
+        q, v, go = rand(gen, len(pairs), 2, 32, dtype=dtype), rand(gen, n, 2, 32, dtype=dtype)[keys], rand(gen, len(pairs), 2, 32, dtype=dtype)
+        k = rand(gen, 2 * len(pairs), 2, 32, dtype=dtype)
+        table = torch.tensor([[e, e] for e in entries], device="cuda")
+        table[:, 1] -= 3.0 if max(map(abs, entries)) < 1e6 else 0.0
+        cq = torch.zeros(len(pairs), 4, dtype=torch.int32, device="cuda")
+        got = attend(ops, q, k, v, go, seg_q.cuda(), (2 * seg_q).cuda(), coords_q=cq, coords_k=ck[keys].contiguous(), bias=table, edges=edges)
+        winner = torch.tensor([max(p, key=lambda b: entries[b]) for p in pairs], device="cuda")
+        want = v.reshape(len(pairs), 2, 2, 32)[torch.arange(len(pairs), device="cuda"), (winner != keys.view(-1, 2)[:, 0]).long()]
+        # one value times a probability of one: exact for 16-bit operands; fp32's three pieces meet again in six products, sums and the division, a
+        # half step or a cut (two half steps) each
+        off = (got[0].double() - want.double()).abs()
+        assert (off <= (16 * U32 if dtype == F32 else 0.0) * want.double().abs()).all(), (entries, off.max().item())
+        # (a probability of one: score gradients are zero but for the roundings of do . v against do . out, dim + 2 half steps of each addend)
+        assert all(torch.isfinite(g).all() for g in got)
+        assert (got[4].abs() <= 2 * 34 * U32 * (go.double() * want.double()).abs().sum((0, 2))).all()
