@@ -511,7 +511,7 @@ int64_t lidiff_nn_dist_grid_workspace_bytes(int64_t n, int64_t m, int32_t elem_b
 int lidiff_nn_dist_grid(const void* a, int64_t n, const void* b, int64_t m, int32_t elem_bytes, double cell, void* d2, int64_t* idx,
                         void* workspace, void* stream);
 
-/* The layouts of what the scan-wise operators hand from a forward call to its backward call (stats, lse): 2. */
+/* The layouts of what the scan-wise operators hand from a forward call to its backward call (stats, lse): 3. */
 int32_t lidiff_scanwise_version(void);
 
 /* ---- scan-wise operators: rows of the same scan share statistics / attend to each other -------------------------------------------
@@ -529,7 +529,7 @@ int lidiff_batch_segments(const int32_t* coords, int64_t rows, const int32_t* d_
 
 /* y = act((x - mean) rstd weight + bias) on x [rows][c] (c a multiple of 4, at most 1024; 16-byte aligned), mean and variance (biased)
  * over a segment's rows and a group's c / groups channels; weight / bias fp32 [c] or NULL; act: 0 none, 1 relu, 2 silu.
- * stats: fp32 [n_segments][groups][2] (mean, rstd), kept for the backward pass.  _bwd: dx, and dweight / dbias fp32 [c] (or NULL). */
+ * stats: fp32 [n_segments][groups][4] (the mean as two numbers whose sum it is, rstd, 0), kept for the backward pass.  _bwd: dx, and dweight / dbias fp32 [c] (or NULL). */
 int64_t lidiff_group_norm_workspace_bytes(int32_t c, int64_t n_segments);
 int lidiff_group_norm(const void* x, int64_t rows, int32_t c, int32_t groups, int32_t dtype, const int32_t* segments,
                       int64_t n_segments, const float* weight, const float* bias, float eps, int32_t act, void* y, float* stats,

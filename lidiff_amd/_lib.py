@@ -107,7 +107,7 @@ SIGNATURES = {
 }
 
 ABI_VERSION = 28
-SCANWISE_VERSION = 2          # layouts of what the scan-wise operators' forward calls hand to their backward calls
+SCANWISE_VERSION = 3          # layouts of what the scan-wise operators' forward calls hand to their backward calls
 _lib = None
 
 

@@ -5,7 +5,9 @@
 //   db_c = sum_s A_c,  dw_c = sum_s B_c,
 //   dx = rstd (dz w_c - [sum_c' w_c' A_c' + xh sum_c' w_c' B_c'] / n)       (sums over the group's channels, n = rows x channels)
 // HBM-bound, three launches a direction: partial sums of a slab of rows (one read of [M, C]), their sum in a fixed order, and the
-// pass that writes.  All statistics are held in double: exact to fp32 whatever the magnitude of the mean, and deterministic.
+// pass that writes.  The sums are held in double and taken of x less a value of the scan's (its first row's, one a group), so that the
+// variance keeps its bits however far the mean is from zero; the mean is kept as two floats, whose first takes the leading bits off x exactly.
+// Fixed orders: the same bits on every run.
 #include "segments.h"
 
 namespace lidiff {
@@ -72,21 +74,29 @@ __device__ __forceinline__ int2 gn_slab(int2 seg, int blk, int nblk) {
     return make_int2(seg.x + (int)(n * blk / nblk), seg.x + (int)(n * (blk + 1) / nblk));
 }
 
-// sums of x and x^2 per (segment, group) over a slab: part[s][g][blk][2]
+// sums of x - first and (x - first)^2 per (segment, group) over a slab: part[s][g][blk][2]; first: the value of the segment's first row in
+// the group's first channel, which goes to stats[s][g].x
 template <typename T, int V>
 __global__ __launch_bounds__(kGnBlock) void gn_stats_kernel(const T* __restrict__ x, int rows, int c, int groups, const int32_t* __restrict__ seg,
-                                                           int nblk, double* __restrict__ part) {
+                                                           int nblk, double* __restrict__ part, float4* __restrict__ stats) {
     extern __shared__ double gn_sm[];                                   // [rows per pass][c][2]
-    const int s = blockIdx.x / nblk, blk = blockIdx.x % nblk;
-    const int2 r = gn_slab(seg_range(seg, s, rows), blk, nblk);
+    const int s = blockIdx.x / nblk, blk = blockIdx.x % nblk, per = c / groups;
+    const int2 all = seg_range(seg, s, rows), r = gn_slab(all, blk, nblk);
     const GnLane<V> at(c);
     double a[V] = {}, b[V] = {};
     if (at.on) {
+        double from[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) from[e] = all.x < all.y ? (double)(float)x[(int64_t)all.x * c + (at.q * V + e) / per * per] : 0.0;
         for (int row = r.x + at.rl; row < r.y; row += at.rpb) {
             float f[V];
             gn_load<T, V>(x + (int64_t)row * c + at.q * V, f);
 #pragma unroll
-            for (int e = 0; e < V; ++e) { a[e] += f[e]; b[e] += (double)f[e] * f[e]; }
+            for (int e = 0; e < V; ++e) {
+                const double off = f[e] - from[e];
+                a[e] += off;
+                b[e] += off * off;
+            }
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -101,18 +111,18 @@ __global__ __launch_bounds__(kGnBlock) void gn_stats_kernel(const T* __restrict_
         gn_sm[i] = t;                                                   // (row lane 0's own place: read by this thread only)
     }
     __syncthreads();
-    const int per = c / groups;
     for (int i = threadIdx.x; i < 2 * groups; i += kGnBlock) {          // over the group's channels, in order
         const int g = i >> 1;
+        if (blk == 0 && i == 2 * g) stats[(int64_t)s * groups + g].x = all.x < all.y ? (float)x[(int64_t)all.x * c + g * per] : 0.f;      // (for the finish)
         double t = 0;
         for (int e = 0; e < per; ++e) t += gn_sm[(g * per + e) * 2 + (i & 1)];
         part[(((int64_t)s * groups + g) * nblk + blk) * 2 + (i & 1)] = t;
     }
 }
 
-// one wave per (segment, group): stats[s][g] = (mean, rstd)
+// one wave per (segment, group): stats[s][g] = (mean's leading float, the rest of it, rstd, 0)
 __global__ __launch_bounds__(kWave) void gn_finish_kernel(const double* __restrict__ part, int nblk, int rows, int c, int groups,
-                                                           const int32_t* __restrict__ seg, float eps, float2* __restrict__ stats) {
+                                                           const int32_t* __restrict__ seg, float eps, float4* __restrict__ stats) {
     const int sg = blockIdx.x;
     double a = 0, b = 0;
     for (int i = threadIdx.x; i < nblk; i += kWave) {
@@ -122,15 +132,16 @@ __global__ __launch_bounds__(kWave) void gn_finish_kernel(const double* __restri
     for (int off = kWave / 2; off > 0; off >>= 1) { a += __shfl_down(a, off); b += __shfl_down(b, off); }
     if (threadIdx.x != 0) return;
     const int2 r = seg_range(seg, sg / groups, rows);
-    const double n = (double)max(r.y - r.x, 1) * (c / groups), mean = a / n;
-    double var = b / n - mean * mean;
+    const double n = (double)max(r.y - r.x, 1) * (c / groups), off = a / n, mean = stats[sg].x + off;
+    double var = b / n - off * off;
     if (var < 0) var = 0;                                               // (a NaN passes)
-    stats[sg] = make_float2((float)mean, (float)(1.0 / sqrt(var + (double)eps)));
+    const float lead = (float)mean;
+    stats[sg] = make_float4(lead, (float)(mean - lead), (float)(1.0 / sqrt(var + (double)eps)), 0.f);
 }
 
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnBlock) void gn_apply_kernel(const T* __restrict__ x, int rows, int c, int groups, const int32_t* __restrict__ seg, int nseg,
-                                                           int tile, const float2* __restrict__ stats, const float* __restrict__ w, const float* __restrict__ b,
+                                                           int tile, const float4* __restrict__ stats, const float* __restrict__ w, const float* __restrict__ b,
                                                            T* __restrict__ y) {
     const GnLane<V> at(c);
     const SegTile t = find_seg_tile(seg, nseg, rows, tile, blockIdx.x);
@@ -140,10 +151,10 @@ __global__ __launch_bounds__(kGnBlock) void gn_apply_kernel(const T* __restrict_
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int ch = at.q * V + e;
-        const float2 st = t.seg >= 0 ? stats[(int64_t)t.seg * groups + ch / per] : make_float2(0.f, 0.f);
+        const float4 st = t.seg >= 0 ? stats[(int64_t)t.seg * groups + ch / per] : make_float4(0.f, 0.f, 0.f, 0.f);
         mean[e] = st.x;
-        scale[e] = st.y * (w ? w[ch] : 1.f);
-        shift[e] = b ? b[ch] : 0.f;
+        scale[e] = st.z * (w ? w[ch] : 1.f);
+        shift[e] = (b ? b[ch] : 0.f) - st.y * scale[e];
     }
     for (int row = t.lo + at.rl; row < t.hi; row += at.rpb) {
         float f[V] = {};
@@ -159,7 +170,7 @@ __global__ __launch_bounds__(kGnBlock) void gn_apply_kernel(const T* __restrict_
 // A_c and B_c over a slab: part[s][blk][2][c]
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnBlock) void gn_bwd_sums_kernel(const T* __restrict__ x, const T* __restrict__ dy, int rows, int c, int groups,
-                                                              const int32_t* __restrict__ seg, int nblk, const float2* __restrict__ stats,
+                                                              const int32_t* __restrict__ seg, int nblk, const float4* __restrict__ stats,
                                                               const float* __restrict__ w, const float* __restrict__ b, double* __restrict__ part) {
     extern __shared__ double gn_sm[];
     const int s = blockIdx.x / nblk, blk = blockIdx.x % nblk;
@@ -167,13 +178,13 @@ __global__ __launch_bounds__(kGnBlock) void gn_bwd_sums_kernel(const T* __restri
     const GnLane<V> at(c);
     if (at.on) {
         double sa[V] = {}, sb[V] = {};
-        float mean[V], rstd[V], wv[V], bv[V];
+        float mean[V], less[V], rstd[V], wv[V], bv[V];                  // xh = (x - mean) rstd - less
         const int per = c / groups;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const int ch = at.q * V + e;
-            const float2 st = stats[(int64_t)s * groups + ch / per];
-            mean[e] = st.x; rstd[e] = st.y;
+            const float4 st = stats[(int64_t)s * groups + ch / per];
+            mean[e] = st.x; rstd[e] = st.z; less[e] = st.y * st.z;
             wv[e] = w ? w[ch] : 1.f;
             bv[e] = b ? b[ch] : 0.f;
         }
@@ -183,7 +194,7 @@ __global__ __launch_bounds__(kGnBlock) void gn_bwd_sums_kernel(const T* __restri
             gn_load<T, V>(dy + (int64_t)row * c + at.q * V, g);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float xh = (f[e] - mean[e]) * rstd[e];
+                const float xh = (f[e] - mean[e]) * rstd[e] - less[e];
                 const float dz = g[e] * gn_act_slope<ACT>(xh * wv[e] + bv[e]);
                 sa[e] += dz;
                 sb[e] += (double)dz * xh;
@@ -223,7 +234,7 @@ __global__ __launch_bounds__(256) void gn_bwd_finish_kernel(const double* __rest
 // the last workgroup of the grid adds the scans' A_c / B_c to db / dw; the others write dx
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnBlock) void gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ dy, int rows, int c, int groups,
-                                                               const int32_t* __restrict__ seg, int nseg, int tile, const float2* __restrict__ stats,
+                                                               const int32_t* __restrict__ seg, int nseg, int tile, const float4* __restrict__ stats,
                                                                const double* __restrict__ chan, const float* __restrict__ w, const float* __restrict__ b,
                                                                T* __restrict__ dx, float* __restrict__ dw, float* __restrict__ db) {
     if (blockIdx.x == gridDim.x - 1) {
@@ -254,12 +265,12 @@ __global__ __launch_bounds__(kGnBlock) void gn_bwd_apply_kernel(const T* __restr
     }
     __syncthreads();
     if (!at.on) return;
-    float mean[V], rstd[V], wv[V], bv[V], ma[V], mb[V];
+    float mean[V], less[V], rstd[V], wv[V], bv[V], ma[V], mb[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int ch = at.q * V + e, g = ch / per;
-        const float2 st = t.seg >= 0 ? stats[(int64_t)t.seg * groups + g] : make_float2(0.f, 0.f);
-        mean[e] = st.x; rstd[e] = st.y;
+        const float4 st = t.seg >= 0 ? stats[(int64_t)t.seg * groups + g] : make_float4(0.f, 0.f, 0.f, 0.f);
+        mean[e] = st.x; rstd[e] = st.z; less[e] = st.y * st.z;
         wv[e] = w ? w[ch] : 1.f;
         bv[e] = b ? b[ch] : 0.f;
         ma[e] = t.seg >= 0 ? sums[2 * g] : 0.f;
@@ -273,7 +284,7 @@ __global__ __launch_bounds__(kGnBlock) void gn_bwd_apply_kernel(const T* __restr
             gn_load<T, V>(dy + (int64_t)row * c + at.q * V, g);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float xh = (f[e] - mean[e]) * rstd[e];
+                const float xh = (f[e] - mean[e]) * rstd[e] - less[e];
                 const float dz = g[e] * gn_act_slope<ACT>(xh * wv[e] + bv[e]);
                 f[e] = rstd[e] * (dz * wv[e] - ma[e] - xh * mb[e]);
             }
@@ -292,16 +303,16 @@ static int gn_slabs(int64_t rows, int c, int v, int64_t nseg) {
 
 template <typename T, int V, int ACT>
 static void gn_fwd_launch(const void* x, int rows, int c, int groups, const int32_t* seg, int nseg, const float* w, const float* b, float eps, void* y,
-                          float2* stats, double* ws, hipStream_t st) {
+                          float4* stats, double* ws, hipStream_t st) {
     const int nblk = gn_slabs(rows, c, V, nseg), rpb = kGnBlock / (c / V), tile = gn_tile(rows, rpb);
-    gn_stats_kernel<T, V><<<(unsigned)(nseg * nblk), kGnBlock, (size_t)rpb * c * 2 * sizeof(double), st>>>((const T*)x, rows, c, groups, seg, nblk, ws);
+    gn_stats_kernel<T, V><<<(unsigned)(nseg * nblk), kGnBlock, (size_t)rpb * c * 2 * sizeof(double), st>>>((const T*)x, rows, c, groups, seg, nblk, ws, stats);
     gn_finish_kernel<<<(unsigned)(nseg * groups), kWave, 0, st>>>(ws, nblk, rows, c, groups, seg, eps, stats);
     gn_apply_kernel<T, V, ACT><<<(unsigned)seg_tiles_bound(rows, tile, seg, nseg), kGnBlock, 0, st>>>(
         (const T*)x, rows, c, groups, seg, nseg, tile, stats, w, b, (T*)y);
 }
 
 template <typename T, int V, int ACT>
-static void gn_bwd_launch(const void* x, const void* dy, int rows, int c, int groups, const int32_t* seg, int nseg, const float2* stats, const float* w,
+static void gn_bwd_launch(const void* x, const void* dy, int rows, int c, int groups, const int32_t* seg, int nseg, const float4* stats, const float* w,
                           const float* b, void* dx, float* dw, float* db, double* ws, hipStream_t st) {
     const int nblk = gn_slabs(rows, c, V, nseg), rpb = kGnBlock / (c / V), tile = gn_tile(rows, rpb);
     double* chan = ws + (int64_t)nseg * nblk * 2 * c;
@@ -343,7 +354,7 @@ static const char* gn_check(int64_t rows, int c, int groups, int dtype, int64_t 
 
 using namespace lidiff;
 
-extern "C" int32_t lidiff_scanwise_version(void) { return 2; }
+extern "C" int32_t lidiff_scanwise_version(void) { return 3; }
 
 extern "C" int64_t lidiff_group_norm_workspace_bytes(int32_t c, int64_t n_segments) {
     const int64_t slabs = n_segments > kGnSlabs ? n_segments : kGnSlabs;               // of all scans together (gn_slabs)
@@ -356,9 +367,9 @@ extern "C" int lidiff_group_norm(const void* x, int64_t rows, int32_t c, int32_t
     const char* bad = gn_check(rows, c, groups, dtype, n_segments, act);
     LIDIFF_CHECK_ARG(bad == nullptr, bad);
     LIDIFF_CHECK_ARG(segments || n_segments == 1, "without segments all rows are one");
-    LIDIFF_CHECK_ARG((((uintptr_t)x | (uintptr_t)y) & 15) == 0 && (((uintptr_t)segments | (uintptr_t)stats | (uintptr_t)workspace) & 7) == 0, "misaligned pointer");
+    LIDIFF_CHECK_ARG((((uintptr_t)x | (uintptr_t)y) & 15) == 0 && (((uintptr_t)segments | (uintptr_t)workspace) & 7) == 0 && ((uintptr_t)stats & 15) == 0, "misaligned pointer");
     const int nseg = (int)n_segments;
-    GN_DISPATCH(gn_fwd_launch, x, (int)rows, c, groups, segments, nseg, weight, bias, eps, y, (float2*)stats, (double*)workspace, (hipStream_t)stream);
+    GN_DISPATCH(gn_fwd_launch, x, (int)rows, c, groups, segments, nseg, weight, bias, eps, y, (float4*)stats, (double*)workspace, (hipStream_t)stream);
     LIDIFF_CHECK_LAUNCH();
     return 0;
 }
@@ -370,10 +381,10 @@ extern "C" int lidiff_group_norm_bwd(const void* x, const void* dy, int64_t rows
     const char* bad = gn_check(rows, c, groups, dtype, n_segments, act);
     LIDIFF_CHECK_ARG(bad == nullptr, bad);
     LIDIFF_CHECK_ARG(segments || n_segments == 1, "without segments all rows are one");
-    LIDIFF_CHECK_ARG((((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx) & 15) == 0 && (((uintptr_t)segments | (uintptr_t)stats | (uintptr_t)workspace) & 7) == 0,
+    LIDIFF_CHECK_ARG((((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx | (uintptr_t)stats) & 15) == 0 && (((uintptr_t)segments | (uintptr_t)workspace) & 7) == 0,
                      "misaligned pointer");
     const int nseg = (int)n_segments;
-    GN_DISPATCH(gn_bwd_launch, x, dy, (int)rows, c, groups, segments, nseg, (const float2*)stats, weight, bias, dx, dweight, dbias, (double*)workspace,
+    GN_DISPATCH(gn_bwd_launch, x, dy, (int)rows, c, groups, segments, nseg, (const float4*)stats, weight, bias, dx, dweight, dbias, (double*)workspace,
                 (hipStream_t)stream);
     LIDIFF_CHECK_LAUNCH();
     return 0;

@@ -2073,7 +2073,7 @@ class _GroupNorm(torch.autograd.Function):
         w = None if weight is None else _aligned(weight.detach().float())
         b = None if bias is None else _aligned(bias.detach().float())
         y = torch.empty_like(x)
-        stats = torch.empty((n_seg, groups, 2), dtype=torch.float32, device=x.device)
+        stats = torch.empty((n_seg, groups, 4), dtype=torch.float32, device=x.device)
         if m:
             ws = torch.empty(_lib.load().lidiff_group_norm_workspace_bytes(c, n_seg), dtype=torch.uint8, device=x.device)
             call("lidiff_group_norm", ptr(x), m, c, groups, _ROW_DTYPES[x.dtype], ptr(segments), n_seg, ptr(w), ptr(b), float(eps),

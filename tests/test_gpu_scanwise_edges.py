@@ -155,3 +155,30 @@ def test_table_entries_far_out_keep_their_order(ops, dtype):
         # (a probability of one: score gradients are zero but for the roundings of do . v against do . out, dim + 2 half steps of each addend)
         assert all(torch.isfinite(g).all() for g in got)
         assert (got[4].abs() <= 2 * 34 * U32 * (go.double() * want.double()).abs().sum((0, 2))).all()
+
+
+@pytest.mark.parametrize("mean", [0.0, 1e3, -1e5, 3e6])
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_group_norm_of_means_far_from_zero(ops, mean, act):
+    """Means up to 3 10^6 times the spread: errors are those of the spread.
+
+    y: x - mean (the leading float: exact or a half step, the rest of it folded into the shift), rstd, the product and the shift, a half step
+    each of at most 1 + |z|; silu as group_norm_ref counts it.  dx = rstd (t - ma - xh mb), each term off by a few half steps of itself and of
+    mean |t xh|."""
+    gen = generator(36)
+    seg = ranges([3000, 1, 1000], [0, 2, 0]).cuda()
+    x = rand(gen, 4003, 16) + mean
+    x[5] += 50.0 * rand(gen, 16)
+    dy = rand(gen, 4003, 16)
+    val, _ = group_norm_ref(x, 4, None, None, seg, 1e-5, act, dy)
+    plain, _ = group_norm_ref(x, 4, None, None, seg, 1e-5, None, dy)
+    z = plain["y"].abs()
+    leaf = x.clone().requires_grad_()
+    y = ops.group_norm(leaf, 4, segments=seg, activation=act)
+    dx, = torch.autograd.grad(y, [leaf], dy)
+    assert_within(y.detach(), val["y"], 16 * U32 * (1 + z) * (1 + (z if act else 0)), 0, f"y {mean}")
+    for lo, hi in seg.tolist():
+        rstd = (x[lo:hi].double().reshape(hi - lo, 4, 4).var((0, 2), unbiased=False) + 1e-5).rsqrt().repeat_interleave(4)
+        t = 1.1 * dy[lo:hi].double().abs()
+        size = t + t.mean() * 8 + z[lo:hi] * (t * (1 + z[lo:hi])).mean() * 8
+        assert_within(dx[lo:hi], val["dx"][lo:hi], 32 * U32 * rstd * size * (1 + (z[lo:hi] if act else 0)), 0, f"dx {mean}")
