@@ -32,24 +32,33 @@ DEFAULT_HPARAMS = {   # lidiff/config/config.yaml
 }
 
 
+def _attention_heads(checkpoint, network, configured):
+    """The heads of a network's attention block: what the checkpoint's weights hold (its own hyper-parameters name them differently for the two
+    networks, and weights without a block to go to would be dropped by the lenient load), else what is configured."""
+    table = None if checkpoint is None else checkpoint["state_dict"].get(f"{network}.attention.distance_bias")
+    return configured if table is None else table.shape[1]
+
+
 class DiffCompletion(nn.Module):
     def __init__(self, diff_path=None, refine_path=None, denoising_steps=50, cond_weight=6.0,
                  hparams=None, device="cuda"):
         super().__init__()
         ckpt_diff = torch.load(diff_path, map_location="cpu") if diff_path else None
+        ckpt_refine = torch.load(refine_path, map_location="cpu") if refine_path else None
         self.hparams = _merge(DEFAULT_HPARAMS, (ckpt_diff or {}).get("hyper_parameters", hparams or {}))
         assert denoising_steps <= self.hparams["diff"]["t_steps"], \
             f"The number of denoising steps cannot be bigger than T={self.hparams['diff']['t_steps']}"
         out_dim = self.hparams["model"]["out_dim"]
         self.partial_enc = minknet.MinkGlobalEnc(in_channels=3, out_channels=out_dim)
         self.model = minknet.MinkUNetDiff(in_channels=3, out_channels=out_dim,
-                                          attention_heads=self.hparams["model"].get("attention_heads", 0))
+                                          attention_heads=_attention_heads(ckpt_diff, "model", self.hparams["model"].get("attention_heads", 0)))
         self.model_refine = minknet.MinkUNet(in_channels=3, out_channels=3 * 6,
-                                             attention_heads=self.hparams["model"].get("refine_attention_heads", 0))
+                                             attention_heads=_attention_heads(ckpt_refine, "model_refine",
+                                                                              self.hparams["model"].get("refine_attention_heads", 0)))
         if ckpt_diff is not None:
             self.load_state_dict(ckpt_diff["state_dict"], strict=False)
-        if refine_path:
-            self.load_state_dict(torch.load(refine_path, map_location="cpu")["state_dict"], strict=False)
+        if ckpt_refine is not None:
+            self.load_state_dict(ckpt_refine["state_dict"], strict=False)
         self.eval()
         self.to(device)
         self.device = torch.device(device)
