@@ -113,6 +113,11 @@ class CoordinateManager:
         """int32 [1] device tensor with the valid rows of a read-free map, None for a map of exact size."""
         return self.maps[ts].count
 
+    def set_scans(self, scans: int, resolution: float | None = None):
+        """The field holds `scans` scans in order, batch index i for scan i -- or i / resolution, rounded, where the batch column is divided
+        along with the points: no host read for the scans' row ranges.  (An index that no scan has is an empty range.)"""
+        self.batches = max(scans if resolution is None else math.ceil((scans - 1) / resolution) + 1, 1)
+
     def n_batches(self) -> int:
         """How many batch indices the field's rows may have (the largest one + 1).  Read from the device once per manager, unless whoever
         made the field knew it (`batches`); rows that are not grouped by ascending batch index raise ValueError there."""

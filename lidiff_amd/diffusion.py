@@ -79,12 +79,15 @@ class DiffusionPoints(nn.Module):
 
     # models.py:162-178 (batch column NOT divided, unlike the inference pipeline)
     def points_to_tensor(self, x_feats, mean=None, std=None):
+        scans = len(x_feats)
         x_feats = ME.utils.batched_coordinates(list(x_feats[:]), dtype=torch.float32, device=self.device)
         x_coord = x_feats.clone()
         x_coord[:, 1:] = torch.round(x_feats[:, 1:] / self.hparams["data"]["resolution"])   # collations.py:8-12
-        return ME.TensorField(features=x_feats[:, 1:], coordinates=x_coord,
-                              quantization_mode=ME.SparseTensorQuantizationMode.UNWEIGHTED_AVERAGE,
-                              minkowski_algorithm=ME.MinkowskiAlgorithm.SPEED_OPTIMIZED, device=self.device)
+        field = ME.TensorField(features=x_feats[:, 1:], coordinates=x_coord,
+                               quantization_mode=ME.SparseTensorQuantizationMode.UNWEIGHTED_AVERAGE,
+                               minkowski_algorithm=ME.MinkowskiAlgorithm.SPEED_OPTIMIZED, device=self.device)
+        field.coordinate_manager.set_scans(scans)
+        return field
 
     # models.py:156-160
     def forward(self, x_full, x_full_sparse, x_part, t):
@@ -199,6 +202,7 @@ class RefineDiffusion(nn.Module):
         x_t = ME.TensorField(features=x_feats, coordinates=x_coord,
                              quantization_mode=ME.SparseTensorQuantizationMode.UNWEIGHTED_AVERAGE,
                              minkowski_algorithm=ME.MinkowskiAlgorithm.SPEED_OPTIMIZED, device=self.device)
+        x_t.coordinate_manager.set_scans(len(batch["pcd_noise"]), self.hparams["data"]["resolution"])
         offset = self.forward_refine(prebuild_maps(x_t)).reshape(-1, up, 3)
         pred = (x_feats[:, None, :] + offset).reshape(batch["pcd_full"].shape[0], -1, 3)
         return chamfer_distance(pred, batch["pcd_full"].to(self.device).float())

@@ -162,8 +162,8 @@ class DiffCompletion(nn.Module):
                                quantization_mode=ME.SparseTensorQuantizationMode.UNWEIGHTED_AVERAGE,
                                minkowski_algorithm=ME.MinkowskiAlgorithm.SPEED_OPTIMIZED, device=self.device)
         mgr = field.coordinate_manager
-        if scans == 1:
-            mgr.batches = 1              # (known here: no host read for the scans' row ranges; several scans: CoordinateManager.n_batches)
+        if scans is not None:
+            mgr.set_scans(scans, self.hparams["data"]["resolution"])
         mgr.pyramid = self.single_read and field.F.device.type == "cuda"
         if (role is not None and mgr.pyramid and (self.read_free or self.hint_lag) and self.pair_cfg and minknet._FUSION
                 and not self.training and feats.shape[0] >= 1):
