@@ -487,7 +487,8 @@ int lidiff_fps(const double* points, int64_t n_points, int64_t n_samples, int64_
  * timed out -- the selection is then incomplete: run lidiff_fps.  Returns non-zero, nothing enqueued, when the device
  * cannot hold the grid co-resident (no cooperative launch, or more than 8192 points per CU) -- which
  * lidiff_fps_coop_supported(n_points) answers beforehand (1 / 0) --, and 3, nothing selected, when the runtime refuses the launch at
- * this moment (another process holds the device's one cooperative queue): run lidiff_fps. */
+ * this moment (another process holds the device's one cooperative queue, or the grid does not fit; lidiff_last_error says which): run
+ * lidiff_fps. */
 int32_t lidiff_fps_coop_supported(int64_t n_points);
 int lidiff_fps_coop(const double* points, int64_t n_points, int64_t n_samples, int64_t* selected, void* workspace,
                     int32_t* status, void* stream);

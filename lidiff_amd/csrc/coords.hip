@@ -1909,9 +1909,10 @@ int lidiff_fps_coop(const double* points, int64_t n_points, int64_t n_samples, i
     void* args[] = {(void*)&points, (void*)&n_points, (void*)&n_samples, (void*)&pt, (void*)&selected, (void*)&part_val,
                     (void*)&part_idx, (void*)&counter, (void*)&status};
     const hipError_t rc = hipLaunchCooperativeKernel((const void*)fps_coop_kernel, dim3(grid), dim3(kFpsBlock), args, 0, st);
-    if (rc == hipErrorIllegalState || rc == hipErrorCooperativeLaunchTooLarge) {      // another process holds the device's cooperative queue
+    // (another process that holds the device's cooperative queue; compute units that the occupancy query counted and the launch did not get)
+    if (rc == hipErrorIllegalState || rc == hipErrorCooperativeLaunchTooLarge) {
         (void)hipGetLastError();
-        set_error("%s: the cooperative launch is not available now (%s): run lidiff_fps", __func__, hipGetErrorString(rc));
+        set_error("%s: the runtime refuses the cooperative launch now (%s): run lidiff_fps", __func__, hipGetErrorString(rc));
         return 3;
     }
     LIDIFF_CHECK_HIP(rc);

@@ -1798,14 +1798,14 @@ def farthest_point_sample(points: torch.Tensor, n_samples: int) -> torch.Tensor:
     if FPS_COOPERATIVE and _lib.load().lidiff_fps_coop_supported(n):
         # one persistent cooperative launch (device-wide barrier per selection).  Its status word is read back -- the caller
         # indexes with the result on the host side of the step anyway.  A barrier time-out (reported, not silent) and a launch
-        # that the runtime refuses because another process holds the cooperative queue (status 3) fall back to the
+        # that the runtime refuses (status 3: another process holds the cooperative queue, say) fall back to the
         # launch-per-selection kernel below (same indices); every other failure raises.
         status = torch.empty(1, dtype=torch.int32, device=pts.device)
         refused = call("lidiff_fps_coop", ptr(pts), n, int(n_samples), ptr(sel), ptr(ws), ptr(status), stream_ptr(), accept=(3,))
         if not refused and int(status.item()) == 0:
             return sel
         import warnings
-        warnings.warn("lidiff_fps_coop: the cooperative launch is held by another process; running lidiff_fps" if refused else
+        warnings.warn(f"{_lib.load().lidiff_last_error().decode()}; running lidiff_fps" if refused else
                       "lidiff_fps_coop: device-wide barrier timed out; re-running the selection with lidiff_fps")
     call("lidiff_fps", ptr(pts), n, int(n_samples), ptr(sel), ptr(ws), stream_ptr())
     return sel

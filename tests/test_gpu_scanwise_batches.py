@@ -49,3 +49,21 @@ def test_fields_of_the_pipeline_know_their_scans(device, asked, scans, fused):
     x = pipe.points_to_tensor(small_batch(scans, 1000)["pcd_full"].to(device)).sparse()
     assert x.segments().shape[0] == (1 if scans == 1 else 21)
     assert len(asked) == 1
+
+
+def test_farthest_points_where_the_cooperative_launch_is_refused(device, monkeypatch):
+    """The warning gives the library's reason, whatever it is; the indices are those of the cooperative launch."""
+    from lidiff_amd import _lib, ops
+    points = torch.randn(3000, 3, dtype=torch.float64, generator=torch.Generator().manual_seed(5)).to(device)
+    want, real = ops.farthest_point_sample(points, 100), ops.call
+    class Library:
+        def __getattr__(self, name):
+            return getattr(lib, name)
+        def lidiff_last_error(self):
+            return b"lidiff_fps_coop: the runtime refuses the cooperative launch now (a reason of its own)"
+    lib = _lib.load()
+    monkeypatch.setattr(ops, "call", lambda name, *a, **k: 3 if name == "lidiff_fps_coop" else real(name, *a, **k))
+    monkeypatch.setattr(_lib, "load", lambda: Library())
+    with pytest.warns(UserWarning, match="a reason of its own.*running lidiff_fps"):
+        got = ops.farthest_point_sample(points, 100)
+    assert torch.equal(got, want)
