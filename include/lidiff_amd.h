@@ -528,7 +528,8 @@ int32_t lidiff_scanwise_version(void);
 int lidiff_batch_segments(const int32_t* coords, int64_t rows, const int32_t* d_rows, int32_t n_batches, int32_t replicas,
                           int32_t* segments, int32_t* d_status, void* stream);
 
-/* y = act((x - mean) rstd weight + bias) on x [rows][c] (c a multiple of 4, at most 1024; 16-byte aligned), mean and variance (biased)
+/* y = act((x - mean) rstd weight + bias) on x [rows][c] (c a multiple of 4, at most 1024; 16-byte aligned; n_segments x groups <= 2^25,
+ * n_segments x c <= 2^26, rows x c <= 2^33), mean and variance (biased)
  * over a segment's rows and a group's c / groups channels; weight / bias fp32 [c] or NULL; act: 0 none, 1 relu, 2 silu.
  * stats: fp32 [n_segments][groups][4] (the mean as two numbers whose sum it is, rstd, 0), kept for the backward pass.  _bwd: dx, and dweight / dbias fp32 [c] (or NULL). */
 int64_t lidiff_group_norm_workspace_bytes(int32_t c, int64_t n_segments);
@@ -541,7 +542,7 @@ int lidiff_group_norm_bwd(const void* x, const void* dy, int64_t rows, int32_t c
 
 /* out[i] = sum_j softmax_j(q_i . k_j scale + bias) v_j over the keys j of query i's segment (segment s of the queries reads segment s of
  * the keys; a query without keys gives zeros).  q [mq][heads][dim], k / v [mk][kv_heads][dim] (query head h reads key head
- * h * kv_heads / heads), dim a multiple of 8 in [8, 128], 1e-6 <= scale <= 1e6; strides: HOST int64 array, in elements: q row, q head, k row, k head, v row,
+ * h * kv_heads / heads), dim a multiple of 8 in [8, 128], 1e-6 <= scale <= 1e6; rows x heads <= 2^26, n_segments x heads <= 2^22; strides: HOST int64 array, in elements: q row, q head, k row, k head, v row,
  * v head (the channels are contiguous; every stride and pointer a multiple of 16 bytes).  out contiguous.
  * bias_mode: 0 none; 1: -slopes[head] * |c_i - c_j|; 2: table[bucket][head], bucket = edges <= |c_i - c_j|^2 (table fp32
  * [buckets][heads], buckets <= 48; cells: the look-up table of the edges that ops.bucket_cells builds).  coords_q / coords_k: int32

@@ -337,6 +337,7 @@ inline const char* at_check(int64_t nseg, int64_t mq, int64_t mk, int heads, int
     if (mq < 1 || mk < 0 || mq > 0x7fffffff - (1 << 22) || mk > 0x7fffffff - (1 << 22)) return "need 1 <= query rows, 0 <= key rows, both below 2^31 - 2^22";
     if (heads < 1 || heads > 1024 || kv_heads < 1 || heads % kv_heads) return "the key heads must divide the query heads (at most 1024)";
     if (mq * heads * 128 > (int64_t)1 << 33 || mk * kv_heads * 128 > (int64_t)1 << 33) return "need rows x heads <= 2^26";      // (one launch's workgroups)
+    if (nseg * heads > 1 << 22) return "need segments x heads <= 2^22";                      // (likewise: a segment takes up to two workgroups a head)
     if (dim < 8 || dim > 128 || dim % 8) return "head dimension: a multiple of 8 in [8, 128]";
     if (dtype < 0 || dtype > 2) return "dtype: 0 fp32, 1 bf16, 2 fp16";
     if (!(scale >= 1e-6f && scale <= 1e6f)) return "need 1e-6 <= scale <= 1e6";

@@ -346,6 +346,7 @@ static const char* gn_check(int64_t rows, int c, int groups, int dtype, int64_t 
     if (groups < 1 || c % groups) return "the groups must divide the channels";
     if (dtype < 0 || dtype > 2) return "dtype: 0 fp32, 1 bf16, 2 fp16";
     if (nseg < 1 || nseg > 1 << 20) return "need 1 <= segments <= 2^20";
+    if (nseg * groups > 1 << 25 || nseg * c > 1 << 26) return "need segments x groups <= 2^25, segments x channels <= 2^26";      // (likewise)
     if (act < 0 || act > 2) return "activation: 0 none, 1 relu, 2 silu";
     return nullptr;
 }

@@ -41,3 +41,21 @@ def test_a_checkpoint_s_attention_block_is_loaded(tmp_path):
     # a checkpoint without hyper-parameters
     torch.save({"state_dict": torch.load(paths["diff"])["state_dict"]}, tmp_path / "bare.ckpt")
     assert DiffCompletion(tmp_path / "bare.ckpt", device="cpu").model.attention.num_heads == 8
+
+
+def test_more_segments_than_a_launch_holds_are_refused():
+    """A launch has at most 2^32 threads in a row: more segments x heads (groups, channels) are refused before anything is queued."""
+    import ctypes
+    from lidiff_amd import _lib
+    lib = _lib.load()
+    P = lambda i=1: ctypes.c_void_p(4096 * i)                       # (never read: the checks come first)
+    word = lambda: lib.lidiff_last_error().decode()
+    for segments, c, groups in ((1 << 20, 256, 64), (1 << 20, 1024, 1), (1 << 19, 128, 128)):
+        assert lib.lidiff_group_norm(P(), 8, c, groups, 0, P(2), segments, None, None, 1e-5, 0, P(3), P(4), P(5), None) == 1 and "segments x" in word()
+        assert lib.lidiff_group_norm_bwd(P(), P(), 8, c, groups, 0, P(2), segments, None, None, P(4), 0, P(3), None, None, P(5), None) == 1 and "segments x" in word()
+    strides = (ctypes.c_int64 * 8)(*[512, 32] * 4)
+    for segments, heads in ((1 << 20, 8), (1 << 18, 32), (1 << 13, 1024)):
+        assert lib.lidiff_segment_attention(P(), P(), P(), strides, None, None, P(2), P(3), segments, 8, 8, heads, heads, 32, 1, 0.2, 0, None, None, None, 0, P(4),
+                                            None, 0, None, P(5), None) == 1 and "segments x heads" in word()
+        assert lib.lidiff_segment_attention_bwd(P(), P(), P(), P(), strides, None, None, P(2), P(3), segments, 8, 8, heads, heads, 32, 1, 0.2, 0, None, None, None, 0,
+                                                P(4), P(5), P(6), P(7), P(8), None, P(9), None) == 1 and "segments x heads" in word()
