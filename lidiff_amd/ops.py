@@ -2029,7 +2029,7 @@ def batch_segments(coords: torch.Tensor, n_batches: int | None = None, d_rows: t
         raise ValueError("d_rows must be one int32 on the device")
     _same_device(coords.device, d_rows=d_rows, status=status)
     require_device(coords)
-    coords = coords.contiguous()
+    coords = _aligned(coords)
     rows = coords.shape[0]
     read = n_batches is None
     if read:
@@ -2138,7 +2138,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
     _check_segments("segments", segments, x.device)
     require_device(x)
     with _on(x.device):
-        return _GroupNorm.apply(x, weight, bias, None if segments is None else segments.contiguous(), int(num_groups), float(eps),
+        return _GroupNorm.apply(x, weight, bias, None if segments is None else _aligned(segments), int(num_groups), float(eps),
                                 _ACTIVATIONS[activation])
 
 

@@ -182,3 +182,19 @@ def test_group_norm_of_means_far_from_zero(ops, mean, act):
         t = 1.1 * dy[lo:hi].double().abs()
         size = t + t.mean() * 8 + z[lo:hi] * (t * (1 + z[lo:hi])).mean() * 8
         assert_within(dx[lo:hi], val["dx"][lo:hi], 32 * U32 * rstd * size * (1 + (z[lo:hi] if act else 0)), 0, f"dx {mean}")
+
+
+def test_index_tensors_at_any_offset_of_their_storage(ops):
+    """Segments and coordinates that are views one element into a buffer: the results of aligned copies."""
+    gen = generator(37)
+    x, c, seg = rand(gen, 90, 32), voxel_rows(gen, 90), ranges([50, 0, 40]).cuda()
+    c[60:, 0] = 1
+    def off(t):
+        flat = torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(t.shape)
+    assert torch.equal(ops.group_norm(x, 8, segments=off(seg)), ops.group_norm(x, 8, segments=seg))
+    assert ops.batch_segments(off(c)).tolist() == [[0, 60], [60, 90]]
+    q, slopes = rand(gen, 90, 4, 32), torch.full((4,), 0.02, device="cuda")
+    assert torch.equal(ops.segment_attention(q, q, q, off(seg), off(seg), coords_q=off(c), coords_k=off(c), slopes=off(slopes)),
+                       ops.segment_attention(q, q, q, seg, seg, coords_q=c, coords_k=c, slopes=slopes))
