@@ -468,7 +468,7 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
         }
         for (int tile = first; tile < last; ++tile) {
             AT_ARRIVE();
-                if (tile + 1 < last) {
+            if (tile + 1 < last) {
                 put_coords(tile + 1);
                 coords(tile + 2);
             }

@@ -198,3 +198,40 @@ def test_index_tensors_at_any_offset_of_their_storage(ops):
     q, slopes = rand(gen, 90, 4, 32), torch.full((4,), 0.02, device="cuda")
     assert torch.equal(ops.segment_attention(q, q, q, off(seg), off(seg), coords_q=off(c), coords_k=off(c), slopes=off(slopes)),
                        ops.segment_attention(q, q, q, seg, seg, coords_q=c, coords_k=c, slopes=slopes))
+
+
+def test_offsets_beyond_32_bits(ops):
+    """Row matrices of more than 2^31 elements, keys whose rows stand 8 MiB apart: the last rows' results are those of a copy of them."""
+    gen = generator(38)
+    rows, c = 8_600_000, 256
+    x = torch.empty(rows, c, dtype=BF16, device="cuda")
+    x[:-1000] = 3.0
+    x[-1000:] = rand(gen, 1000, c, dtype=BF16)
+    seg = torch.tensor([[0, rows - 1000], [rows - 1000, rows]], dtype=torch.int32, device="cuda")
+    leaf, last = x.requires_grad_(), x[-1000:].detach().clone().requires_grad_()
+    y = ops.group_norm(leaf, 8, segments=seg, activation="silu")
+    z = ops.group_norm(last, 8, activation="silu")
+    # (more slabs share the rows of a scan alone: the doubles' sums round elsewhere, 2^-24 of the statistics at most, a half step of bf16 once)
+    assert ((y[-1000:].double() - z.double()).abs() <= 2.0 ** -7 * z.double().abs() + 1e-6).all() and (y[:1000] == 0).all()
+    go = rand(gen, 1000, c, dtype=BF16)
+    dy = torch.zeros_like(x)
+    dy[-1000:] = go
+    g, = torch.autograd.grad(y, [leaf], dy)
+    h, = torch.autograd.grad(z, [last], go)
+    assert ((g[-1000:].double() - h.double()).abs() <= 2.0 ** -7 * h.double().abs() + 1e-5).all() and (g[:1000] == 0).all()
+    del x, y, g, dy, leaf
+    torch.cuda.empty_cache()
+    wide = torch.empty(600, (1 << 22) - 8, dtype=BF16, device="cuda")
+    parts = [rand(gen, 600, 2, 32, dtype=BF16) for _ in range(3)]
+    for i, t in enumerate(parts):
+        wide[:, 64 * i:64 * i + 64] = t.reshape(600, 64)
+    slots = [wide[:, 64 * i:64 * i + 64].unflatten(1, (2, 32)) for i in range(3)]
+    go, slopes, cs = rand(gen, 600, 2, 32, dtype=BF16), torch.full((2,), 0.02, device="cuda"), voxel_rows(gen, 600)
+    outs = []
+    for q, k, v in (slots, parts):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        assert leaves[0].stride(0) in ((1 << 22) - 8, 64)
+        out = ops.segment_attention(*leaves, coords_q=cs, coords_k=cs, slopes=slopes)
+        outs.append((out.detach(),) + torch.autograd.grad(out, leaves, go))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
