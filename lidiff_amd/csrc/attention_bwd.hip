@@ -1,8 +1,14 @@
 // Attention between the rows of the same scan, backward.  With s = q . k scale + bias, p = exp(s - lse) (rebuilt from the forward pass's
 // sums), delta_i = sum_d do_i out_i and ds = p (do . v - delta):
 //   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i,   d table[b][h] = sum of ds over the pairs of bucket b.
-// What bounds them: issue of vector instructions, then LDS (41 157 x 5 824 x 2, 8 heads of 32, bf16, slopes: dq 1.26 ms, dk / dv 1.75 ms =
-// 0.56 and 0.54 PFLOP/s of their three and four products).
+// What bounds them: issue of vector instructions, then LDS (41 157 x 5 824 x 2, 8 heads of 32, bf16, slopes: dq 1.24 ms, dk / dv 1.79 ms =
+// 0.54 and 0.50 PFLOP/s of their three and four products; vector issue 81 and 73 %, LDS 54 and 66 %, matrix pipe 24 and 22 % of the cycles).
+// fp32 operands: neither pipe is full (7 702 x 5 824 x 2, 4 heads of 64, table: vector 50 %, matrix 34 and 42 %): 1.8 waves a SIMD wait a
+// third of their time.
+// 16-bit operands: probabilities and score gradients are rounded once, to the operands' type, before their products: gradients are off by
+// 1.4 to 1.6 times their own rounding (the last where few keys share a row and delta carries the output's rounded probabilities).
+// fp32: all tiles chain into one accumulator.  The matrix pipe's one-sided cuts show as 5e-7 of dk and dv at 41 157 queries; their error as a
+// whole is 0.8e-6 there (fp32 torch operations: 2.3e-6).
 // Two kernels that each own their outputs (queries; keys), so nothing is added by atomics and every run gives the same bits: seven products
 // per pair and channel instead of five.  delta and the gradient of the table take the UNROUNDED output of the forward pass: the rows of ds
 // sum to zero only as exactly as delta is known.
@@ -60,6 +66,7 @@ __device__ __forceinline__ void at_lift_to(float& lift, f32x4 (&ds)[N], f32x4 (&
 }
 __device__ __forceinline__ float at_unlift(float lift) { return __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, lift)); }      // 1 / 2^n, exact
 
+// (At 2 heads of 32 with the table's gradient, 16-bit: 74 to 82 registers of the 256 are spilled, of dk / dv 2 to 11.)
 // What a workgroup takes: heads at a time (the distances of a pair are the same for every head), rows of a tile.  One buffer per tile, as in
 // the forward kernel (41 157 x 5 824 x 2, bf16, dq: 1.43 against 1.69 ms).
 template <typename T, int DP> struct AtBwdPlan {

@@ -36,15 +36,17 @@ __device__ __forceinline__ void at_put_lse(const AtFwd& a, int head, int qi, flo
 
 // What a workgroup takes: QB x 16 queries a wave, HG heads, tiles of 64 keys.
 // HG: the distances of a (query, key) pair are the same for every head, so a wave takes as many heads as its registers hold.
-// What bounds it: issue of vector instructions (bf16, 4 heads of 32, slopes: some 115 a head and 64 keys, 67 % of the time busy; matrix pipe
-// 17 %, LDS 30 %).  The next head's products started ahead of this head's probabilities gave nothing (1.19 against 1.18 ms; with the table
+// What bounds it: issue of vector instructions (41 157 x 5 824 x 2, bf16, 4 heads of 32 a wave, slopes: 1.16 ms; some 115 a head and 64 keys,
+// 82 % of the cycles busy; matrix pipe 21 %, LDS 40 %).  With 16-bit operands the probabilities are rounded to their type before they meet the
+// values: the output is off by 1.3 times its own rounding.  In two pieces it would be off by that rounding alone, but a training call of that
+// size takes 5.08 ms then, not 4.51.  The next head's products started ahead of this head's probabilities gave nothing (1.19 against 1.18 ms; with the table
 // 2.0 against 1.5: a wave less): the other waves of the SIMD fill those cycles already.
 // One buffer per tile: three workgroups of a compute unit cover each other's waits better than two with a second buffer do (41 157 x 5 824
 // x 2, bf16: 1.23 against 1.48 ms).  fp32 operands are three times the LDS reads: two blocks of queries share them (0.38 against 0.42 ms
 // at 5 824 x 5 824; bf16: 1.41 against 1.23, for the registers).
 template <typename T, int DP> struct AtFwdPlan {
     static constexpr int kHeads = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 ? 2 : 1;
-    static constexpr int kExactHeads = kHeads > 2 ? 2 : kHeads;      // (the pieces take the registers of two heads: 1.63 against 1.91 ms)
+    static constexpr int kExactHeads = kHeads > 2 ? 2 : kHeads;      // (the pieces take the registers of two heads: 1.63 against 1.91 ms at 2 x 12 809^2)
     static constexpr int kQB = sizeof(T) == 4 && DP <= 64 ? 2 : 1;
 };
 constexpr int kFwdRows = 64;

@@ -16,7 +16,7 @@ constexpr int kGnBlock = 256;
 constexpr int kGnSlabs = 1024;           // workgroups of a reduction over all scans together (4 per compute unit)
 constexpr int kGnRowsPerThread = 16;     // rows a thread of the writing pass walks over, fewer where that would leave compute units idle
 
-// rows of a workgroup of the writing pass (5 824 x 256, fp32: 8.2 us with 16 rows a thread, 7.5 with one)
+// rows of a workgroup of the writing pass (5 824 x 256, fp32: 9.2 us with 16 rows a thread, 8.5 with one)
 static int gn_tile(int rows, int rpb) {
     const int n = rows / (rpb * kGnSlabs);
     return rpb * (n < 1 ? 1 : n < kGnRowsPerThread ? n : kGnRowsPerThread);

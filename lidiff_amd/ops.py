@@ -2263,7 +2263,9 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seg_q: 
     """Attention of query rows q [Mq, H, D] over the key / value rows k, v [Mk, Hkv, D] of the same scan: seg_q / seg_k [S, 2]
     (batch_segments) hold the scans' row ranges on both sides, ascending and disjoint; None, None: one scan.  Returns [Mq, H, D]; a
     query whose scan has no keys, and a row of no scan, gives zeros.  Query head h reads key head h * Hkv // H.  fp32, bf16 or fp16
-    (softmax and sums in fp32); D a multiple of 8 up to 128; scale defaults to 1 / sqrt(D).  Scores may carry a bias that depends on
+    (scores, softmax and sums in fp32; with 16-bit operands the probabilities, and in the backward pass the score gradients, are rounded once to
+    the operands' type before their matrix products; fp32 operands enter as three bf16 pieces, so an infinite one makes its products NaN);
+    D a multiple of 8 up to 128; scale defaults to 1 / sqrt(D).  Scores may carry a bias that depends on
     the distance of the two voxels (coords_q / coords_k: int32 [M, 4] = (batch, x, y, z)):
       slopes [H]            -slopes[h] * |c_i - c_j|, fixed (no gradient)
       bias [buckets, H]     a learned table: bias[b, h], b = number of `edges` (ascending whole squared distances, one less than
