@@ -548,8 +548,8 @@ int lidiff_group_norm_bwd(const void* x, const void* dy, int64_t rows, int32_t c
  * [buckets][heads], buckets <= 48; cells: the look-up table of the edges that ops.bucket_cells builds).  coords_q / coords_k: int32
  * [rows][4] = (batch, x, y, z); the batch column is not read.
  * out_f32 (unrounded copy) and lse ([2][heads][mq]: log2 of the sum of exponentials as two numbers whose sum it is; +inf and 0 without
- * keys) are kept for the backward pass; either may be NULL.  exact: with a table and 16-bit operands, out_f32 from probabilities in
- * pieces (bf16: 24 bits in three, fp16: 22 in two; for dtable).  workspace:
+ * keys) are kept for the backward pass; either may be NULL.  exact: with 16-bit operands, out and out_f32 from probabilities in
+ * pieces (two: 16 and 22 bits; with a table, for dtable, bf16 in three: 24 bits).  workspace:
  * may be NULL where workspace_bytes says 0. */
 int64_t lidiff_segment_attention_workspace_bytes(int64_t mq, int64_t mk, int64_t n_segments, int32_t heads, int32_t kv_heads,
                                                  int32_t dim, int32_t dtype, int32_t bias_mode);

@@ -21,7 +21,7 @@ struct AtFwd {
     int splits;                                               // the keys of a scan are shared out over `splits` workgroups
     void* out;                                                // [mq][heads][dim]
     float* out32;                                             // the same unrounded (for the backward pass), or null
-    int exact;                                                // probabilities in pieces: out32 is wanted to fp32 precision
+    int exact;                                                // 16-bit operands: probabilities in pieces
     float* lse;                                               // [2][heads][mq]: log2 of the sum of exponentials in two numbers, +inf and 0 for a row without keys; or null
     float *part_o, *part_ml;                                  // splits > 1: [splits][mq][heads][dim], [splits][2][heads][mq]
 };
@@ -55,8 +55,8 @@ inline int at_fwd_heads(int most, int heads, int share, int mode) {      // whol
     return mode != kNone && heads % most == 0 && (share == 1 || share % most == 0) ? most : 1;
 }
 
-// EXACT (16-bit operands, when the table's gradient is wanted): probabilities enter the product with the values in pieces, rounding and
-// rests (bf16 three: 24 bits, fp16 two: 22).  d table sums ds over millions of pairs whose rows cancel to zero through delta = do . out, so
+// EXACT (16-bit operands): probabilities enter the product with the values in pieces, rounding and rests: two where the keys are few, for the
+// table's gradient as many as carry 22 to 24 bits (bf16 three, fp16 two).  d table sums ds over millions of pairs whose rows cancel to zero through delta = do . out, so
 // the rounding of the probabilities behind out shows in it.  Of 2 x 12 809^2 pairs, bf16, against 64 bits: one piece 10^-3, two 1.2e-6,
 // three 0.8e-6, the same in fp32 torch operations 0.8e-6; two pieces take 1.67 ms, three 2.0.
 template <typename T, int DP, int HG, int SLOTS, int BIAS, int QB, bool EXACT>
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kern
                             at_here(s[n][b]);
                         }
                 }
-                constexpr int PIECES = EXACT ? AtType<T>::kPieces : 1;
+                constexpr int PIECES = !EXACT ? 1 : BIAS == kTable ? AtType<T>::kPieces : 2;
                 Frag p[QB][KB / 2][PIECES];
 #pragma unroll
                 for (int n = 0; n < QB; ++n) {
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(256) void at_join_kernel(const AtFwd a, int width, 
     if (a.out32) at_store4(a.out32 + at, r);
 }
 
-template <typename T, int DP, int HG, int SLOTS, int BIAS, bool EXACT = false>
+template <typename T, int DP, int HG, int SLOTS, int BIAS, bool EXACT>
 static hipError_t at_fwd_launch(const AtFwd& a, hipStream_t st) {
     typedef AtFwdPlan<T, DP> Plan;
     constexpr int QB = Plan::kQB;
@@ -368,11 +368,11 @@ static hipError_t at_fwd_launch(const AtFwd& a, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <typename T, int DP, int HG, int SLOTS>
+template <typename T, int DP, int HG, int SLOTS, bool EXACT = false>
 static hipError_t at_fwd_bias(const AtFwd& a, int mode, hipStream_t st) {
-    if (mode == kTable) return at_fwd_launch<T, DP, HG, SLOTS, kTable>(a, st);
-    if (mode == kSlope) return at_fwd_launch<T, DP, HG, SLOTS, kSlope>(a, st);
-    if constexpr (HG == 1) return at_fwd_launch<T, DP, HG, SLOTS, kNone>(a, st);
+    if (mode == kTable) return at_fwd_launch<T, DP, HG, SLOTS, kTable, EXACT>(a, st);
+    if (mode == kSlope) return at_fwd_launch<T, DP, HG, SLOTS, kSlope, EXACT>(a, st);
+    if constexpr (HG == 1) return at_fwd_launch<T, DP, HG, SLOTS, kNone, EXACT>(a, st);
     return hipErrorInvalidValue;
 }
 
@@ -380,11 +380,11 @@ template <typename T, int DP>
 static hipError_t at_fwd_width(const AtFwd& a, int mode, hipStream_t st) {
     constexpr int most = AtFwdPlan<T, DP>::kHeads, exact = AtFwdPlan<T, DP>::kExactHeads;
     if constexpr (sizeof(T) == 2) {
-        if (mode == kTable && a.exact) {
+        if (a.exact) {
             if constexpr (exact > 1)
                 if (at_fwd_heads(exact, a.heads, a.share, mode) == exact)
-                    return a.share > 1 ? at_fwd_launch<T, DP, exact, 1, kTable, true>(a, st) : at_fwd_launch<T, DP, exact, exact, kTable, true>(a, st);
-            return at_fwd_launch<T, DP, 1, 1, kTable, true>(a, st);
+                    return a.share > 1 ? at_fwd_bias<T, DP, exact, 1, true>(a, mode, st) : at_fwd_bias<T, DP, exact, exact, true>(a, mode, st);
+            return at_fwd_bias<T, DP, 1, 1, true>(a, mode, st);
         }
     }
     if constexpr (most > 1)

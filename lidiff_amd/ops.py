@@ -1998,6 +1998,10 @@ _ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2}
 _BIAS_NONE, _BIAS_SLOPES, _BIAS_TABLE = 0, 1, 2
 MAX_BUCKETS = 48
+# Keys of an average scan up to which 16-bit probabilities enter their product in two pieces: one tile of keys, where that costs nothing (2 x 20 000
+# queries, 8 heads of 32, bf16, slopes: training 139 us either way with 64 keys, 192 : 203 with 256, 443 : 487 with 1 024), and where the roundings
+# of few probabilities would not average out of do . out (dq off by 1.6 times its own rounding, else 1.4 to 1.5).
+SHORT_KEYS = 64
 _ON_CURRENT = contextlib.nullcontext()
 
 
@@ -2218,12 +2222,13 @@ class _SegmentAttention(torch.autograd.Function):
         out32 = None if not grads else out if q.dtype == torch.float32 else torch.empty((mq, heads, dim), dtype=torch.float32, device=dev)
         lse = torch.empty((2, heads, mq), dtype=torch.float32, device=dev) if grads else None
         if mq:
+            exact = (grads and table is not None and ctx.needs_input_grad[3]) or (mk <= SHORT_KEYS * n_seg and (grads or table is None))
             nbytes = _lib.load().lidiff_segment_attention_workspace_bytes(mq, mk, n_seg, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], mode)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
             call("lidiff_segment_attention", ptr(q), ptr(k), ptr(v), _strides(q, k, v), ptr(coords_q), ptr(coords_k), ptr(seg_q), ptr(seg_k),
                  n_seg, mq, mk, heads, kv_heads, dim, _ROW_DTYPES[q.dtype], float(scale), mode, ptr(slopes), ptr(tab), ptr(cells),
                  0 if table is None else table.shape[0], ptr(out), ptr(out32) if out32 is not out else None,
-                 int(grads and table is not None and ctx.needs_input_grad[3]), ptr(lse), ptr(ws), _stream_of(dev))
+                 int(exact), ptr(lse), ptr(ws), _stream_of(dev))
         if grads:
             ctx.save_for_backward(q, k, v, table, seg_q, seg_k, coords_q, coords_k, slopes, out32, lse)
             ctx.edges, ctx.scale, ctx.mode = edges, scale, mode
@@ -2263,8 +2268,8 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seg_q: 
     """Attention of query rows q [Mq, H, D] over the key / value rows k, v [Mk, Hkv, D] of the same scan: seg_q / seg_k [S, 2]
     (batch_segments) hold the scans' row ranges on both sides, ascending and disjoint; None, None: one scan.  Returns [Mq, H, D]; a
     query whose scan has no keys, and a row of no scan, gives zeros.  Query head h reads key head h * Hkv // H.  fp32, bf16 or fp16
-    (scores, softmax and sums in fp32; with 16-bit operands the probabilities, and in the backward pass the score gradients, are rounded once to
-    the operands' type before their matrix products; fp32 operands enter as three bf16 pieces, so an infinite one makes its products NaN);
+    (scores, softmax and sums in fp32; with 16-bit operands the probabilities -- but for few keys -- and in the backward pass the score gradients are
+    rounded once to the operands' type before their matrix products; fp32 operands enter as three bf16 pieces, so an infinite one makes its products NaN);
     D a multiple of 8 up to 128; scale defaults to 1 / sqrt(D).  Scores may carry a bias that depends on
     the distance of the two voxels (coords_q / coords_k: int32 [M, 4] = (batch, x, y, z)):
       slopes [H]            -slopes[h] * |c_i - c_j|, fixed (no gradient)

@@ -235,3 +235,35 @@ def test_offsets_beyond_32_bits(ops):
         outs.append((out.detach(),) + torch.autograd.grad(out, leaves, go))
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("bias", ["none", "slopes", 16])
+def test_few_keys_are_weighted_with_more_than_the_operands_bits(ops, dtype, bias):
+    """Up to a tile of keys a scan, 16-bit operands: the output is off by its own rounding (and 2^-15 of the weighted values' sizes: two pieces of
+    bf16 hold 16 bits), dq and dk by the score gradients' rounding and their own -- do . out brings none of the probabilities'."""
+    gen = generator(39)
+    heads, lens_q, lens_k = 4, [150, 12, 1, 60], [2, 64, 3, 0]
+    seg_q, seg_k = ranges(lens_q), ranges(lens_k)
+    mq, mk = sum(lens_q), sum(lens_k)
+    q, k, v, go = (rand(gen, n, heads, 32, dtype=dtype) for n in (mq, mk, mk, mq))
+    kw = {} if bias == "none" else dict(coords_q=voxel_rows(gen, mq), coords_k=voxel_rows(gen, mk))
+    if bias == "slopes":
+        kw["slopes"] = torch.full((heads,), 0.01, device="cuda")
+    elif bias != "none":
+        kw.update(bias=rand(gen, bias, heads), edges=edges_of(ops, bias))
+    got = attend(ops, q, k, v, go, seg_q.cuda(), seg_k.cuda(), **kw)
+    names = {"coords_q": "cq", "coords_k": "ck"}
+    # the 64-bit form on fp32 copies of the operands: its bounds then count no rounding of probabilities or score gradients
+    val, bnd = attention_ref(q.float(), k.float(), v.float(), seg_q, seg_k, go=go.float(), **{names.get(n, n): t for n, t in kw.items()})
+    u = torch.finfo(dtype).eps / 2
+    size = torch.zeros_like(val["out"])
+    for (q0, q1), (k0, k1) in zip(seg_q.tolist(), seg_k.tolist()):
+        if k1 > k0:
+            size[q0:q1] = v[k0:k1].double().abs().amax(0)
+    assert_within(got[0], val["out"], bnd["out"] + 2.0 ** -15 * size + u * (val["out"].abs() + size * 2.0 ** -14), TINY[dtype], "out")
+    for name, g in (("dq", got[1]), ("dk", got[2]), ("dv", got[3])):
+        # (2-norms: independent roundings of the terms, of the sums, of the result: root of two half steps' mean squares, u / sqrt(3) each at
+        # most, a fifth on top for the few terms there are)
+        off = (g.double() - val[name]).norm() / val[name].norm()
+        assert off <= 1.2 * math.sqrt(2 / 3) * u + 1e-5, (name, off.item() / u)
