@@ -136,7 +136,9 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
         return;
     }
     const int2 kr = t.seg >= 0 ? seg_range(a.seg_k, t.seg, a.mk) : make_int2(0, 0);
-    const int k_lo = __builtin_amdgcn_readfirstlane(kr.x), k_hi = __builtin_amdgcn_readfirstlane(kr.y), last = (k_hi - k_lo + ROWS - 1) / ROWS;
+    const int k_lo = __builtin_amdgcn_readfirstlane(kr.x), k_hi = __builtin_amdgcn_readfirstlane(kr.y);
+    // (one key: its probability is 1 whatever its score is, so there are no score gradients -- do . v less do . out would be their roundings)
+    const int last = k_hi - k_lo == 1 ? 0 : (k_hi - k_lo + ROWS - 1) / ROWS;
     const int q0 = t.lo + wave * 16 * QB;
     const float scale2 = a.scale * kLog2e;
 
@@ -548,6 +550,14 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
         }
     }
     if (!have) return;
+    if (t.hi - t.lo == 1 && t.seg >= 0) {                      // (a lone key has no score gradients, as above)
+        const int2 own = seg_range(a.seg_k, t.seg, a.mk);
+        if (own.y - own.x == 1)
+#pragma unroll
+            for (int h = 0; h < SLOTS; ++h)
+#pragma unroll
+                for (int b = 0; b < DB; ++b) dk[h][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 #pragma unroll
     for (int h = 0; h < SLOTS; ++h) {
         // (p, and with it ds, carries kLift already)

@@ -267,3 +267,27 @@ def test_few_keys_are_weighted_with_more_than_the_operands_bits(ops, dtype, bias
         # most, a fifth on top for the few terms there are)
         off = (g.double() - val[name]).norm() / val[name].norm()
         assert off <= 1.2 * math.sqrt(2 / 3) * u + 1e-5, (name, off.item() / u)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("bias", ["none", "slopes", 16])
+def test_a_lone_key_has_no_score_gradients(ops, dtype, bias):
+    """Scans of one key: its probability is 1, so the output is its value and dq, dk and the table's gradient are zero, not roundings."""
+    gen = generator(40)
+    lens_q, lens_k = [200, 3, 0, 1, 70], [1, 1, 1, 1, 5]
+    seg_q, seg_k = ranges(lens_q, [2, 0, 0, 0, 1]), ranges(lens_k, [1, 0, 3, 0, 0])
+    mq, mk = int(seg_q[-1, 1]), int(seg_k[-1, 1])
+    q, k, v, go = (rand(gen, n, h, 32, dtype=dtype) for n, h in ((mq, 4), (mk, 2), (mk, 2), (mq, 4)))
+    kw = {} if bias == "none" else dict(coords_q=voxel_rows(gen, mq), coords_k=voxel_rows(gen, mk))
+    if bias == "slopes":
+        kw["slopes"] = torch.full((4,), 0.01, device="cuda")
+    elif bias != "none":
+        kw.update(bias=rand(gen, bias, 4), edges=edges_of(ops, bias))
+    got = attend(ops, q, k, v, go, seg_q.cuda(), seg_k.cuda(), **kw)
+    val, bnd = attention_ref(q, k, v, seg_q, seg_k, go=go, **{{"coords_q": "cq", "coords_k": "ck"}.get(n, n): t for n, t in kw.items()})
+    for name, g in zip(("out", "dq", "dk", "dv", "dt"), got):
+        assert_within(g, val[name], bnd[name], 1e-30 if name == "dt" else TINY[dtype], name)
+    assert (got[1][:int(seg_q[3, 1])] == 0).all() and (got[2][:int(seg_k[3, 1])] == 0).all()
+    if bias == 16:
+        one = attend(ops, q[:200], k[:1], v[:1], go[:200], **{n: t[:200 if n == "coords_q" else 1] if n[:6] == "coords" else t for n, t in kw.items()})
+        assert (one[4] == 0).all()
