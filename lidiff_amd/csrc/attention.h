@@ -65,6 +65,16 @@ __device__ __forceinline__ void at_mma_apart(f32x4& acc, const AtPieces& a, cons
     acc += part;
 }
 
+// sums over the rows of a scan: fp32 operands have every 32 rows summed by themselves, so that the cuts do not add up along the chain; with
+// 16-bit operands they are far below the operands' rounding
+template <typename F>
+__device__ __forceinline__ void at_mma_rows(f32x4& acc, const F& a, const F& b) { at_mma(acc, a, b); }
+__device__ __forceinline__ void at_mma_rows(f32x4& acc, const AtPieces& a, const AtPieces& b) {
+    f32x4 part = {0.f, 0.f, 0.f, 0.f};
+    at_mma(part, a, b);
+    acc += part;
+}
+
 // the operand with its signs turned where `mask` is 0x80008000
 __device__ __forceinline__ void at_turn(bf16x8& f, uint32_t mask) { f = __builtin_bit_cast(bf16x8, __builtin_bit_cast(at_words, f) ^ mask); }
 __device__ __forceinline__ void at_turn(f16x8& f, uint32_t mask) { f = __builtin_bit_cast(f16x8, __builtin_bit_cast(at_words, f) ^ mask); }

@@ -7,8 +7,6 @@
 // third of their time.
 // 16-bit operands: probabilities and score gradients are rounded once, to the operands' type, before their products: gradients are off by
 // 1.4 to 1.6 times their own rounding (the last where few keys share a row and delta carries the output's rounded probabilities).
-// fp32: all tiles chain into one accumulator.  The matrix pipe's one-sided cuts show as 5e-7 of dk and dv at 41 157 queries; their error as a
-// whole is 0.8e-6 there (fp32 torch operations: 2.3e-6).
 // Two kernels that each own their outputs (queries; keys), so nothing is added by atomics and every run gives the same bits: seven products
 // per pair and channel instead of five.  delta and the gradient of the table take the UNROUNDED output of the forward pass: the rows of ds
 // sum to zero only as exactly as delta is known.
@@ -339,7 +337,7 @@ __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_bwd_q_ke
                     for (int b = 0; b < DB; ++b) {
                         const Frag kf = Tile::frag_turned(ks, place, slot, j, b);
 #pragma unroll
-                        for (int n = 0; n < QB; ++n) at_mma(dq[n][h][b], kf, p[n]);
+                        for (int n = 0; n < QB; ++n) at_mma_rows(dq[n][h][b], kf, p[n]);
                     }
                 }
                 if (GRAD) {
@@ -537,8 +535,8 @@ __global__ __launch_bounds__(kAtBlock, (AtBwdPlan<T, DP>::kKeyWaves)) void at_bw
                         at_pack(ds, at_join(dp[0], dp[1]));
 #pragma unroll
                         for (int b = 0; b < DB; ++b) {
-                            at_mma(dv[slot][b], Tile::frag_turned(gs, place, h, j, b), p);
-                            at_mma(dk[slot][b], Tile::frag_turned(qs, place, h, j, b), ds);
+                            at_mma_rows(dv[slot][b], Tile::frag_turned(gs, place, h, j, b), p);
+                            at_mma_rows(dk[slot][b], Tile::frag_turned(qs, place, h, j, b), ds);
                         }
                     }
                 }

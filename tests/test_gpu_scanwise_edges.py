@@ -291,3 +291,27 @@ def test_a_lone_key_has_no_score_gradients(ops, dtype, bias):
     if bias == 16:
         one = attend(ops, q[:200], k[:1], v[:1], go[:200], **{n: t[:200 if n == "coords_q" else 1] if n[:6] == "coords" else t for n, t in kw.items()})
         assert (one[4] == 0).all()
+
+
+@pytest.mark.parametrize("nq,nk,heads,kv_heads,dim", [(1, 8893, 2, 2, 128), (320, 6816, 4, 1, 64), (20000, 1500, 2, 2, 32)])
+def test_fp32_gradients_of_long_sums(ops, nq, nk, heads, kv_heads, dim):
+    """fp32 sums over thousands of rows: no further from 64 bits than the same formulas in fp32 torch operations (5 / 4 of their error), whose sums
+    are pairwise -- the matrix pipe's one-sided cuts must not add up along a scan."""
+    gen = generator(41)
+    q, k, v, go = rand(gen, nq, heads, dim), rand(gen, nk, kv_heads, dim), rand(gen, nk, kv_heads, dim), rand(gen, nq, heads, dim)
+    got = attend(ops, q, k, v, go)
+    def formulas(dtype):
+        res = [torch.zeros(t.shape, dtype=dtype, device="cuda") for t in (q, q, k, v)]
+        for h in range(heads):
+            Q, K, V, G = (t.to(dtype)[:, i].contiguous() for t, i in ((q, h), (k, h * kv_heads // heads), (v, h * kv_heads // heads), (go, h)))
+            p = torch.softmax(Q @ K.T.contiguous() / math.sqrt(dim), 1)
+            out = p @ V
+            ds = p * (G @ V.T.contiguous() - (G * out).sum(1, keepdim=True))
+            res[0][:, h], res[1][:, h] = out, ds @ K / math.sqrt(dim)
+            res[2][:, h * kv_heads // heads] += ds.T.contiguous() @ Q / math.sqrt(dim)
+            res[3][:, h * kv_heads // heads] += p.T.contiguous() @ G
+        return res
+    for name, mine, exact, plain in zip(("out", "dq", "dk", "dv"), got, formulas(torch.float64), formulas(F32)):
+        off, other = ((t.double() - exact).norm().item() for t in (mine, plain))
+        # (12 half steps of the result: six products with a cut each, scores and exponentials of a few half steps each; below that both are as good)
+        assert off <= max(1.25 * other, 12 * U32 * exact.norm().item()), (name, off / exact.norm().item(), other / exact.norm().item())
