@@ -1,9 +1,9 @@
 // Attention between the rows of the same scan, backward.  With s = q . k scale + bias, p = exp(s - lse) (rebuilt from the forward pass's
 // sums), delta_i = sum_d do_i out_i and ds = p (do . v - delta):
 //   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i,   d table[b][h] = sum of ds over the pairs of bucket b.
-// What bounds them: issue of vector instructions, then LDS (41 157 x 5 824 x 2, 8 heads of 32, bf16, slopes: dq 1.24 ms, dk / dv 1.79 ms =
-// 0.54 and 0.50 PFLOP/s of their three and four products; vector issue 81 and 73 %, LDS 54 and 66 %, matrix pipe 24 and 22 % of the cycles).
-// fp32 operands: neither pipe is full (7 702 x 5 824 x 2, 4 heads of 64, table: vector 50 %, matrix 34 and 42 %): 1.8 waves a SIMD wait a
+// What bounds them: issue of vector instructions, then LDS (41 157 x 5 824 x 2, 8 heads of 32, bf16, slopes: dq 1.23 ms, dk / dv 1.80 ms =
+// 0.58 and 0.53 PFLOP/s of their three and four products; vector issue 81 and 72 %, LDS 54 and 65 %, matrix pipe 24 and 22 % of the cycles).
+// fp32 operands: neither pipe is full (7 702 x 5 824 x 2, 4 heads of 64, table: vector 52 %, matrix 33 and 40 %): 1.8 waves a SIMD wait a
 // third of their time.
 // 16-bit operands: probabilities and score gradients are rounded once, to the operands' type, before their products: gradients are off by
 // 1.4 to 1.6 times their own rounding (the last where few keys share a row and delta carries the output's rounded probabilities).

@@ -36,11 +36,11 @@ __device__ __forceinline__ void at_put_lse(const AtFwd& a, int head, int qi, flo
 
 // What a workgroup takes: QB x 16 queries a wave, HG heads, tiles of 64 keys.
 // HG: the distances of a (query, key) pair are the same for every head, so a wave takes as many heads as its registers hold.
-// What bounds it: issue of vector instructions (41 157 x 5 824 x 2, bf16, 4 heads of 32 a wave, slopes: 1.16 ms; some 115 a head and 64 keys,
+// What bounds it: issue of vector instructions (41 157 x 5 824 x 2, bf16, 4 heads of 32 a wave, slopes: 1.15 ms; some 115 a head and 64 keys,
 // 82 % of the cycles busy; matrix pipe 21 %, LDS 40 %).  With 16-bit operands the probabilities are rounded to their type before they meet the
 // values: the output is off by 1.3 times its own rounding.  In two pieces it would be off by that rounding alone, but a training call of that
-// size takes 5.08 ms then, not 4.51.  The next head's products started ahead of this head's probabilities gave nothing (1.19 against 1.18 ms; with the table
-// 2.0 against 1.5: a wave less): the other waves of the SIMD fill those cycles already.
+// size takes 5.08 ms then, not 4.51.  The next head's products started ahead of this head's probabilities gave nothing (1.19 against 1.18 ms;
+// with the table 2.0 against 1.5: a wave less): the other waves of the SIMD fill those cycles already.
 // One buffer per tile: three workgroups of a compute unit cover each other's waits better than two with a second buffer do (41 157 x 5 824
 // x 2, bf16: 1.23 against 1.48 ms).  fp32 operands are three times the LDS reads: two blocks of queries share them (0.38 against 0.42 ms
 // at 5 824 x 5 824; bf16: 1.41 against 1.23, for the registers).
@@ -56,9 +56,9 @@ inline int at_fwd_heads(int most, int heads, int share, int mode) {      // whol
 }
 
 // EXACT (16-bit operands): probabilities enter the product with the values in pieces, rounding and rests: two where the keys are few, for the
-// table's gradient as many as carry 22 to 24 bits (bf16 three, fp16 two).  d table sums ds over millions of pairs whose rows cancel to zero through delta = do . out, so
-// the rounding of the probabilities behind out shows in it.  Of 2 x 12 809^2 pairs, bf16, against 64 bits: one piece 10^-3, two 1.2e-6,
-// three 0.8e-6, the same in fp32 torch operations 0.8e-6; two pieces take 1.67 ms, three 2.0.
+// table's gradient as many as carry 22 to 24 bits (bf16 three, fp16 two).  d table sums ds over millions of pairs whose rows cancel to zero
+// through delta = do . out, so the rounding of the probabilities behind out shows in it.  Of 2 x 12 809^2 pairs, bf16, against 64 bits: one
+// piece 10^-3, two 1.2e-6, three 0.8e-6, the same in fp32 torch operations 0.8e-6; two pieces take 1.67 ms, three 2.0.
 template <typename T, int DP, int HG, int SLOTS, int BIAS, int QB, bool EXACT>
 __global__ __launch_bounds__(kAtBlock, at_waves(sizeof(T), DP)) void at_fwd_kernel(const AtFwd a) {
     constexpr int ROWS = kFwdRows, DC = DP / 32, DB = DP / 16, KB = ROWS / 16;
